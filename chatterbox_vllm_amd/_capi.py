@@ -67,6 +67,32 @@ class T3GemmDesc(C.Structure):
     ]
 
 
+class T3Kv4Cache(C.Structure):
+    _fields_ = [
+        ("pool_dev", C.c_void_p), ("block_table_dev", C.c_void_p), ("layer_stride", C.c_int64),
+        ("n_layers", C.c_int32), ("n_pages", C.c_int32), ("n_streams", C.c_int32), ("max_pages", C.c_int32),
+        ("Hkv", C.c_int32), ("hd", C.c_int32),
+    ]
+
+
+class T3Kv4Batch(C.Structure):
+    _fields_ = [
+        ("seq_start_dev", C.c_void_p), ("stream_dev", C.c_void_p), ("ctx_dev", C.c_void_p),
+        ("n_seqs", C.c_int32), ("rows", C.c_int32), ("max_rows", C.c_int32), ("max_ctx", C.c_int32),
+    ]
+
+
+class T3Kv4EvictDesc(C.Structure):
+    _fields_ = [
+        ("src_dev", C.c_void_p), ("dst_dev", C.c_void_p), ("ctx_dev", C.c_void_p), ("weights_dev", C.c_void_p),
+        ("weights_stride", C.c_int64), ("new_ctx_dev", C.c_void_p), ("kept_dev", C.c_void_p),
+        ("n", C.c_int32), ("max_ctx", C.c_int32), ("keep", C.c_int32), ("sink", C.c_int32), ("recent", C.c_int32),
+        ("layer", C.c_int32), ("n_layers", C.c_int32),
+    ]
+
+
+_KV4 = [C.POINTER(T3Kv4Cache), C.POINTER(T3Kv4Batch)]
+
 # name -> (argtypes, restype); every symbol include/t3_hip.h declares
 SIGNATURES = {
     "t3_last_error": ([], C.c_char_p),
@@ -131,6 +157,13 @@ SIGNATURES = {
                                    C.c_int32, _P], C.c_int),
     "t3_op_sample_greedy": ([_P, C.c_int32, C.c_int32, _P, _P, C.c_int32, C.c_float, _P, _P, C.c_int32, _P, _P, _P],
                             C.c_int),
+    "t3_op_kv4_page_bytes": ([C.c_int32, C.c_int32], C.c_int64),
+    "t3_op_kv4_append": (_KV4 + [_P, _P, C.c_int64, C.c_int64, C.c_int32, C.c_int32, _P], C.c_int),
+    "t3_op_kv4_read": (_KV4 + [_P, _P, C.c_int32, C.c_int32, C.c_int32, _P], C.c_int),
+    "t3_op_attn_kv4_work_bytes": (_KV4 + [C.c_int32, C.c_int32], C.c_int64),
+    "t3_op_attn_kv4": (_KV4 + [_P, C.c_int64, _P, C.c_int64, C.c_int32, C.c_int32, C.c_float, _P, C.c_int64, _P, C.c_int64,
+                               C.c_int32, _P], C.c_int),
+    "t3_op_kv4_evict": ([C.POINTER(T3Kv4Cache), C.POINTER(T3Kv4EvictDesc), _P], C.c_int),
 }
 
 

@@ -342,6 +342,79 @@ int t3_op_sample_greedy(const void* logits_dev, int32_t ldl, int32_t vocab, cons
                         uint8_t* seen_dev, int32_t seen_stride, int32_t* out_tokens_dev,
                         float* out_logits_dev, void* stream);
 
+/* ---- 4-bit KV cache: append, attention, eviction, read ------------------------------------------------------
+ * A paged cache in 4.25 bits a value beside the engine's bf16 pool: 128 bytes of a (token, head) at head_dim 64 become 34.
+ * It has no counterpart in the reference, whose cache is vLLM's in the model's type (tts.py:130-140).
+ *
+ * Values: e2m1 codes (0, .5, 1, 1.5, 2, 3, 4, 6 and a sign); 32 consecutive dims of one (token, head) share a power of two,
+ * the smallest that leaves the largest of them below 7 (so none is cut by more than half a step).  Both are exact in bf16.
+ * Powers below 2^-125 and above 2^125 are not used: smaller values become 0, larger ones 6 * 2^125.  An entry (token, head)
+ * with a NaN or an infinity among its K or V values is kept as a NaN entry: a row that attends to it gets NaN for that head.
+ *
+ * Layout: pool[layer][page][kv head][t3_op_kv4_page_bytes(1, hd) bytes], pages of 64 tokens of one stream, named by the
+ * block table [n_streams][max_pages] as in the bf16 pool.  Byte order: csrc/kv4_layout.h. */
+typedef struct t3_kv4_cache {
+    void* pool_dev;                   /* 16-byte aligned                                                              */
+    const int32_t* block_table_dev;   /* [n_streams][max_pages] page ids                                              */
+    int64_t layer_stride;             /* bytes from one layer's pages to the next one's, a multiple of 16             */
+    int32_t n_layers, n_pages, n_streams, max_pages;
+    int32_t Hkv, hd;                  /* key/value heads (1..1024); head_dim 64 or 128                                */
+} t3_kv4_cache;
+/* The batch that append, attention and read share: sequence i owns rows [seq_start[i], seq_start[i+1]) of the row tensors
+ * (prompt rows, drafted tokens, or one row for a decode step), which are the entries ctx[i] - n_i .. ctx[i] - 1 of its stream:
+ * ctx counts the entries of the stream AFTER the rows are appended.  A stream may occur in one sequence of a call to append.
+ * stream < 0: the sequence is skipped, its rows are left as they were.  Rows before entry 0 (n_i > ctx[i]) are not stored and
+ * attend to nothing (output 0).  Numbers that do not fit (stream >= n_streams, ctx beyond max_ctx or the block table, rows
+ * beyond `rows` or more than max_rows of them, page ids outside the pool) never lead outside a buffer: nothing is stored for
+ * them, and their rows' outputs (the first max_rows of them) are NaN. */
+typedef struct t3_kv4_batch {
+    const int32_t* seq_start_dev;     /* [n_seqs + 1], ascending; rows behind the last one are left as they were      */
+    const int32_t* stream_dev;        /* [n_seqs]                                                                     */
+    const int32_t* ctx_dev;           /* [n_seqs]                                                                     */
+    int32_t n_seqs, rows;             /* rows: rows that the row tensors have                                         */
+    int32_t max_rows;                 /* no sequence has more rows                                                    */
+    int32_t max_ctx;                  /* no sequence has more entries                                                 */
+} t3_kv4_batch;
+int64_t t3_op_kv4_page_bytes(int32_t Hkv, int32_t hd);       /* bytes of one page; 0: geometry not supported */
+/* K and V rows -> cache.  k_dev / v_dev: row r at k_dev + r * k_stride elements, [Hkv][hd] inside it (a view of the q|k|v
+ * buffer will do); 16-byte aligned, strides multiples of 8.  dtype 0: bf16, 1: fp16. */
+int t3_op_kv4_append(const t3_kv4_cache* cache, const t3_kv4_batch* batch, const void* k_dev, const void* v_dev,
+                     int64_t k_stride, int64_t v_stride, int32_t dtype, int32_t layer, void* stream);
+/* cache -> K and V rows, the values the codes stand for (exact in bf16; in fp16 rounded, and cut at its largest value), of
+ * layers [layer, layer + n_layers): k_dev, v_dev [n_layers][rows][Hkv][hd], contiguous, 16-byte aligned. */
+int t3_op_kv4_read(const t3_kv4_cache* cache, const t3_kv4_batch* batch, void* k_dev, void* v_dev, int32_t dtype,
+                   int32_t layer, int32_t n_layers, void* stream);
+/* Attention of the batch's rows over the cache: row j of n of a sequence sees its first ctx - n + j + 1 entries (causal).
+ * q_dev: row r at q_dev + r * q_stride elements, [H][hd] inside it, H = group * Hkv, group 1..64 query heads per key head; out
+ * likewise.  A row that sees nothing gets 0.  scale > 0 multiplies the scores.
+ * weights_dev (optional): [n_streams][Hkv][weights_stride] fp32; every entry's softmax weights, summed over the call's rows and
+ * over the query heads of its key head, are added to it (in a fixed order: equal calls give equal bits).  weights_stride >=
+ * max_ctx.  A refused sequence adds nothing.
+ * work_dev: t3_op_attn_kv4_work_bytes() bytes, 16-byte aligned, for this call alone while it runs: calls that may overlap
+ * (streams, replayed graphs) need one each.  It need not be cleared.
+ * A row's bits depend on its sequence alone, not on what else is in the call. */
+int64_t t3_op_attn_kv4_work_bytes(const t3_kv4_cache* cache, const t3_kv4_batch* batch, int32_t H, int32_t with_weights);
+int t3_op_attn_kv4(const t3_kv4_cache* cache, const t3_kv4_batch* batch, const void* q_dev, int64_t q_stride, void* out_dev,
+                   int64_t out_stride, int32_t H, int32_t dtype, float scale, float* weights_dev, int64_t weights_stride,
+                   void* work_dev, int64_t work_bytes, int32_t layer, void* stream);
+/* Shortens streams to their most attended entries.  Entry i moves stream src[i] (ctx[i] entries) into the pages of stream
+ * dst[i], for every layer of [layer, layer + n_layers) and every key head by that head's own weights: the first `sink` and the
+ * last `recent` entries stay, and of the others the heaviest, `keep` in all (equal weights: the earlier entry; NaN counts as the
+ * lowest).  min(ctx, keep) entries remain, in their old order; their weights move along and the rest of dst's weights row is
+ * cleared.  src is left as it was: its pages are the caller's to free (or to keep, where another stream shares them).
+ * weights_dev [n_layers][n_streams][Hkv][weights_stride] fp32, new_ctx_dev [n], kept_dev [n_layers][n][Hkv][keep] (old entry of
+ * each new one, ascending, -1 behind the last).  sink + recent <= keep <= weights_stride, max_ctx <= weights_stride.
+ * Refused with new_ctx = -1 (nothing moved, kept -1): streams or page ids out of range, ctx < 0 or > max_ctx, a page of dst that
+ * is also a page of src, a dst that an earlier entry has too or that any entry has as src. */
+typedef struct t3_kv4_evict_desc {
+    const int32_t* src_dev; const int32_t* dst_dev; const int32_t* ctx_dev;   /* [n]                                  */
+    float* weights_dev; int64_t weights_stride;
+    int32_t* new_ctx_dev; int32_t* kept_dev;
+    int32_t n, max_ctx, keep, sink, recent;
+    int32_t layer, n_layers;
+} t3_kv4_evict_desc;
+int t3_op_kv4_evict(const t3_kv4_cache* cache, const t3_kv4_evict_desc* desc, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

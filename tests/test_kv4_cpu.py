@@ -1,0 +1,223 @@
+"""4-bit KV cache without a GPU: the byte order and the bounds arithmetic of csrc/kv4_layout.h compiled for the host, and the
+refusals of the C entry points, which come before any GPU call."""
+import ctypes as C
+import os
+import re
+import subprocess
+
+import pytest
+import torch
+
+import _kv4
+from chatterbox_vllm_amd import _capi
+
+ROOT = os.path.abspath(os.path.join(os.path.dirname(__file__), ".."))
+CSRC = os.path.join(ROOT, "chatterbox_vllm_amd", "csrc")
+
+PROGRAM = r"""
+#include "kv4_layout.h"
+#include <stdio.h>
+#include <stdlib.h>
+#include <string.h>
+#define REQUIRE(x) do { if (!(x)) { printf("line %d: %s\n", __LINE__, #x); return 1; } } while (0)
+int main() {
+    for (int hd = 64; hd <= 128; hd *= 2) {                      // every code and scale has a place of its own, none outside
+        const int bytes = kv4_slab_bytes(hd);
+        char* used = (char*)calloc(bytes, 1);
+        for (int t = 0; t < 64; ++t)
+            for (int d = 0; d < hd; ++d) {
+                const int at[2] = {kv4_k_at(hd, t, d), kv4_v_at(hd, t, d)};
+                for (int i = 0; i < 2; ++i) {
+                    REQUIRE(at[i] >= i * 32 * hd && at[i] < (i + 1) * 32 * hd);
+                    REQUIRE(!(used[at[i]] & (1 << d % 2)));
+                    used[at[i]] |= 1 << d % 2;
+                }
+                if (d % 32 == 0) {
+                    const int sc[2] = {kv4_ks_at(hd, t, d), kv4_vs_at(hd, t, d)};
+                    for (int i = 0; i < 2; ++i) { REQUIRE(sc[i] >= 64 * hd && sc[i] < bytes && !used[sc[i]]); used[sc[i]] = 3; }
+                }
+                printf("%d %d %d %d %d %d\n", hd, t, d, at[0], at[1], kv4_ks_at(hd, t, d));
+            }
+        for (int i = 0; i < bytes; ++i) REQUIRE(used[i] == 3);
+        // pieces that are moved as one word: 8 K dims in 4 bytes, 4 V dims of 8 tokens in 16
+        for (int t = 0; t < 64; ++t)
+            for (int d = 0; d < hd; d += 8) {
+                REQUIRE(kv4_k_at(hd, t, d) % 4 == 0 && kv4_k_at(hd, t, d + 7) == kv4_k_at(hd, t, d) + 3);
+                REQUIRE(kv4_v_at(hd, t / 8 * 8, d) % 16 == 0 && kv4_v_at(hd, t, d) == kv4_v_at(hd, t / 8 * 8, d) + 2 * (t % 8));
+                REQUIRE(kv4_v_at(hd, t, d + 3) == kv4_v_at(hd, t, d) + 1);
+            }
+        for (int t = 0; t < 64; ++t)
+            for (int d = 0; d < hd; d += hd / 4) REQUIRE(kv4_k_at(hd, t, d) % (hd / 8) == 0 && kv4_k_at(hd, t, d + hd / 4 - 1) == kv4_k_at(hd, t, d) + hd / 8 - 1);
+        free(used);
+    }
+    const int v[] = {-2147483647 - 1, -5, -1, 0, 1, 2, 3, 4, 5, 6, 7, 64, 2147483647};
+    const int n = sizeof(v) / sizeof(v[0]);
+    for (int a = 0; a < n; ++a) for (int b = 0; b < n; ++b) for (int s = 0; s < n; ++s) for (int c = 0; c < n; ++c)
+        for (int rows = 1; rows < 7; rows += 2) for (int most = 1; most <= rows; ++most) {
+            const Kv4Seq q = kv4_seq(v[a], v[b], v[s], v[c], rows, most, 4, 64);
+            REQUIRE(q.start >= 0 && q.n >= 0 && q.start + q.n <= rows);
+            if (q.state == 0) REQUIRE(q.start == v[a] && q.n == v[b] - v[a] && q.n >= 1 && q.n <= most && v[s] >= 0 && v[s] < 4 && v[c] >= 0 && v[c] <= 64);
+            if (v[s] < 0) REQUIRE(q.state == 1);
+            if (q.n == 0) REQUIRE(q.state == 1);
+            if (v[s] >= 0 && v[a] >= 0 && v[b] > v[a] && v[b] <= rows && v[b] - v[a] <= most && v[s] < 4 && v[c] >= 0 && v[c] <= 64) REQUIRE(q.state == 0);
+        }
+    for (int a = 0; a < n; ++a) REQUIRE(kv4_page_ok(v[a], 5) == (v[a] >= 0 && v[a] < 5));
+    float last = 0.f;
+    for (unsigned bits = 0; bits < 0x7f800000u; bits += 977) {   // the smallest power of two that leaves it below 7
+        float x; memcpy(&x, &bits, 4);
+        const int b = kv4_scale_byte(bits);
+        REQUIRE(b >= 2 && b <= 252);
+        const double s = __builtin_ldexp(1.0, b - 127);
+        if (b < 252) REQUIRE(x / s < 7.0);
+        if (b > 2) REQUIRE(x / (s / 2) >= 7.0);
+        last = x;
+    }
+    REQUIRE(last > 3e38f);
+    const float w[] = {-__builtin_inff(), -3.f, -1e-40f, 0.f, 1e-40f, 1e-30f, 0.5f, 3.f, __builtin_inff()};
+    for (int i = 0; i < 9; ++i) for (int j = 0; j < 9; ++j) {
+        unsigned x, y; memcpy(&x, &w[i], 4); memcpy(&y, &w[j], 4);
+        REQUIRE((kv4_weight_key(x) < kv4_weight_key(y)) == (w[i] < w[j]));
+        REQUIRE(kv4_weight_key(x) > kv4_weight_key(0x7fc00000u) && kv4_weight_key(0xffc00000u) == 0);
+    }
+    REQUIRE(kv4_weight_key(0x80000000u) == kv4_weight_key(0));
+    return 0;
+}
+"""
+
+
+def test_layout_and_bounds(tmp_path):
+    src, exe = tmp_path / "layout.cpp", tmp_path / "layout"
+    src.write_text(PROGRAM)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Xlinker", "--no-undefined", "-fsanitize=undefined", "-fno-sanitize-recover", f"-I{CSRC}",
+                    str(src), "-o", str(exe)], check=True)
+    run = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert run.returncode == 0, (run.stdout.splitlines() or [run.stderr])[-1] + run.stderr
+    got = torch.tensor([[int(x) for x in line.split()] for line in run.stdout.splitlines()])
+    for hd in (64, 128):                                         # the byte order that the tests' own model states
+        g = got[got[:, 0] == hd]
+        t, d = g[:, 1], g[:, 2]
+        assert torch.equal(g[:, 3], _kv4.k_at(hd, t, d)) and torch.equal(g[:, 4], _kv4.v_at(hd, t, d))
+        assert torch.equal(g[:, 5], 64 * hd + d // 32 * 64 + t)
+
+
+def test_model_rounds_to_the_nearest_level():
+    """The tests' quantiser against a search over all sixteen codes and every scale."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(64, 32, generator=g, dtype=torch.float64) * torch.exp2(torch.randint(-30, 30, (64, 1), generator=g).double())
+    codes, b = _kv4.quantise(x)
+    held = _kv4.value(codes, b)
+    every = torch.cat([_kv4.LEVELS, -_kv4.LEVELS])[None, None] * torch.exp2(b.double() - 127)[..., None]
+    assert torch.equal((held - x).abs(), (every - x[..., None]).abs().amin(-1))
+    top = x.abs().amax(-1)
+    assert (top / torch.exp2(b[:, 0].double() - 127) < 7).all() and (top / torch.exp2(b[:, 0].double() - 128) >= 7).all()
+
+
+def test_struct_layouts():
+    assert C.sizeof(_capi.T3Kv4Cache) == 3 * 8 + 6 * 4
+    assert C.sizeof(_capi.T3Kv4Batch) == 3 * 8 + 4 * 4
+    assert C.sizeof(_capi.T3Kv4EvictDesc) == 7 * 8 + 7 * 4 + 4
+
+
+A = 1 << 20                                                      # an address that is aligned and never followed
+
+
+def _cache(**kw):
+    d = dict(pool_dev=A, block_table_dev=A, layer_stride=8 * 16 * 4352, n_layers=2, n_pages=8, n_streams=4, max_pages=4, Hkv=16, hd=64)
+    d.update(kw)
+    return _capi.T3Kv4Cache(**d)
+
+
+def _batch(**kw):
+    d = dict(seq_start_dev=A, stream_dev=A, ctx_dev=A, n_seqs=2, rows=6, max_rows=3, max_ctx=256)
+    d.update(kw)
+    return _capi.T3Kv4Batch(**d)
+
+
+def _evict(**kw):
+    d = dict(src_dev=A, dst_dev=A, ctx_dev=A, weights_dev=A, weights_stride=256, new_ctx_dev=A, kept_dev=A, n=2, max_ctx=256, keep=32,
+             sink=4, recent=8, layer=0, n_layers=2)
+    d.update(kw)
+    return _capi.T3Kv4EvictDesc(**d)
+
+
+def _refused(lib, rc, words):
+    assert rc != 0
+    assert re.search(words, lib.t3_last_error().decode()), lib.t3_last_error()
+
+
+BAD_CACHES = [(dict(pool_dev=None), "null"), (dict(block_table_dev=None), "null"), (dict(hd=96), "head_dim"), (dict(hd=32), "head_dim"),
+              (dict(Hkv=0), "heads"), (dict(Hkv=1025), "heads"), (dict(n_pages=0), "empty"), (dict(n_streams=0), "empty"),
+              (dict(max_pages=0), "empty"), (dict(pool_dev=A + 8), "aligned"), (dict(layer_stride=8 * 16 * 4352 - 16), "overlap"),
+              (dict(layer_stride=8 * 16 * 4352 + 8), "overlap"), (dict(n_layers=0), "layer"), (dict(max_pages=1 << 25), "entries")]
+BAD_BATCHES = [(dict(seq_start_dev=None), "null"), (dict(stream_dev=None), "null"), (dict(ctx_dev=None), "null"), (dict(n_seqs=0), "sequences"),
+               (dict(n_seqs=70000), "sequences"), (dict(rows=0), "bounds"), (dict(max_rows=7), "bounds"), (dict(max_rows=0), "bounds"),
+               (dict(max_ctx=0), "bounds")]
+
+
+@pytest.mark.parametrize("cache,batch,words", [(c, {}, w) for c, w in BAD_CACHES] + [({}, b, w) for b, w in BAD_BATCHES])
+def test_descriptors_are_refused(cache, batch, words):
+    lib = _capi.load()
+    c, b = C.byref(_cache(**cache)), C.byref(_batch(**batch))
+    _refused(lib, lib.t3_op_kv4_append(c, b, A, A, 1024, 1024, 0, 0, None), words)
+    _refused(lib, lib.t3_op_kv4_read(c, b, A, A, 0, 0, 1, None), words)
+    _refused(lib, lib.t3_op_attn_kv4(c, b, A, 1024, A, 1024, 16, 0, 0.125, None, 0, A, 1 << 30, 0, None), words)
+    assert lib.t3_op_attn_kv4_work_bytes(c, b, 16, 0) == -1
+    if not batch:
+        _refused(lib, lib.t3_op_kv4_evict(c, C.byref(_evict()), None), words)
+
+
+@pytest.mark.parametrize("kw,words", [
+    (dict(k=None), "null"), (dict(v=None), "null"), (dict(dtype=2), "dtype"), (dict(dtype=-1), "dtype"), (dict(layer=2), "layer"),
+    (dict(layer=-1), "layer"), (dict(k=A + 2), "aligned"), (dict(v=A + 8), "aligned"), (dict(ks=1023), "aligned"), (dict(vs=1028), "aligned"),
+    (dict(ks=512), "overlap"), (dict(ks=-1024), "overlap")])
+def test_append_refusals(kw, words):
+    lib = _capi.load()
+    d = dict(k=A, v=A, ks=1024, vs=1024, dtype=0, layer=0)
+    d.update(kw)
+    _refused(lib, lib.t3_op_kv4_append(C.byref(_cache()), C.byref(_batch()), d["k"], d["v"], d["ks"], d["vs"], d["dtype"], d["layer"], None), words)
+
+
+@pytest.mark.parametrize("kw,words", [
+    (dict(k=None), "null"), (dict(v=None), "null"), (dict(dtype=3), "dtype"), (dict(layer=1, n=2), "layer"), (dict(n=0), "layer"),
+    (dict(n=-1), "layer"), (dict(layer=2147483647, n=2), "layer"), (dict(k=A + 8), "aligned")])
+def test_read_refusals(kw, words):
+    lib = _capi.load()
+    d = dict(k=A, v=A, dtype=0, layer=0, n=1)
+    d.update(kw)
+    _refused(lib, lib.t3_op_kv4_read(C.byref(_cache()), C.byref(_batch()), d["k"], d["v"], d["dtype"], d["layer"], d["n"], None), words)
+
+
+@pytest.mark.parametrize("kw,words", [
+    (dict(q=None), "null"), (dict(out=None), "null"), (dict(dtype=2), "dtype"), (dict(H=24), "query heads"), (dict(H=0), "query heads"),
+    (dict(H=8), "query heads"), (dict(H=16 * 65), "query heads"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"),
+    (dict(scale=float("inf")), "scale"), (dict(qs=1020), "overlap"), (dict(qs=1028), "aligned"), (dict(os=512), "overlap"), (dict(q=A + 4), "aligned"), (dict(out=A + 8), "aligned"),
+    (dict(w=A, ws=255), "weights_stride"), (dict(w=A, ws=256, work=None), "work"), (dict(w=A, ws=256, size=6 * 16 * 8 - 1), "work"),
+    (dict(w=A, ws=256, work=A + 8), "work"), (dict(layer=2), "layer")])
+def test_attention_refusals(kw, words):
+    lib = _capi.load()
+    d = dict(q=A, qs=1024, out=A, os=1024, H=16, dtype=0, scale=0.125, w=None, ws=0, work=A, size=1 << 30, layer=0)
+    d.update(kw)
+    _refused(lib, lib.t3_op_attn_kv4(C.byref(_cache()), C.byref(_batch()), d["q"], d["qs"], d["out"], d["os"], d["H"], d["dtype"], d["scale"],
+                                     d["w"], d["ws"], d["work"], d["size"], d["layer"], None), words)
+
+
+@pytest.mark.parametrize("kw,words", [
+    (dict(src_dev=None), "null"), (dict(dst_dev=None), "null"), (dict(ctx_dev=None), "null"), (dict(weights_dev=None), "null"),
+    (dict(new_ctx_dev=None), "null"), (dict(kept_dev=None), "null"), (dict(n=0), "entries"), (dict(n=5000), "entries"), (dict(max_ctx=257), "max_ctx"),
+    (dict(max_ctx=0), "max_ctx"), (dict(keep=0), "keep"), (dict(sink=25), "sink"), (dict(sink=-1), "sink"), (dict(recent=-1), "sink"),
+    (dict(sink=2147483647, recent=2147483647), "sink"), (dict(keep=257), "keep"), (dict(layer=1), "layer"), (dict(n_layers=3), "layer"), (dict(n_layers=0), "layer")])
+def test_evict_refusals(kw, words):
+    lib = _capi.load()
+    _refused(lib, lib.t3_op_kv4_evict(C.byref(_cache()), C.byref(_evict(**kw)), None), words)
+    _refused(lib, lib.t3_op_kv4_evict(C.byref(_cache()), None, None), "null")
+
+
+def test_sizes():
+    lib = _capi.load()
+    assert lib.t3_op_kv4_page_bytes(16, 64) == 16 * 4352 and lib.t3_op_kv4_page_bytes(1, 128) == 8704
+    assert lib.t3_op_kv4_page_bytes(16, 80) == 0 and lib.t3_op_kv4_page_bytes(0, 64) == 0
+    c, b = C.byref(_cache()), C.byref(_batch())
+    assert lib.t3_op_attn_kv4_work_bytes(c, b, 16, 0) == 0       # one chunk: nothing to join
+    assert lib.t3_op_attn_kv4_work_bytes(c, b, 16, 1) >= 6 * 16 * 8
+    c = C.byref(_cache(max_pages=1 << 20))
+    assert lib.t3_op_attn_kv4_work_bytes(c, C.byref(_batch(max_ctx=40000)), 16, 0) > 0

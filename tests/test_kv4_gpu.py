@@ -1,0 +1,585 @@
+"""The 4-bit KV cache on the GPU against the plain 64-bit restatement in _kv4.py: bytes and kept indices are exact, attention is
+held to bounds that follow from the roundings (_kv4.out_bound, _kv4.weights_bound)."""
+import math
+
+import pytest
+import torch
+
+import _kv4
+from chatterbox_vllm_amd import _capi
+from chatterbox_vllm_amd.kv4_cache import KV4Cache, page_bytes
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def starts(rows):
+    s = [0]
+    for r in rows:
+        s.append(s[-1] + r)
+    return s
+
+
+def device_cache(m):
+    return KV4Cache(m.kv, m.hd, pool=m.pool.to(DEV), block_table=m.table.to(DEV))
+
+
+def check_attend(m, cache, rows, ctx, group, dtype, with_weights, streams=None, layer=0, seed=0, qkv=None, batch=None):
+    """One call against the model; returns (q, out, weights)."""
+    n = len(rows)
+    streams = list(range(n)) if streams is None else streams
+    H, R = m.kv * group, sum(rows)
+    g = torch.Generator().manual_seed(seed)
+    q = (torch.randn(R, H, m.hd, generator=g) * 1.5).to(DT[dtype])
+    s = starts(rows)
+    batch = cache.batch(i32(s), i32(streams), i32(ctx), rows=R, max_rows=max(rows), max_ctx=max(ctx)) if batch is None else batch
+    w0 = torch.rand(m.table.shape[0], m.kv, m.table.shape[1] * 64, generator=g)
+    w = w0.to(DEV) if with_weights else None
+    out = cache.attend(q.to(DEV), batch, layer=layer, weights=w)
+    torch.cuda.synchronize()
+    scale = m.hd ** -0.5
+    want_w, added, slack = w0.double().clone(), torch.zeros_like(w0, dtype=torch.float64), torch.zeros_like(w0, dtype=torch.float64)
+    for i in range(n):
+        k, v = m.get(m.pool, streams[i], torch.arange(ctx[i]), layer)
+        ref, p, size, bound = _kv4.attend(q[s[i]:s[i + 1]].double(), k, v, ctx[i], scale)
+        err = (out[s[i]:s[i + 1]].cpu().double() - ref).abs()
+        tol = _kv4.out_bound(ref, size, bound, ctx[i], DT[dtype])
+        assert (err <= tol).all(), f"sequence {i} ({rows[i]} rows, {ctx[i]} entries): {(err / tol).max():.2f} of the bound"
+        added[streams[i], :, :ctx[i]] += p
+        slack[streams[i], :, :ctx[i]] += _kv4.weights_bound(p, torch.zeros_like(p), bound, ctx[i], rows[i] * group)
+    if with_weights:
+        err = (w.cpu().double() - (want_w + added)).abs()
+        tol = slack + (want_w + added) * 2.0 ** -23
+        assert (err <= tol).all(), f"weights: {(err / tol.clamp_min(1e-300)).max():.2f} of the bound"
+        assert torch.equal(w.cpu()[added == 0], w0[added == 0])
+    return q, out, w
+
+
+# ---- append, read ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("hd,kv", [(64, 16), (64, 1), (128, 8), (128, 3)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("rows,ctx", [([1], [1]), ([1, 1, 1], [64, 65, 200]), ([5, 64, 1, 130], [5, 128, 1, 193]), ([9, 3], [4, 130])])
+def test_append_and_read_bytes(hd, kv, dtype, rows, ctx):
+    m = _kv4.Model(hd, kv, 2, 40, 6, 4, seed=1)
+    cache = device_cache(m)
+    streams, s, R = [4, 1, 5, 2][:len(rows)], starts(rows), sum(rows)
+    g = torch.Generator().manual_seed(2)
+    buf = torch.randn(R + 2, 3 * kv, hd, generator=g) * torch.exp2(torch.randint(-20, 12, (R + 2, 3 * kv, 1), generator=g).float())
+    buf = buf.to(DT[dtype])
+    want, held = m.pool.clone(), []
+    for i in range(len(rows)):
+        slots = torch.arange(ctx[i] - rows[i], ctx[i])
+        ok = slots >= 0                                          # rows before entry 0 are not stored
+        rk, rv = buf[s[i]:s[i + 1], kv:2 * kv], buf[s[i]:s[i + 1], 2 * kv:]
+        k, v = (torch.zeros(rows[i], kv, hd, dtype=torch.float64) for _ in range(2))
+        k[ok], v[ok] = m.put(want, streams[i], slots[ok], rk[ok], rv[ok], layer=1)
+        held.append((k, v))
+    batch = cache.batch(i32(s), i32(streams), i32(ctx), rows=R, max_rows=max(rows), max_ctx=max(ctx))
+    dbuf = buf.to(DEV)[:R]                                       # views of a wider buffer
+    cache.append(dbuf[:, kv:2 * kv], dbuf[:, 2 * kv:], batch, layer=1)
+    torch.cuda.synchronize()
+    assert torch.equal(cache.pool.cpu(), want)
+    for out in DT:
+        top = torch.finfo(DT[out]).max
+        k, v = cache.read(batch, layer=1, dtype=DT[out])
+        both = cache.read(batch, layer=0, n_layers=2, dtype=DT[out])
+        torch.cuda.synchronize()
+        for got, two, ref in ((k, both[0], 0), (v, both[1], 1)):
+            ref = torch.cat([h[ref] for h in held]).clamp(-top, top).to(DT[out])
+            assert torch.equal(got.cpu(), ref) and torch.equal(two[1].cpu(), ref)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_append_special_values(hd):
+    """Zeros, ties, the largest and smallest magnitudes; an entry with a NaN or an infinity becomes a NaN entry, its neighbours do not."""
+    kv, m = 2, _kv4.Model(hd, 2, 1, 4, 1, 2, seed=3)
+    cache = device_cache(m)
+    tiny, big = 2.0 ** -133, torch.finfo(torch.bfloat16).max
+    rows = torch.zeros(12, 2 * kv, hd)
+    pattern = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0])
+    rows[1] = pattern.repeat(hd // 8)
+    rows[2] = -rows[1] * 2.0 ** -100
+    rows[3] = rows[1] * 2.0 ** 100
+    rows[4, :, 0] = 6.96875                                       # the last bf16 below 7; then 7 itself
+    rows[5, :, 0], rows[5, :, 1] = 7.0, 0.6
+    rows[6] = tiny
+    rows[7], rows[7, 0] = big, -big
+    rows[8] = 1.0
+    rows[8, 0, hd - 1], rows[8, 3, 5] = math.nan, math.inf        # K head 0; V head 1
+    rows[9], rows[9, 1, 0] = 2.0, -math.inf                       # K head 1
+    rows[10] = 2.0 ** -126 * pattern.repeat(hd // 8)
+    rows[11] = -0.0
+    rows = rows.to(torch.bfloat16)
+    want = m.pool.clone()
+    k, v = m.put(want, 0, torch.arange(12), rows[:, :kv], rows[:, kv:])
+    batch = cache.batch(i32([0, 12]), i32([0]), i32([12]), rows=12)
+    d = rows.to(DEV)
+    cache.append(d[:, :kv], d[:, kv:], batch)
+    gk, gv = cache.read(batch)
+    torch.cuda.synchronize()
+    assert torch.equal(cache.pool.cpu(), want)
+    for got, ref in ((gk, k), (gv, v)):
+        assert torch.equal(torch.nan_to_num(got.cpu().double(), 77.0), torch.nan_to_num(ref, 77.0))
+    nan = torch.isnan(gk.cpu())
+    assert nan[8].all() and nan[9, 1].all() and not nan[9, 0].any() and not nan[[0, 1, 2, 3, 4, 5, 6, 7, 10, 11]].any()
+    # fp16: what rounds up past its largest value is cut there
+    h = torch.full((12, 2 * kv, hd), 65504.0, dtype=torch.float16, device=DEV)
+    cache.append(h[:, :kv], h[:, kv:], batch)
+    assert (cache.read(batch, dtype=torch.float16)[0] == 65504).all() and (cache.read(batch)[0] == 65536).all()
+
+
+# ---- attention ---------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("hd,kv,group", [(64, 16, 1), (64, 2, 5), (128, 2, 1), (128, 2, 8), (128, 1, 16), (64, 1, 33)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("with_weights", [False, True])
+def test_decode(hd, kv, group, dtype, with_weights):
+    ctx = [1, 2, 63, 64, 65, 500, 512, 513, 1030]
+    m = _kv4.Model(hd, kv, 2, 17 * 9 + 2, 9, 17, seed=4)
+    for i, t in enumerate(ctx):
+        m.fill(i, t, layer=1)
+    check_attend(m, device_cache(m), [1] * 9, ctx, group, dtype, with_weights, layer=1)
+
+
+@pytest.mark.parametrize("hd,ctx", [(64, [8192, 8193, 20000]), (128, [16390, 8100, 9217])])
+def test_decode_long(hd, ctx):
+    """Lengths at which the chunks change, and many of them."""
+    m = _kv4.Model(hd, 1, 1, 3 * 313, 3, 313, seed=5)
+    for i, t in enumerate(ctx):
+        m.fill(i, t)
+    check_attend(m, device_cache(m), [1] * 3, ctx, 2, "bf16", True)
+
+
+@pytest.mark.parametrize("hd,kv,group,rows,ctx", [
+    (64, 2, 1, [5, 1, 8, 3], [5, 70, 600, 2]),                    # the last: rows before entry 0 see nothing
+    (128, 3, 8, [5, 2, 8, 4], [700, 130, 8, 65]),
+    (64, 1, 1, [64, 65, 63], [64, 65, 640]),                      # both sides of the form for few columns
+    (128, 1, 7, [9, 10, 1], [90, 10, 513]),
+    (128, 2, 64, [1, 2], [65, 129])])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_drafts_and_mixed_batches(hd, kv, group, rows, ctx, dtype):
+    m = _kv4.Model(hd, kv, 1, 4 * 11 + 1, 4, 11, seed=6)
+    for i, t in enumerate(ctx):
+        m.fill(i, t)
+    check_attend(m, device_cache(m), rows, ctx, group, dtype, True)
+
+
+@pytest.mark.parametrize("hd,kv,group,rows,ctx", [
+    (64, 2, 1, [130, 70, 257], [130, 200, 257]),
+    (64, 1, 3, [100, 33], [300, 33]),
+    (128, 1, 4, [300, 17, 90], [301, 17, 20]),                    # the last: 70 rows see nothing
+    (128, 2, 5, [77], [500])])
+@pytest.mark.parametrize("dtype,with_weights", [("bf16", True), ("fp16", False), ("fp16", True)])
+def test_prompts(hd, kv, group, rows, ctx, dtype, with_weights):
+    m = _kv4.Model(hd, kv, 1, 3 * 8 + 1, 3, 8, seed=7)
+    for i, t in enumerate(ctx):
+        m.fill(i, t)
+    check_attend(m, device_cache(m), rows, ctx, group, dtype, with_weights)
+
+
+@pytest.mark.parametrize("rows", [[1, 1, 1, 1], [4, 1, 2, 3], [90, 1, 200, 7]])
+def test_rows_do_not_depend_on_the_batch(rows):
+    ctx = [700, 65, 1500, 33]
+    m = _kv4.Model(64, 2, 1, 4 * 24, 4, 24, seed=8)
+    for i, t in enumerate(ctx):
+        m.fill(i, t)
+    ctx = [max(a, b) for a, b in zip(ctx, rows)]
+    cache = device_cache(m)
+    q = torch.randn(sum(rows), 6, 64, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(DEV)
+    s = starts(rows)
+    full = cache.attend(q, cache.batch(i32(s), i32([0, 1, 2, 3]), i32(ctx), rows=sum(rows)))
+    for i in range(4):
+        alone = cache.attend(q[s[i]:s[i + 1]], cache.batch(i32([0, rows[i]]), i32([i]), i32([ctx[i]]), rows=rows[i], max_ctx=ctx[i]))
+        assert torch.equal(alone, full[s[i]:s[i + 1]])
+
+
+def test_sharp_and_flat_scores():
+    """Scores in the hundreds (one entry takes all) and all equal; NaN entries reach the rows that see them and no others."""
+    m = _kv4.Model(64, 1, 1, 9, 1, 9, seed=9)
+    k, v = torch.randn(513, 1, 64) * 30, torch.randn(513, 1, 64)
+    m.put(m.pool, 0, torch.arange(513), k, v)
+    check_attend(m, device_cache(m), [1], [513], 1, "bf16", True)
+    m.put(m.pool, 0, torch.arange(513), torch.ones(513, 1, 64), v)
+    check_attend(m, device_cache(m), [3], [513], 1, "fp16", True)
+    for rows in (5, 200):                                         # both forms; the entry of the row before the last two is NaN
+        t = 300
+        kk = torch.randn(t, 1, 64)
+        kk[t - 3, 0, 7] = math.nan
+        m.put(m.pool, 0, torch.arange(t), kk, v[:t])
+        cache = device_cache(m)
+        q = torch.randn(rows, 1, 64).to(torch.bfloat16)
+        out = cache.attend(q.to(DEV), cache.batch(i32([0, rows]), i32([0]), i32([t]), rows=rows)).cpu()
+        assert torch.isnan(out[-3:]).all()
+        ref, _, size, bound = _kv4.attend(q[:-3].double(), *(x[:t - 3] for x in m.get(m.pool, 0, torch.arange(t))), t - 3, 0.125)
+        assert ((out[:-3].double() - ref).abs() <= _kv4.out_bound(ref, size, bound, t, torch.bfloat16)).all()
+
+
+def test_what_lies_behind_the_last_entry_does_not_matter():
+    """Every byte behind the last entry set, scales to NaN among them."""
+    outs = []
+    for fill in (0, 255):
+        m = _kv4.Model(128, 2, 1, 4, 1, 4, seed=10)
+        m.pool.fill_(fill)
+        for t in (1, 40, 130):
+            m.g.manual_seed(t)
+            m.fill(0, t)
+            outs.append(check_attend(m, device_cache(m), [1], [t], 2, "bf16", True)[1])
+            outs.append(check_attend(m, device_cache(m), [min(t, 70)], [t], 2, "bf16", True)[1])
+    assert all(torch.equal(a, b) for a, b in zip(outs[:6], outs[6:]))
+
+
+def test_skipped_rows_and_strides():
+    m = _kv4.Model(64, 2, 1, 30, 5, 5, seed=11)
+    for i in range(5):
+        m.fill(i, 300)
+    cache = device_cache(m)
+    rows, R = [3, 100, 1, 0, 2], 106
+    s = starts(rows)
+    batch = cache.batch(i32(s), i32([0, -1, 2, 3, -7]), i32([40, 300, 280, 10, 9]), rows=R + 4)      # four rows behind the last sequence
+    wide = torch.randn(R + 4, 9, 64).to(torch.bfloat16).to(DEV)
+    out = torch.full((R + 4, 5, 64), 7.0, dtype=torch.bfloat16, device=DEV)
+    got = cache.attend(wide[:, 2:6], batch, out=out[:, 1:])
+    assert got.data_ptr() == out[:, 1:].data_ptr()
+    touched = [0, 1, 2, 103]
+    rest = [i for i in range(R + 4) if i not in touched]
+    assert (out[rest] == 7).all() and (out[:, 0] == 7).all()
+    tight = cache.attend(wide[:, 2:6].contiguous(), batch)
+    assert torch.equal(tight[touched], out[touched, 1:])
+    before = cache.pool.clone()
+    cache.append(wide[:, :2], wide[:, 2:4], batch)
+    changed = (cache.pool != before).view(30, -1).any(1).nonzero().view(-1).tolist()
+    assert sorted(changed) == sorted({int(m.table[0, 0]), int(m.table[2, 4])})
+
+
+def test_numbers_that_do_not_fit_give_nan_and_store_nothing():
+    """The kernels' own checks: nothing outside the buffers is followed, the rows in question are NaN, the others are right."""
+    m = _kv4.Model(64, 2, 1, 30, 6, 5, seed=12)
+    for i in range(6):
+        m.fill(i, 200)
+    m.table[3, 1] = 30                                            # a page that there is not; stream 4 has one at the same place
+    m.table[4, 1] = -1
+    cache = device_cache(m)
+    for rows in (1, 100):
+        n, R = 7, 7 * rows
+        ctx, streams = [200, 200, 321, 200, 100, 100, 200], [0, 6, 2, 3, 4, 1, 5]
+        q = torch.randn(R, 2, 64).to(torch.bfloat16).to(DEV)
+        batch = cache.batch(i32(starts([rows] * n)), i32(streams), i32(ctx), rows=R, max_rows=rows, max_ctx=320)
+        w = torch.zeros(6, 2, 320, device=DEV)
+        out = cache.attend(q, batch, weights=w).view(n, rows, 2, 64).cpu()
+        for i in (1, 2, 3, 4):
+            assert torch.isnan(out[i, -1]).all()
+        assert torch.isnan(out[[1, 2]]).all()
+        for i in (0, 5, 6):
+            ref, _, size, bound = _kv4.attend(q.cpu().double()[i * rows:(i + 1) * rows], *m.get(m.pool, streams[i], torch.arange(ctx[i])), ctx[i], 0.125)
+            assert ((out[i].double() - ref).abs() <= _kv4.out_bound(ref, size, bound, 200, torch.bfloat16)).all()
+        assert not torch.isnan(w[[0, 1, 2, 5]]).any() and (w[2] == 0).all()
+        k, v = cache.read(batch)
+        k, v = k.view(n, rows, 2, 64), v.view(n, rows, 2, 64)
+        assert torch.isnan(k[[1, 2]]).all() and torch.isnan(v[[1, 2]]).all()
+        if rows == 100:                                           # its rows are entries 100 .. 199, the missing page 64 .. 127
+            assert torch.isnan(v[3, :28]).all() and torch.isnan(k[3, :28]).all() and not torch.isnan(v[3, 28:]).any()
+        before = cache.pool.clone()
+        cache.append(q, q, cache.batch(i32(starts([rows] * n)), i32([6, 9, 2, -1, 7, -2, 8]), i32([200, 5, 321, 0, 1, 2, 3]), rows=R, max_ctx=320))
+        assert torch.equal(cache.pool, before)
+    # a stream whose second page is missing: rows that end in the first see nothing of it
+    q = torch.randn(100, 2, 64).to(torch.bfloat16)
+    out = cache.attend(q.to(DEV), cache.batch(i32([0, 100]), i32([4]), i32([100]), rows=100)).cpu()
+    assert torch.isnan(out[64:]).all() and not torch.isnan(out[:64]).any()
+    # more rows than the bound, rows beyond the tensor, sequences out of order
+    q = torch.randn(8, 2, 64).to(torch.bfloat16).to(DEV)
+    out = torch.full((8, 2, 64), 7.0, dtype=torch.bfloat16, device=DEV)
+    cache.attend(q, cache.batch(i32([0, 4, 5]), i32([0, 1]), i32([9, 9]), rows=8, max_rows=3), out=out)
+    assert torch.isnan(out[:3]).all() and (out[3] == 7).all() and not torch.isnan(out[4]).any() and (out[5:] == 7).all()
+    out.fill_(7.0)
+    cache.attend(q, cache.batch(i32([6, 11]), i32([0]), i32([9]), rows=8, max_rows=8), out=out)
+    assert torch.isnan(out[6:]).all() and (out[:6] == 7).all()
+    out.fill_(7.0)
+    cache.attend(q, cache.batch(i32([5, 2, -3]), i32([0, 1]), i32([9, 9]), rows=8), out=out)
+    assert (out == 7).all()
+
+
+def test_weights_of_a_stream_that_occurs_twice():
+    """Two sequences of one stream (two drafts, say) are added in their order; equal calls give equal bits."""
+    m = _kv4.Model(64, 2, 1, 20, 4, 5, seed=13)
+    for i in range(4):
+        m.fill(i, 300)
+    rows, ctx, streams = [1, 3, 2, 1, 90], [250, 300, 120, 300, 290], [2, 0, 2, 2, 0]
+    cache = device_cache(m)
+    _, _, w = check_attend(m, cache, rows, ctx, 2, "bf16", True, streams=streams)
+    for _ in range(3):
+        assert torch.equal(check_attend(m, cache, rows, ctx, 2, "bf16", True, streams=streams)[2], w)
+
+
+def test_offsets_past_32_bits():
+    """A pool of more than 4 GiB, pages at its end."""
+    pages = (1 << 32) // page_bytes(8, 128) + 40
+    pool = torch.empty(1, pages, page_bytes(8, 128), dtype=torch.uint8, device=DEV)
+    table = torch.arange(pages - 1, pages - 9, -1, dtype=torch.int32, device=DEV).view(2, 4)
+    small = KV4Cache(8, 128, num_pages=8, block_table=torch.arange(7, -1, -1, dtype=torch.int32, device=DEV).view(2, 4))
+    big = KV4Cache(8, 128, pool=pool, block_table=table)
+    g = torch.Generator(device=DEV).manual_seed(0)
+    k, v, q = (torch.randn(300, h, 128, generator=g, device=DEV).to(torch.bfloat16) for h in (8, 8, 16))
+    got = []
+    for c in (small, big):
+        b = c.batch(i32([0, 200, 300]), i32([0, 1]), i32([200, 250]), rows=300)
+        c.pool[:, -8:].zero_()
+        c.append(k, v, b)
+        w = c.new_weights()
+        w[0, 0] += torch.arange(256, device=DEV)
+        got.append([c.attend(q, b, weights=w[0]), *c.read(b), w.clone()])
+        c.block_table[1] = c.block_table[1].flip(0)
+        got[-1] += [*c.evict(i32([0]), i32([1]), i32([200]), 90, 5, 20, w), *c.read(c.batch(i32([0, 90]), i32([1]), i32([90]), rows=90))]
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    del pool, big
+
+
+# ---- eviction ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("hd,kv,layers", [(64, 3, 2), (128, 2, 1)])
+@pytest.mark.parametrize("keep,sink,recent,ctx", [
+    (100, 7, 20, [300, 101, 100, 64, 1, 0]), (64, 0, 0, [65, 640, 127, 64, 63, 2]), (1, 0, 0, [5, 1, 640, 0, 64, 65]),
+    (30, 10, 20, [31, 200, 30, 29, 640, 11]), (257, 34, 128, [640, 258, 257, 256, 400, 1])])
+def test_evict(hd, kv, layers, keep, sink, recent, ctx):
+    n = 6
+    m = _kv4.Model(hd, kv, layers, 2 * n * 10 + 1, 2 * n, 10, seed=14)
+    for layer in range(layers):
+        for i, t in enumerate(ctx):
+            m.fill(i, t, layer=layer) if t else None
+    g = torch.Generator().manual_seed(15)
+    w = torch.rand(layers, 2 * n, kv, 640, generator=g)
+    w = torch.where(w < 0.3, torch.zeros(()), (w * 20).floor())   # many ties
+    w[:, 0, 0, 30:40], w[:, 1, 1, 40:50] = math.nan, math.inf
+    w[:, 0, 1, :], w[:, 1, 0, 5] = 0.0, -1.0
+    w[:, 0, 1, ::3] = -0.0
+    cache = device_cache(m)
+    dw = w.to(DEV)
+    dst = [11, 6, 8, 7, 10, 9]
+    before = cache.pool.clone()
+    new, kept = cache.evict(i32(list(range(n))), i32(dst), i32(ctx), keep, sink, recent, dw)
+    torch.cuda.synchronize()
+    left = [min(t, keep) for t in ctx]
+    assert new.tolist() == left
+    pool, after = cache.pool.cpu(), dw.cpu()
+    used = m.table[:n].flatten().long()
+    assert torch.equal(pool[:, used], before.cpu()[:, used]) and torch.equal(torch.nan_to_num(after[:, :n], 9.5), torch.nan_to_num(w[:, :n], 9.5))
+    for layer in range(layers):
+        for i in range(n):
+            held = m.get(m.pool, i, torch.arange(ctx[i]), layer)
+            got = m.get(pool, dst[i], torch.arange(left[i]), layer)
+            for h in range(kv):
+                stay = _kv4.choose(w[layer, i, h].tolist(), ctx[i], keep, sink, recent)
+                assert kept[layer, i, h].tolist() == stay + [-1] * (keep - left[i])
+                for a, b in zip(got, held):
+                    assert torch.equal(a[:, h], b[stay, h])
+                assert torch.equal(torch.nan_to_num(after[layer, dst[i], h, :left[i]], 9.5), torch.nan_to_num(w[layer, i, h][stay], 9.5))
+                assert (after[layer, dst[i], h, left[i]:] == 0).all()
+
+
+def test_evict_long_and_nan_entries():
+    """More entries than threads of a workgroup take at once; all weights equal, all different; a NaN entry stays one."""
+    m = _kv4.Model(64, 2, 1, 2 * 160, 2, 160, seed=16)
+    k = torch.randn(10001, 2, 64)
+    k[3, 1, 0] = math.nan
+    m.put(m.pool, 0, torch.arange(10001), k, k)
+    cache = device_cache(m)
+    w = cache.new_weights()
+    w[0, 0, 1] = torch.rand(160 * 64, device=DEV)
+    host = w.cpu()
+    new, kept = cache.evict(i32([0]), i32([1]), i32([10001]), 5000, 4, 1000, w)
+    for h in range(2):
+        stay = _kv4.choose(host[0, 0, h].tolist(), 10001, 5000, 4, 1000)
+        assert kept[0, 0, h].tolist() == stay
+        held, got = m.get(m.pool, 0, torch.tensor(stay)), m.get(cache.pool.cpu(), 1, torch.arange(5000))
+        assert all(torch.equal(torch.nan_to_num(a[:, h], 9.5), torch.nan_to_num(b[:, h], 9.5)) for a, b in zip(got, held))
+    assert torch.isnan(cache.read(cache.batch(i32([0, 5]), i32([1]), i32([5]), rows=5))[0][3, 1]).all()
+
+
+def test_evict_refuses_entry_by_entry():
+    m = _kv4.Model(64, 2, 1, 40, 12, 3, seed=17)
+    for i in range(12):
+        m.fill(i, 190)
+    m.table[3, 2] = m.table[4, 1]                                 # 3 -> 4: a page of both
+    m.table[5, 1] = 40                                            # a page that there is not
+    m.table[7, 0] = -3
+    cache = device_cache(m)
+    w = cache.new_weights()
+    w += torch.rand(w.shape, device=DEV)
+    pool, w0 = cache.pool.clone(), w.clone()
+    #      good  range  range  self   pages  page   page   dst again   dst is a src   too long
+    src = [0,    12,    0,     1,     3,     5,     0,     1,          0,             0]
+    dst = [11,   10,    -1,    1,     4,     6,     7,     11,         3,             9]
+    ctx = [190,  100,   100,   100,   190,   190,   190,   190,        190,           193]
+    new, kept = cache.evict(i32(src), i32(dst), i32(ctx), 70, 2, 10, w)
+    assert new.tolist() == [70] + [-1] * 9
+    assert (kept[:, 1:] == -1).all() and (kept[:, 0] >= 0).all()
+    own = m.table[11].long().to(DEV)
+    others = [p for p in range(40) if p not in own.tolist()]
+    assert torch.equal(cache.pool[:, others], pool[:, others]) and torch.equal(w[:, :11], w0[:, :11])
+    # one source may go to several destinations
+    new, kept = cache.evict(i32([0, 0]), i32([10, 9]), i32([190, 100]), 70, 2, 10, w)
+    assert new.tolist() == [70, 70] and kept.max() < 190
+
+
+# ---- the operators together ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("hd,kv,group", [(64, 4, 1), (128, 2, 4)])
+def test_a_stream_from_prompt_to_eviction_and_on(hd, kv, group):
+    """Prompt in, attend with weights, decode some tokens, evict, decode on: every step against the 64-bit model."""
+    m = _kv4.Model(hd, kv, 2, 60, 6, 8, seed=18)
+    cache = device_cache(m)
+    g = torch.Generator().manual_seed(19)
+    n, layer = 2, 1
+    weights = cache.new_weights()
+    model_w = torch.zeros(6, kv, 8 * 64, dtype=torch.float64)
+    slack = 0.0
+
+    def step(rows, ctx, streams):
+        nonlocal slack
+        s, R = starts(rows), sum(rows)
+        qkv = torch.randn(R, kv * group + 2 * kv, hd, generator=g).to(torch.bfloat16)
+        d = qkv.to(DEV)
+        q, k, v = d[:, :kv * group], d[:, kv * group:-kv], d[:, -kv:]
+        batch = cache.batch(i32(s), i32(streams), i32(ctx), rows=R)
+        cache.append(k, v, batch, layer=layer)
+        out = cache.attend(q, batch, layer=layer, weights=weights[layer]).cpu().double()
+        for i, st in enumerate(streams):
+            m.put(m.pool, st, torch.arange(ctx[i] - rows[i], ctx[i]), qkv[s[i]:s[i + 1], kv * group:-kv], qkv[s[i]:s[i + 1], -kv:], layer)
+            kk, vv = m.get(m.pool, st, torch.arange(ctx[i]), layer)
+            ref, p, size, bound = _kv4.attend(qkv[s[i]:s[i + 1], :kv * group].double(), kk, vv, ctx[i], hd ** -0.5)
+            assert ((out[s[i]:s[i + 1]] - ref).abs() <= _kv4.out_bound(ref, size, bound, ctx[i], torch.bfloat16)).all()
+            model_w[st, :, :ctx[i]] += p
+            slack = max(slack, _kv4.weights_bound(p, p, bound, ctx[i], rows[i] * group).max().item())
+
+    ctx = [150, 97]
+    step(ctx, ctx, [0, 1])
+    steps = 1
+    for _ in range(5):
+        ctx = [t + 1 for t in ctx]
+        step([1, 1], ctx, [0, 1])
+        steps += 1
+    w = weights[layer].cpu().double()
+    assert ((w - model_w).abs() <= 8 * steps * slack).all()
+    new, kept = cache.evict(i32([0, 1]), i32([2, 3]), i32(ctx), keep=80, sink=8, recent=16, weights=weights[layer:], layer=layer)
+    assert new.tolist() == [80, 80]
+    host = weights[layer].cpu()
+    for i in range(n):
+        for h in range(kv):
+            stay = _kv4.choose(w[i, h].tolist(), ctx[i], 80, 8, 16)
+            assert kept[0, i, h].tolist() == stay
+            assert torch.equal(host[2 + i, h, :80].double(), w[i, h][stay]) and (host[2 + i, h, 80:] == 0).all()
+    m.pool = cache.pool.cpu().clone()
+    model_w = host.double().clone()
+    ctx = [80, 80]
+    for _ in range(3):
+        ctx = [t + 1 for t in ctx]
+        step([1, 1], ctx, [2, 3])
+    step([2, 90], [85, 173], [2, 3])
+    assert ((weights[layer].cpu().double() - model_w).abs() <= 8 * 5 * slack + model_w * 2.0 ** -21).all()
+
+
+def test_captured_steps_replay():
+    """A decode step (append, attend with weights, read) and an eviction captured into graphs: replays follow what is written into
+    the batch's tensors, two graphs do not disturb each other, eager work runs in between."""
+    n = 4
+    m = _kv4.Model(64, 4, 1, 90, 8, 11, seed=20)
+    for i in range(n):
+        m.fill(i, 600)
+    cache, eager = device_cache(m), device_cache(m)
+    g = torch.Generator(device=DEV).manual_seed(21)
+
+    def inputs():
+        return torch.randn(n, 16, 64, generator=g, device=DEV).to(torch.bfloat16)
+
+    def step(c, x, b, w):
+        c.append(x[:, 8:12], x[:, 12:], b)
+        return (c.attend(x[:, :8], b, weights=w), *c.read(b))
+
+    x, ctx, w, we = inputs(), i32([600, 64, 65, 512]), cache.new_weights(), eager.new_weights()
+    s, streams = i32(starts([1] * n)), i32(list(range(n)))
+    batch, ebatch = cache.batch(s, streams, ctx, rows=n, max_rows=1), eager.batch(s, streams, ctx, rows=n, max_rows=1)
+    src, dst, ectx = i32([0, 2]), i32([4, 5]), i32([600, 70])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):                                 # warm-up, on scratch weights
+        step(cache, x, batch, cache.new_weights()[0])
+    torch.cuda.current_stream().wait_stream(side)
+    cache.pool.copy_(eager.pool)
+    torch.cuda.synchronize()
+    one, two = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(one):
+        got = step(cache, x, batch, w[0])
+    with torch.cuda.graph(two):
+        new, kept = cache.evict(src, dst, ectx, 50, 4, 8, w)
+    cache.pool.copy_(eager.pool)
+    w.zero_()
+    for t in range(4):
+        x.copy_(inputs())
+        ctx.add_(1)
+        ectx.copy_(i32([int(ctx[0]), int(ctx[2])]))
+        one.replay()
+        two.replay()
+        torch.cuda.synchronize()
+        want = step(eager, x, ebatch, we[0])
+        enew, ekept = eager.evict(src, dst, ectx, 50, 4, 8, we)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), t
+        assert torch.equal(new, enew) and torch.equal(kept, ekept) and torch.equal(w, we) and torch.equal(cache.pool, eager.pool)
+
+
+def test_two_streams_at_once():
+    """Calls in flight on two streams use work buffers of their own."""
+    m = _kv4.Model(64, 4, 1, 4 * 40, 4, 40, seed=22)
+    for i in range(4):
+        m.fill(i, 2500)
+    cache = device_cache(m)
+    q = torch.randn(2, 2, 8, 64).to(torch.bfloat16).to(DEV)
+    batches = [cache.batch(i32([0, 1, 2]), i32(s), i32([2500, 2400]), rows=2, max_rows=1) for s in ([0, 1], [2, 3])]
+    want = [cache.attend(q[i], batches[i]) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(cache.attend(q[i], batches[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i in range(2) for o in got[i])
+
+
+def test_python_refusals():
+    cache = KV4Cache(2, 64, num_pages=4, num_streams=2, max_pages=2)
+    b = cache.batch(i32([0, 3]), i32([0]), i32([3]), rows=3)
+    x = torch.zeros(3, 2, 64, dtype=torch.bfloat16, device=DEV)
+    w = cache.new_weights()
+    other = KV4Cache(2, 64, num_pages=4, num_streams=2, max_pages=2)
+    for i, bad in enumerate((lambda: KV4Cache(2, 80, num_pages=1, num_streams=1, max_pages=1), lambda: KV4Cache(2, 64, num_streams=1, max_pages=1),
+                lambda: KV4Cache(2, 64, num_pages=1), lambda: KV4Cache(2, 64, pool=cache.pool[:, :, :-1], block_table=cache.block_table),
+                lambda: KV4Cache(2, 64, pool=cache.pool[:, ::2], block_table=cache.block_table), lambda: KV4Cache(2, 64, pool=cache.pool.cpu(), block_table=cache.block_table),
+                lambda: KV4Cache(2, 64, pool=cache.pool, block_table=cache.block_table.long()), lambda: KV4Cache(2, 64, pool=cache.pool, block_table=cache.block_table.t()),
+                lambda: cache.batch(i32([0, 3]), i32([0, 1]), i32([3]), rows=3), lambda: cache.batch(torch.tensor([0, 3], device=DEV), i32([0]), i32([3]), rows=3),
+                lambda: cache.batch(i32([0, 3]).cpu(), i32([0]), i32([3]), rows=3),
+                lambda: cache.append(x.float(), x, b), lambda: cache.append(x, x.half(), b), lambda: cache.append(x[:2], x[:2], b), lambda: cache.append(x.cpu(), x, b),
+                lambda: cache.append(x.transpose(0, 1).contiguous().transpose(0, 1), x, b), lambda: cache.append(x[..., :32], x, b), lambda: cache.append(x, x, other.batch(i32([0, 3]), i32([0]), i32([3]), rows=3)),
+                lambda: cache.attend(x[:, :1], b), lambda: cache.attend(x[0], b), lambda: cache.attend(x, b, out=x.half()), lambda: cache.attend(x, b, out=x[:2]),
+                lambda: cache.attend(x, b, weights=w), lambda: cache.attend(x, b, weights=w[0].double()), lambda: cache.attend(x, b, weights=w[0, :1]),
+                lambda: cache.read(b, dtype=torch.float32), lambda: cache.read(b, n_layers=0),
+                lambda: cache.evict(i32([0]), i32([1, 0]), i32([3]), 2, 0, 0, w), lambda: cache.evict(i32([0]), i32([1]), i32([3]), 2, 0, 0, w[0]),
+                lambda: cache.evict(i32([0]), i32([1]), i32([3]), 0, 0, 0, w), lambda: cache.evict(i32([0]).long(), i32([1]), i32([3]), 2, 0, 0, w))):
+        try:
+            bad()
+        except ValueError:
+            continue
+        pytest.fail(f"call {i} was not refused")
+    for i, bad in enumerate((lambda: cache.append(x, x, b, layer=1), lambda: cache.attend(x, b, scale=-1.0), lambda: cache.attend(x, b, layer=-1), lambda: cache.read(b, n_layers=2),
+                lambda: cache.evict(i32([0]), i32([1]), i32([3]), 2, 2, 1, w), lambda: cache.evict(i32([0]), i32([1]), i32([3]), 500, 2, 1, w),
+                lambda: cache.append(torch.zeros(3 * 130, dtype=torch.bfloat16, device=DEV).as_strided((3, 2, 64), (130, 64, 1)), x, b))):
+        try:
+            bad()
+        except _capi.T3Error:
+            continue
+        pytest.fail(f"call {i} was not refused by the library")
+    with pytest.raises(ValueError):
+        page_bytes(2, 96)
+    torch.cuda.synchronize()
