@@ -17,15 +17,14 @@
 #include "kv4_common.h"
 
 #define KV4_FEW_COLUMNS 64        // rows x group up to which a sequence is cut along its cache
+#ifndef KV4_KEEP_COLUMNS
+#define KV4_KEEP_COLUMNS 16
+#endif
 #define KV4_NONE -1e30f           // running maximum before the first visible token
 
-// pages of a chunk
-KV4_FN int kv4_chunk_pages(int ctx) { return ctx > 8192 ? 16 : 8; }
-KV4_FN int kv4_chunks(int ctx) { const int p = (ctx + KV4_PAGE - 1) / KV4_PAGE, n = kv4_chunk_pages(ctx); return (p + n - 1) / n; }
-KV4_FN int kv4_max_chunks(int max_ctx) {                 // over all lengths up to max_ctx
-    const int a = kv4_chunks(max_ctx < 8192 ? max_ctx : 8192), b = kv4_chunks(max_ctx);
-    return a > b ? a : b;
-}
+// A chunk is 16 pages: the four waves of its workgroup take four each.
+#define KV4_CHUNK_PAGES 16
+KV4_FN int kv4_chunks(int ctx) { return (int)(((int64_t)ctx + KV4_CHUNK_PAGES * KV4_PAGE - 1) / (KV4_CHUNK_PAGES * KV4_PAGE)); }
 
 struct Kv4Attn {
     const uint16_t* q; int64_t q_stride;
@@ -34,6 +33,8 @@ struct Kv4Attn {
     float c;                      // scale * log2(e)
     float* states;                // [sequence][key head][tile][chunk] x kv4_state_floats
     f32x2* norm;                  // [rows][H]: m and 1 / l of each column, or null
+    float* scores;                // [sequence][key head][kept][width] raw scores of sequences of at most KV4_KEEP_COLUMNS columns, or null
+    int kept; int64_t width;      // columns and entries that buffer has room for
 };
 // state of (chunk, tile): m[16], l[16], O[16][hd]
 template <int HD> __device__ __forceinline__ int64_t kv4_state_at(const Kv4Attn& a, int Hkv, int seq, int h, int tile, int chunk) {
@@ -43,11 +44,14 @@ template <int HD> __device__ __forceinline__ int64_t kv4_state_at(const Kv4Attn&
 template <int HD> struct Kv4Page {
     u32x4 k[HD / 32], v[HD / 32], vs[HD / 64];
     unsigned ks;
-    __device__ __forceinline__ void load(const uint8_t* slab, int lane) {
+    __device__ __forceinline__ void load_k(const uint8_t* slab, int lane) {
         const int g = lane >> 4, r = lane & 15;
 #pragma unroll
         for (int x = 0; x < HD / 32; ++x) k[x] = *reinterpret_cast<const u32x4*>(slab + x * 1024 + lane * 16);
         ks = *reinterpret_cast<const unsigned*>(slab + 64 * HD + g * (HD / 4) / KV4_BLOCK * KV4_PAGE + 4 * r);
+    }
+    __device__ __forceinline__ void load_v(const uint8_t* slab, int lane) {
+        const int g = lane >> 4, r = lane & 15;
 #pragma unroll
         for (int x = 0; x < HD / 32; ++x) v[x] = *reinterpret_cast<const u32x4*>(slab + 32 * HD + x * 1024 + lane * 16);
 #pragma unroll
@@ -119,22 +123,34 @@ template <int HD, int NC> struct Kv4State {
     }
 };
 
-// One page.  seen[n]: tokens of this page that column tile n's column sees (>= 64: all); tail: tokens of the page that exist.
-template <int HD, bool F16, int NC, bool MASK>
-__device__ __forceinline__ void kv4_page_step(const Kv4Page<HD>& pg, const Kv4Query<HD, F16> (&q)[NC], Kv4State<HD, NC>& st,
-                                              const int (&seen)[NC], int tail, float c, int lane) {
-    const int g = lane >> 4;
-    f32x4 s[NC][4];
-    kv4_scores<HD, F16, NC>(pg, q, s);
-    bf16x8 ph[NC][2], pl[NC][2];
+// What a page that is not seen whole needs: scores of tokens behind a column's last one go to -inf (seen[n]: how many of the page
+// it sees), and the value scales behind the last entry of the stream to 0, for those bytes may be anything and 0 * finite is 0.
+template <int NC> __device__ __forceinline__ void kv4_hide_scores(f32x4 (&s)[NC][4], const int (&seen)[NC], int lane) {
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-        if constexpr (MASK) {
+        const int mine = seen[n] - 16 * (lane >> 4);              // of the lane's 16 tokens
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) s[n][i][j] = 16 * g + 4 * j + i < seen[n] ? s[n][i][j] : -INFINITY;
-        }
+            for (int j = 0; j < 4; ++j) s[n][i][j] = 4 * j + i < mine ? s[n][i][j] : -INFINITY;
+    }
+}
+template <int HD> __device__ __forceinline__ void kv4_hide_values(Kv4Page<HD>& pg, int tail, int lane) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const int mine = tail - 16 * (lane >> 4) - 4 * w;         // of the word's 4 tokens
+        const unsigned keep = mine >= 4 ? 0xffffffffu : mine <= 0 ? 0u : (1u << (8 * mine)) - 1u;
+#pragma unroll
+        for (int x = 0; x < HD / 64; ++x) pg.vs[x][w] &= keep;
+    }
+}
+
+// Probabilities of one page from its scores; the state's sums move to the new maximum.  ph + pl: slot y of step x is token
+// 16 g + 8 x + y.
+template <int HD, int NC>
+__device__ __forceinline__ void kv4_softmax(const f32x4 (&s)[NC][4], Kv4State<HD, NC>& st, float c, bf16x8 (&ph)[NC][2], bf16x8 (&pl)[NC][2]) {
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
         float top = s[n][0][0];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -162,6 +178,11 @@ __device__ __forceinline__ void kv4_page_step(const Kv4Page<HD>& pg, const Kv4Qu
 #pragma unroll
             for (int e = 0; e < 4; ++e) st.o[n][h][e] *= alpha;
     }
+}
+
+// O^T += V^T P^T of one page
+template <int HD, int NC>
+__device__ __forceinline__ void kv4_values(const Kv4Page<HD>& pg, const bf16x8 (&ph)[NC][2], const bf16x8 (&pl)[NC][2], Kv4State<HD, NC>& st) {
 #pragma unroll
     for (int h = 0; h < HD / 64; ++h)
 #pragma unroll
@@ -171,12 +192,7 @@ __device__ __forceinline__ void kv4_page_step(const Kv4Page<HD>& pg, const Kv4Qu
             for (int w = 0; w < 4; ++w) {
                 const unsigned codes = pg.v[2 * h + x][w];
                 const int t = 8 * x + 2 * w;                      // tokens 16 g + t, + t + 1
-                unsigned b0 = kv4_byte(pg.vs[h][t / 4], t % 4), b1 = kv4_byte(pg.vs[h][t / 4], t % 4 + 1);
-                if constexpr (MASK) {                             // what lies behind the last entry may be anything: 0 * finite
-                    b0 = 16 * g + t < tail ? b0 : 0u;
-                    b1 = 16 * g + t + 1 < tail ? b1 : 0u;
-                }
-                const float s0 = kv4_scale(b0), s1 = kv4_scale(b1);
+                const float s0 = kv4_scale(kv4_byte(pg.vs[h][t / 4], t % 4)), s1 = kv4_scale(kv4_byte(pg.vs[h][t / 4], t % 4 + 1));
                 const unsigned t0 = kv4_pair<0>(codes, s0), t0b = kv4_pair<1>(codes, s0);
                 const unsigned t1 = kv4_pair<2>(codes, s1), t1b = kv4_pair<3>(codes, s1);
                 a[0][w] = __builtin_amdgcn_perm(t1, t0, 0x05040100u);
@@ -206,12 +222,15 @@ template <bool F16> __device__ __forceinline__ unsigned kv4_pack2(float lo, floa
 }
 // A page of a stream.  An id outside the pool is not followed: the page then holds NaN keys, and values that a row which does not
 // see it can multiply by zero.
-template <int HD> __device__ __forceinline__ void kv4_fetch(Kv4Page<HD>& pg, const Kv4View& c, const int32_t* bt, int p, int h, int lane) {
-    const int page = __builtin_amdgcn_readfirstlane(bt[p]);
+template <int HD> __device__ __forceinline__ void kv4_fetch_k(Kv4Page<HD>& pg, const Kv4View& c, int page, int h, int lane) {
     const bool ok = kv4_page_ok(page, c.n_pages);
-    pg.load(c.pool + ((int64_t)(ok ? page : 0) * c.Hkv + h) * kv4_slab_bytes(HD), lane);
+    pg.load_k(c.pool + ((int64_t)(ok ? page : 0) * c.Hkv + h) * kv4_slab_bytes(HD), lane);
+    if (!ok) pg.ks = 0xffffffffu;
+}
+template <int HD> __device__ __forceinline__ void kv4_fetch_v(Kv4Page<HD>& pg, const Kv4View& c, int page, int h, int lane) {
+    const bool ok = kv4_page_ok(page, c.n_pages);
+    pg.load_v(c.pool + ((int64_t)(ok ? page : 0) * c.Hkv + h) * kv4_slab_bytes(HD), lane);
     if (!ok) {
-        pg.ks = 0xffffffffu;
 #pragma unroll
         for (int x = 0; x < HD / 64; ++x) pg.vs[x] = u32x4{0u, 0u, 0u, 0u};
     }
@@ -232,12 +251,12 @@ template <int HD> __device__ void kv4_fill_columns(const Kv4Attn& a, const Kv4Se
 // Few columns: one workgroup per (chunk, tile of 16 columns and key head, sequence).
 // ------------------------------------------------------------------------------------------------------------------
 template <int HD, bool F16>
-__global__ __launch_bounds__(256) void kv4_attn_few_kernel(Kv4View c, Kv4Rows b, Kv4Attn a) {
+__global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_few_kernel(Kv4View c, Kv4Rows b, Kv4Attn a) {
     __shared__ float sm[4][2][16];
     __shared__ __attribute__((aligned(16))) float so[4][16][HD + 4];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int h = blockIdx.y % c.Hkv, tile = blockIdx.y / c.Hkv, chunk = blockIdx.x, H = c.Hkv * a.group;
-    const Kv4Seq s = kv4_seq_of(b, c, blockIdx.z);
+    const int h = blockIdx.x % c.Hkv, tile = blockIdx.x / c.Hkv, chunk = blockIdx.z, H = c.Hkv * a.group;
+    const Kv4Seq s = kv4_seq_of(b, c, blockIdx.y);
     const int rows = s.n < b.max_rows ? s.n : b.max_rows;
     const int cols = rows * a.group;
     if (s.state == 1 || cols > KV4_FEW_COLUMNS || tile * 16 >= cols) return;
@@ -246,7 +265,7 @@ __global__ __launch_bounds__(256) void kv4_attn_few_kernel(Kv4View c, Kv4Rows b,
         if (chunk == 0) kv4_fill_columns<HD>(a, s, h, tile * 16, c1, tid, 256);
         return;
     }
-    const int chunks = kv4_chunks(s.ctx), per = kv4_chunk_pages(s.ctx);
+    const int chunks = kv4_chunks(s.ctx);
     if (chunk >= (chunks > 0 ? chunks : 1)) return;
 
     const int col = tile * 16 + (lane & 15), j = col / a.group, head = h * a.group + col % a.group;
@@ -257,14 +276,40 @@ __global__ __launch_bounds__(256) void kv4_attn_few_kernel(Kv4View c, Kv4Rows b,
     Kv4State<HD, 1> st;
     st.clear();
 
-    const int p0 = chunk * per, pages = (s.ctx + KV4_PAGE - 1) / KV4_PAGE, p1 = pages < p0 + per ? pages : p0 + per;
-    const int32_t* bt = c.table + (int64_t)s.stream * c.max_pages;
-    for (int p = p0 + w; p < p1; p += 4) {
-        Kv4Page<HD> pg;
-        kv4_fetch<HD>(pg, c, bt, p, h, lane);
-        const int first = p * KV4_PAGE, seen[1] = {sees - first};
-        if (least >= first + KV4_PAGE) kv4_page_step<HD, F16, 1, false>(pg, q, st, seen, KV4_PAGE, a.c, lane);
-        else kv4_page_step<HD, F16, 1, true>(pg, q, st, seen, s.ctx - first, a.c, lane);
+    const int p0 = chunk * KV4_CHUNK_PAGES, pages = (s.ctx + KV4_PAGE - 1) / KV4_PAGE;
+    const int np = pages - p0 < KV4_CHUNK_PAGES ? pages - p0 : KV4_CHUNK_PAGES;
+    // the chunk's page ids, one a lane.  The next page's keys are under way from when this one's have been used, its values
+    // likewise: half a step of other work covers each load, in the registers of one page
+    const int32_t* bt = c.table + (int64_t)s.stream * c.max_pages + p0;
+    const int ids = lane < np ? bt[lane] : -1;
+    // where the lane's 16 tokens' scores go, if they are wanted
+    float* keep = a.scores && cols <= KV4_KEEP_COLUMNS && col < cols
+                      ? a.scores + ((int64_t)(blockIdx.y * c.Hkv + h) * a.kept + col) * a.width + 16 * (lane >> 4) : nullptr;
+    Kv4Page<HD> pg;
+    if (w < np) {
+        const int id = __builtin_amdgcn_readlane(ids, w);
+        kv4_fetch_k<HD>(pg, c, id, h, lane);
+        kv4_fetch_v<HD>(pg, c, id, h, lane);
+    }
+    for (int p = w; p < np; p += 4) {
+        const int next = __builtin_amdgcn_readlane(ids, p + 4 < np ? p + 4 : p);
+        const int first = (p0 + p) * KV4_PAGE, seen[1] = {sees - first};
+        f32x4 sc[1][4];
+        bf16x8 ph[1][2], pl[1][2];
+        kv4_scores<HD, F16, 1>(pg, q, sc);
+        if (keep) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                *reinterpret_cast<f32x4*>(keep + first + 4 * x) = f32x4{sc[0][0][x], sc[0][1][x], sc[0][2][x], sc[0][3][x]};
+        }
+        if (p + 4 < np) kv4_fetch_k<HD>(pg, c, next, h, lane);
+        if (least < first + KV4_PAGE) {
+            kv4_hide_scores<1>(sc, seen, lane);
+            kv4_hide_values<HD>(pg, s.ctx - first, lane);
+        }
+        kv4_softmax<HD, 1>(sc, st, a.c, ph, pl);
+        kv4_values<HD, 1>(pg, ph, pl, st);
+        if (p + 4 < np) kv4_fetch_v<HD>(pg, c, next, h, lane);
     }
     float l = st.l[0];
     l += __shfl_xor(l, 16);
@@ -297,7 +342,7 @@ __global__ __launch_bounds__(256) void kv4_attn_few_kernel(Kv4View c, Kv4Rows b,
             for (int e = 0; e < 8; ++e) o[e] = fmaf(so[x][k][d + e], f, o[e]);
         }
         if (chunks > 1) {
-            float* sp = a.states + kv4_state_at<HD>(a, c.Hkv, blockIdx.z, h, tile, chunk);
+            float* sp = a.states + kv4_state_at<HD>(a, c.Hkv, blockIdx.y, h, tile, chunk);
             if (d == 0) { sp[k] = M; sp[16 + k] = L; }
 #pragma unroll
             for (int e = 0; e < 8; e += 4)
@@ -313,38 +358,54 @@ __global__ __launch_bounds__(256) void kv4_attn_few_kernel(Kv4View c, Kv4Rows b,
     }
 }
 
-// joins the chunks of a (sequence, key head, tile) in order; a thread 4 dims of a column
+// Joins the chunks of a column.  A thread has 4 dims; 1024 / HD groups of threads walk the chunks side by side, group x the chunks
+// x, x + groups, ..., and are then added in order.
 template <int HD, bool F16>
 __global__ __launch_bounds__(256) void kv4_attn_join_kernel(Kv4View c, Kv4Rows b, Kv4Attn a) {
-    const int h = blockIdx.x % c.Hkv, tile = blockIdx.x / c.Hkv, H = c.Hkv * a.group;
+    constexpr int T = HD / 4, GROUPS = 256 / T, step = 16 * (HD + 2);
+    __shared__ float sm[GROUPS][2];
+    __shared__ __attribute__((aligned(16))) f32x4 so[GROUPS][T];
+    const int h = blockIdx.x % c.Hkv, col = blockIdx.x / c.Hkv, H = c.Hkv * a.group;
     const Kv4Seq s = kv4_seq_of(b, c, blockIdx.y);
     const int rows = s.n < b.max_rows ? s.n : b.max_rows, cols = rows * a.group;
-    if (s.state || cols > KV4_FEW_COLUMNS || tile * 16 >= cols) return;
+    if (s.state || cols > KV4_FEW_COLUMNS || col >= cols) return;
     const int chunks = kv4_chunks(s.ctx);
     if (chunks <= 1) return;
-    const float* sp = a.states + kv4_state_at<HD>(a, c.Hkv, blockIdx.y, h, tile, 0);
-    constexpr int step = 16 * (HD + 2);
-    for (int i = threadIdx.x; i < 16 * (HD / 4); i += 256) {
-        const int k = i / (HD / 4), d = i % (HD / 4) * 4, col = tile * 16 + k;
-        if (col >= cols) continue;
-        float M = sp[k];
-        for (int x = 1; x < chunks; ++x) M = fmaxf(M, sp[(int64_t)x * step + k]);
-        float L = 0.f;
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        for (int x = 0; x < chunks; ++x) {
-            const float* p = sp + (int64_t)x * step;
-            const float f = __builtin_amdgcn_exp2f(p[k] - M);
-            L = fmaf(p[16 + k], f, L);
-            const f32x4 v = *reinterpret_cast<const f32x4*>(p + 32 + k * HD + d);
+    const int k = col & 15, group = threadIdx.x / T, t = threadIdx.x % T;
+    const float* sp = a.states + kv4_state_at<HD>(a, c.Hkv, blockIdx.y, h, col >> 4, 0);
+    float M = KV4_NONE, L = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int x = group; x < chunks; x += GROUPS) {
+        const float* p = sp + (int64_t)x * step;
+        const float m = p[k], l = p[16 + k];
+        const f32x4 v = *reinterpret_cast<const f32x4*>(p + 32 + k * HD + 4 * t);
+        const float top = fmaxf(M, m), f0 = __builtin_amdgcn_exp2f(M - top), f1 = __builtin_amdgcn_exp2f(m - top);
+        L = fmaf(L, f0, l * f1);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = fmaf(v[e], f, o[e]);
-        }
-        const int j = col / a.group, head = h * a.group + col % a.group;
-        const float inv = L == 0.f ? 0.f : 1.0f / L;
-        const u32x2 r = {kv4_pack2<F16>(o[0] * inv, o[1] * inv), kv4_pack2<F16>(o[2] * inv, o[3] * inv)};
-        *reinterpret_cast<u32x2*>(a.out + (int64_t)(s.start + j) * a.out_stride + head * HD + d) = r;
-        if (a.norm && d == 0) a.norm[(int64_t)(s.start + j) * H + head] = f32x2{M, inv};
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(o[e], f0, v[e] * f1);
+        M = top;
     }
+    if (t == 0) { sm[group][0] = M; sm[group][1] = L; }
+    so[group][t] = o;
+    __syncthreads();
+    if (threadIdx.x >= T) return;
+    M = sm[0][0];
+#pragma unroll
+    for (int x = 1; x < GROUPS; ++x) M = fmaxf(M, sm[x][0]);
+    L = 0.f;
+    o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < GROUPS; ++x) {
+        const float f = __builtin_amdgcn_exp2f(sm[x][0] - M);
+        L = fmaf(sm[x][1], f, L);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(so[x][t][e], f, o[e]);
+    }
+    const int j = col / a.group, head = h * a.group + col % a.group;
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
+    const u32x2 r = {kv4_pack2<F16>(o[0] * inv, o[1] * inv), kv4_pack2<F16>(o[2] * inv, o[3] * inv)};
+    *reinterpret_cast<u32x2*>(a.out + (int64_t)(s.start + j) * a.out_stride + head * HD + 4 * t) = r;
+    if (a.norm && t == 0) a.norm[(int64_t)(s.start + j) * H + head] = f32x2{M, inv};
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -375,12 +436,21 @@ __global__ __launch_bounds__(256) void kv4_attn_many_kernel(Kv4View c, Kv4Rows b
     st.clear();
     const int32_t* bt = c.table + (int64_t)s.stream * c.max_pages;
     for (int first = 0; first < most; first += KV4_PAGE) {
+        const int id = __builtin_amdgcn_readfirstlane(bt[first / KV4_PAGE]);
         Kv4Page<HD> pg;
-        kv4_fetch<HD>(pg, c, bt, first / KV4_PAGE, h, lane);
+        kv4_fetch_k<HD>(pg, c, id, h, lane);
+        kv4_fetch_v<HD>(pg, c, id, h, lane);
 #pragma unroll
         for (int n = 0; n < NC; ++n) seen[n] = sees[n] - first;
-        if (least >= first + KV4_PAGE) kv4_page_step<HD, F16, NC, false>(pg, q, st, seen, KV4_PAGE, a.c, lane);
-        else kv4_page_step<HD, F16, NC, true>(pg, q, st, seen, s.ctx - first, a.c, lane);
+        f32x4 sc[NC][4];
+        bf16x8 ph[NC][2], pl[NC][2];
+        kv4_scores<HD, F16, NC>(pg, q, sc);
+        if (least < first + KV4_PAGE) {
+            kv4_hide_scores<NC>(sc, seen, lane);
+            kv4_hide_values<HD>(pg, s.ctx - first, lane);
+        }
+        kv4_softmax<HD, NC>(sc, st, a.c, ph, pl);
+        kv4_values<HD, NC>(pg, ph, pl, st);
     }
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
@@ -406,41 +476,82 @@ __global__ __launch_bounds__(256) void kv4_attn_many_kernel(Kv4View c, Kv4Rows b
 
 // ------------------------------------------------------------------------------------------------------------------
 // Weights: W[stream][key head][t] += sum over the sequence's columns of exp2(s c - m) / l.  One wave per (page, key head, stream)
-// forms the scores again from K (half a page's bytes, mostly still on the chip) and walks the columns in order, so no atomics.
+// walks the columns in order, so there are no atomics.  Scores of sequences of few columns were kept by the pass above; the others
+// are formed again from K (half a page's bytes, mostly still on the chip).
 // A stream that occurs in several sequences of the call is done, in their order, by the waves of the first of them.
 // ------------------------------------------------------------------------------------------------------------------
+// Walks the sequences of `stream` from `seq` on, 64 looked at at a time: fn(sequence index).  False if an earlier one has it.
+template <typename Fn> __device__ __forceinline__ bool kv4_of_stream(const Kv4Rows& b, int seq, int stream, int lane, Fn fn) {
+    for (int i = lane; i - lane < seq; i += 64)
+        if (__any(i < seq && b.stream[i < seq ? i : 0] == stream)) return false;
+    for (int i0 = seq; i0 < b.n_seqs; i0 += 64) {
+        const int i = i0 + lane;
+        uint64_t todo = __ballot(i < b.n_seqs && b.stream[i < b.n_seqs ? i : seq] == stream);
+        for (; todo; todo &= todo - 1) fn(i0 + __builtin_ctzll(todo));
+    }
+    return true;
+}
+
+// Every sequence of the call has its scores kept: a thread four entries.
+__global__ __launch_bounds__(256) void kv4_weights_kept_kernel(Kv4View c, Kv4Rows b, Kv4Attn a, float* weights, int64_t weights_stride) {
+    const int lane = threadIdx.x & 63, h = blockIdx.y, H = c.Hkv * a.group, seq = blockIdx.z, stream = b.stream[seq];
+    if (stream < 0 || stream >= c.n_streams) return;
+    const int first = (blockIdx.x * 256 + threadIdx.x) * 4;
+    f32x4 mine = {0.f, 0.f, 0.f, 0.f};
+    const bool own = kv4_of_stream(b, seq, stream, lane, [&](int i) {
+        const Kv4Seq s = kv4_seq_of(b, c, i);
+        if (s.state || first >= s.ctx) return;
+        const int rows = s.n < b.max_rows ? s.n : b.max_rows, cols = rows * a.group;
+        const float* sp = a.scores + (int64_t)(i * c.Hkv + h) * a.kept * a.width + first;
+        for (int col = 0; col < cols; ++col) {
+            const int j = col / a.group, seen = s.ctx - s.n + j + 1 - first;
+            const f32x2 norm = a.norm[(int64_t)(s.start + j) * H + h * a.group + col % a.group];
+            const f32x4 x = *reinterpret_cast<const f32x4*>(sp + col * a.width);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float v = __builtin_amdgcn_exp2f(fmaf(x[e], a.c, -norm[0]));
+                mine[e] += e < seen ? v * norm[1] : 0.f;
+            }
+        }
+    });
+    if (!own) return;
+    float* wp = weights + ((int64_t)stream * c.Hkv + h) * weights_stride + first;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (mine[e] != 0.f && first + e < weights_stride) wp[e] += mine[e];
+}
+
 template <int HD, bool F16>
 __global__ __launch_bounds__(256) void kv4_weights_kernel(Kv4View c, Kv4Rows b, Kv4Attn a, float* weights, int64_t weights_stride) {
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.y, H = c.Hkv * a.group, seq = blockIdx.z, p = blockIdx.x * 4 + w, first = p * KV4_PAGE;
     const int stream = b.stream[seq];
     if (stream < 0 || stream >= c.n_streams) return;
-    for (int i = lane; i - lane < seq; i += 64)
-        if (__any(i < seq && b.stream[i < seq ? i : 0] == stream)) return;      // an earlier sequence's waves do it
     const int32_t* bt = c.table + (int64_t)stream * c.max_pages;
     Kv4Page<HD> pg;
     bool have = false;
-    float sum[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) sum[e] = 0.f;
-    // the sequences of this stream from here on, found 64 at a time
-    uint64_t todo = 0;
-    for (int i0 = seq - 64, i; ; ) {
-        while (todo == 0) {
-            i0 += 64;
-            if (i0 >= b.n_seqs) break;
-            todo = __ballot(i0 + lane < b.n_seqs && b.stream[i0 + lane < b.n_seqs ? i0 + lane : seq] == stream);
-        }
-        if (todo == 0) break;
-        i = i0 + __builtin_ctzll(todo);
-        todo &= todo - 1;
+    float mine = 0.f;                                             // of token first + lane
+    const bool own = kv4_of_stream(b, seq, stream, lane, [&](int i) {
         const Kv4Seq s = kv4_seq_of(b, c, i);
-        if (s.state || first >= s.ctx) continue;
+        if (s.state || first >= s.ctx) return;
+        const int rows = s.n < b.max_rows ? s.n : b.max_rows, cols = rows * a.group;
+        if (a.scores && cols <= KV4_KEEP_COLUMNS) {
+            const float* sp = a.scores + (int64_t)(i * c.Hkv + h) * a.kept * a.width + first + lane;
+            for (int col = 0; col < cols; ++col) {
+                const int j = col / a.group;
+                const f32x2 norm = a.norm[(int64_t)(s.start + j) * H + h * a.group + col % a.group];
+                const float v = __builtin_amdgcn_exp2f(fmaf(sp[col * a.width], a.c, -norm[0]));
+                mine += first + lane < s.ctx - s.n + j + 1 ? v * norm[1] : 0.f;
+            }
+            return;
+        }
         if (!have) {
-            kv4_fetch<HD>(pg, c, bt, p, h, lane);
+            kv4_fetch_k<HD>(pg, c, __builtin_amdgcn_readfirstlane(bt[p]), h, lane);
             have = true;
         }
-        const int rows = s.n < b.max_rows ? s.n : b.max_rows, cols = rows * a.group;
+        float sum[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sum[e] = 0.f;
         // rows before the first that sees this page add nothing
         int j0 = first - (s.ctx - s.n);
         j0 = j0 < 0 ? 0 : j0;
@@ -459,21 +570,18 @@ __global__ __launch_bounds__(256) void kv4_weights_kernel(Kv4View c, Kv4Rows b, 
                 sum[e] += 16 * (lane >> 4) + e < seen ? v * norm[1] : 0.f;
             }
         }
-    }
-    if (!have) return;
+        // over the 16 columns; lane r of a group takes token 16 g + r
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        sum[e] += __shfl_xor(sum[e], 1);
-        sum[e] += __shfl_xor(sum[e], 2);
-        sum[e] += __shfl_xor(sum[e], 4);
-        sum[e] += __shfl_xor(sum[e], 8);
-    }
-    // lane r of the group keeps token 16 g + r
-    float mine = 0.f;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) mine = (lane & 15) == e ? sum[e] : mine;
+        for (int e = 0; e < 16; ++e) {
+            sum[e] += __shfl_xor(sum[e], 1);
+            sum[e] += __shfl_xor(sum[e], 2);
+            sum[e] += __shfl_xor(sum[e], 4);
+            sum[e] += __shfl_xor(sum[e], 8);
+            mine += (lane & 15) == e ? sum[e] : 0.f;
+        }
+    });
     const int64_t t = first + lane;
-    if (t < weights_stride) {
+    if (own && t < weights_stride) {
         float* wp = weights + ((int64_t)stream * c.Hkv + h) * weights_stride + t;
         if (mine != 0.f) *wp += mine;
     }
@@ -482,12 +590,22 @@ __global__ __launch_bounds__(256) void kv4_weights_kernel(Kv4View c, Kv4Rows b, 
 // ------------------------------------------------------------------------------------------------------------------
 // Entry points
 // ------------------------------------------------------------------------------------------------------------------
-static int64_t states_bytes(const t3_kv4_cache* c, const t3_kv4_batch* b, int H, int* tiles, int* chunks) {
+// the work buffer: chunk states | kept scores | m and 1 / l
+struct Kv4Work { int64_t states, scores, norm, width; int tiles, chunks, kept; };
+static Kv4Work plan_work(const t3_kv4_cache* c, const t3_kv4_batch* b, int H, bool weights) {
+    Kv4Work w{};
     const int64_t cols = (int64_t)b->max_rows * (H / c->Hkv), few = cols < KV4_FEW_COLUMNS ? cols : KV4_FEW_COLUMNS;
-    const int64_t cap = (int64_t)c->max_pages * KV4_PAGE;
-    *tiles = (int)((few + 15) / 16);
-    *chunks = kv4_max_chunks((int)(b->max_ctx < cap ? b->max_ctx : cap));
-    return *chunks > 1 ? (int64_t)b->n_seqs * c->Hkv * *tiles * *chunks * (16 * (c->hd + 2)) * 4 : 0;
+    const int64_t cap = (int64_t)c->max_pages * KV4_PAGE, most = b->max_ctx < cap ? b->max_ctx : cap, pairs = (int64_t)b->n_seqs * c->Hkv;
+    w.tiles = (int)((few + 15) / 16);
+    w.chunks = kv4_chunks((int)most);
+    w.states = w.chunks > 1 ? pairs * w.tiles * w.chunks * (16 * (c->hd + 2)) * 4 : 0;
+    if (weights) {
+        w.kept = (int)(few < KV4_KEEP_COLUMNS ? few : KV4_KEEP_COLUMNS);
+        w.width = (most + KV4_PAGE - 1) / KV4_PAGE * KV4_PAGE;
+        w.scores = pairs * w.kept * w.width * 4;
+        w.norm = (int64_t)b->rows * H * 8;
+    }
+    return w;
 }
 static int check_heads(const t3_kv4_cache* c, int H) {
     T3_REQUIRE(H >= c->Hkv && H % c->Hkv == 0 && H / c->Hkv <= 64, "attn_kv4: query heads must be 1..64 times the key heads");
@@ -496,22 +614,25 @@ static int check_heads(const t3_kv4_cache* c, int H) {
 
 extern "C" int64_t t3_op_attn_kv4_work_bytes(const t3_kv4_cache* cache, const t3_kv4_batch* batch, int32_t H, int32_t with_weights) {
     if (kv4_check_cache(cache, 0, 1, nullptr) || kv4_check_batch(batch) || check_heads(cache, H)) return -1;
-    int tiles, chunks;
-    return states_bytes(cache, batch, H, &tiles, &chunks) + (with_weights ? ((int64_t)batch->rows * H * 8 + 15) / 16 * 16 : 0);
+    const Kv4Work w = plan_work(cache, batch, H, with_weights != 0);
+    return (w.states + w.scores + w.norm + 15) / 16 * 16;
 }
 
 template <int HD, bool F16>
 static int launch_attn(const Kv4View& c, const Kv4Rows& b, const Kv4Attn& a, float* weights, int64_t weights_stride, hipStream_t st) {
     constexpr int NC = 4;
     const int64_t cols = (int64_t)b.max_rows * a.group;
-    T3_LAUNCH((kv4_attn_few_kernel<HD, F16>), dim3(a.chunks, a.tiles * c.Hkv, b.n_seqs), dim3(256), 0, st, c, b, a);
+    T3_LAUNCH((kv4_attn_few_kernel<HD, F16>), dim3(a.tiles * c.Hkv, b.n_seqs, a.chunks), dim3(256), 0, st, c, b, a);
     if (a.chunks > 1)
-        T3_LAUNCH((kv4_attn_join_kernel<HD, F16>), dim3(a.tiles * c.Hkv, b.n_seqs), dim3(256), 0, st, c, b, a);
+        T3_LAUNCH((kv4_attn_join_kernel<HD, F16>), dim3((cols < KV4_FEW_COLUMNS ? (int)cols : KV4_FEW_COLUMNS) * c.Hkv, b.n_seqs), dim3(256), 0, st, c, b, a);
     if (cols > KV4_FEW_COLUMNS)
         T3_LAUNCH((kv4_attn_many_kernel<HD, F16, NC>), dim3((unsigned)((cols + 64 * NC - 1) / (64 * NC)), c.Hkv, b.n_seqs), dim3(256), 0, st, c, b, a);
     if (weights) {
         const int64_t cap = (int64_t)c.max_pages * KV4_PAGE, most = b.max_ctx < cap ? b.max_ctx : cap;
-        T3_LAUNCH((kv4_weights_kernel<HD, F16>), dim3((unsigned)((most + 4 * KV4_PAGE - 1) / (4 * KV4_PAGE)), c.Hkv, b.n_seqs), dim3(256), 0, st,
+        if (cols <= KV4_KEEP_COLUMNS)
+            T3_LAUNCH(kv4_weights_kept_kernel, dim3((unsigned)((most + 1023) / 1024), c.Hkv, b.n_seqs), dim3(256), 0, st, c, b, a, weights, weights_stride);
+        else
+            T3_LAUNCH((kv4_weights_kernel<HD, F16>), dim3((unsigned)((most + 4 * KV4_PAGE - 1) / (4 * KV4_PAGE)), c.Hkv, b.n_seqs), dim3(256), 0, st,
                   c, b, a, weights, weights_stride);
     }
     T3_HIP_CHECK(hipGetLastError());
@@ -540,9 +661,12 @@ extern "C" int t3_op_attn_kv4(const t3_kv4_cache* cache, const t3_kv4_batch* bat
     a.out = static_cast<uint16_t*>(out_dev); a.out_stride = out_stride;
     a.group = H / cache->Hkv;
     a.c = scale * 1.44269504088896340736f;
-    const int64_t sb = states_bytes(cache, batch, H, &a.tiles, &a.chunks);
-    a.states = static_cast<float*>(work_dev);
-    a.norm = weights_dev ? reinterpret_cast<f32x2*>(static_cast<uint8_t*>(work_dev) + sb) : nullptr;
+    const Kv4Work w = plan_work(cache, batch, H, weights_dev != nullptr);
+    uint8_t* work = static_cast<uint8_t*>(work_dev);
+    a.tiles = w.tiles; a.chunks = w.chunks; a.kept = w.kept; a.width = w.width;
+    a.states = reinterpret_cast<float*>(work);
+    a.scores = w.scores ? reinterpret_cast<float*>(work + w.states) : nullptr;
+    a.norm = weights_dev ? reinterpret_cast<f32x2*>(work + w.states + w.scores) : nullptr;
     const Kv4View c = kv4_view(cache, layer);
     const Kv4Rows b = kv4_rows(batch);
     if (cache->hd == 64) return dtype ? launch_attn<64, true>(c, b, a, weights_dev, weights_stride, st) : launch_attn<64, false>(c, b, a, weights_dev, weights_stride, st);
