@@ -16,6 +16,8 @@
 // row's bits do not depend on the batch.  Longer ones (prompts) run whole: a wave keeps four column tiles and walks the cache.
 #include "kv4_common.h"
 
+#include <type_traits>
+
 #define KV4_FEW_COLUMNS 64        // rows x group up to which a sequence is cut along its cache
 #ifndef KV4_KEEP_COLUMNS
 #define KV4_KEEP_COLUMNS 16
@@ -44,6 +46,7 @@ template <int HD> __device__ __forceinline__ int64_t kv4_state_at(const Kv4Attn&
 template <int HD> struct Kv4Page {
     u32x4 k[HD / 32], v[HD / 32], vs[HD / 64];
     unsigned ks;
+    unsigned bad_k, good_v;                                       // all ones or all zeros, the same in every lane
     __device__ __forceinline__ void load_k(const uint8_t* slab, int lane) {
         const int g = lane >> 4, r = lane & 15;
 #pragma unroll
@@ -87,9 +90,10 @@ template <int HD, bool F16> struct Kv4Query {
 // S^T of a page for NC column tiles: s[n][i][j] = token 16 g + 4 j + i, column lane & 15
 template <int HD, bool F16, int NC>
 __device__ __forceinline__ void kv4_scores(const Kv4Page<HD>& pg, const Kv4Query<HD, F16> (&q)[NC], f32x4 (&s)[NC][4]) {
+    const unsigned ks = pg.ks | pg.bad_k;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float sc = kv4_scale(kv4_byte(pg.ks, i));
+        const float sc = kv4_scale(kv4_byte(ks, i));
 #pragma unroll
         for (int n = 0; n < NC; ++n) s[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -145,6 +149,28 @@ template <int HD> __device__ __forceinline__ void kv4_hide_values(Kv4Page<HD>& p
     }
 }
 
+// over the four lane groups
+__device__ __forceinline__ float kv4_group_max(float x) {
+    const unsigned u = __float_as_uint(x);
+    const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const unsigned v = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+    const auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float kv4_group_sum(float x) {
+    const unsigned u = __float_as_uint(x);
+    const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const unsigned v = __float_as_uint(__uint_as_float(a[0]) + __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+// two values as bf16 hi and lo parts, one word each
+__device__ __forceinline__ void kv4_split(float p0, float p1, unsigned& hi, unsigned& lo) {
+    typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+    hi = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{p0, p1}), bf16x2));
+    lo = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{p0 - bf_lo(hi), p1 - bf_hi(hi)}), bf16x2));
+}
+
 // Probabilities of one page from its scores; the state's sums move to the new maximum.  ph + pl: slot y of step x is token
 // 16 g + 8 x + y.
 template <int HD, int NC>
@@ -156,22 +182,25 @@ __device__ __forceinline__ void kv4_softmax(const f32x4 (&s)[NC][4], Kv4State<HD
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) top = fmaxf(top, s[n][i][j]);
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float m = fmaxf(st.m[n], top * c), alpha = __builtin_amdgcn_exp2f(st.m[n] - m);
+        const float m = fmaxf(st.m[n], kv4_group_max(top) * c), alpha = __builtin_amdgcn_exp2f(st.m[n] - m);
         st.m[n] = m;
         float sum = 0.f;
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+        for (int x = 0; x < 2; ++x) {
+            u32x4 hi, lo;
 #pragma unroll
-            for (int y = 0; y < 8; ++y) {
-                const int e = 8 * x + y;                          // token 16 g + e
-                const float p = __builtin_amdgcn_exp2f(fmaf(s[n][e & 3][e >> 2], c, -m));
-                sum += p;
-                const __bf16 hi = (__bf16)p;
-                ph[n][x][y] = hi;
-                pl[n][x][y] = (__bf16)(p - (float)hi);
+            for (int y = 0; y < 8; y += 2) {
+                const int e = 8 * x + y;                          // tokens 16 g + e, + e + 1
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[n][e & 3][e >> 2], c, -m));
+                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[n][(e & 3) + 1][e >> 2], c, -m));
+                sum += p0 + p1;
+                unsigned h, l;
+                kv4_split(p0, p1, h, l);
+                hi[y / 2] = h; lo[y / 2] = l;
             }
+            ph[n][x] = __builtin_bit_cast(bf16x8, hi);
+            pl[n][x] = __builtin_bit_cast(bf16x8, lo);
+        }
         st.l[n] = fmaf(st.l[n], alpha, sum);
 #pragma unroll
         for (int h = 0; h < HD / 64; ++h)
@@ -192,7 +221,8 @@ __device__ __forceinline__ void kv4_values(const Kv4Page<HD>& pg, const bf16x8 (
             for (int w = 0; w < 4; ++w) {
                 const unsigned codes = pg.v[2 * h + x][w];
                 const int t = 8 * x + 2 * w;                      // tokens 16 g + t, + t + 1
-                const float s0 = kv4_scale(kv4_byte(pg.vs[h][t / 4], t % 4)), s1 = kv4_scale(kv4_byte(pg.vs[h][t / 4], t % 4 + 1));
+                const unsigned vs = pg.vs[h][t / 4] & pg.good_v;
+                const float s0 = kv4_scale(kv4_byte(vs, t % 4)), s1 = kv4_scale(kv4_byte(vs, t % 4 + 1));
                 const unsigned t0 = kv4_pair<0>(codes, s0), t0b = kv4_pair<1>(codes, s0);
                 const unsigned t1 = kv4_pair<2>(codes, s1), t1b = kv4_pair<3>(codes, s1);
                 a[0][w] = __builtin_amdgcn_perm(t1, t0, 0x05040100u);
@@ -221,19 +251,17 @@ template <bool F16> __device__ __forceinline__ unsigned kv4_pack2(float lo, floa
     }
 }
 // A page of a stream.  An id outside the pool is not followed: the page then holds NaN keys, and values that a row which does not
-// see it can multiply by zero.
+// see it can multiply by zero.  `bad` is applied where the bytes are used, so that nothing waits for a load when it is issued.
+template <int HD> __device__ __forceinline__ const uint8_t* kv4_slab_of(const Kv4View& c, int page, int h) {
+    return c.pool + ((int64_t)(kv4_page_ok(page, c.n_pages) ? page : 0) * c.Hkv + h) * kv4_slab_bytes(HD);
+}
 template <int HD> __device__ __forceinline__ void kv4_fetch_k(Kv4Page<HD>& pg, const Kv4View& c, int page, int h, int lane) {
-    const bool ok = kv4_page_ok(page, c.n_pages);
-    pg.load_k(c.pool + ((int64_t)(ok ? page : 0) * c.Hkv + h) * kv4_slab_bytes(HD), lane);
-    if (!ok) pg.ks = 0xffffffffu;
+    pg.bad_k = kv4_page_ok(page, c.n_pages) ? 0u : 0xffffffffu;
+    pg.load_k(kv4_slab_of<HD>(c, page, h), lane);
 }
 template <int HD> __device__ __forceinline__ void kv4_fetch_v(Kv4Page<HD>& pg, const Kv4View& c, int page, int h, int lane) {
-    const bool ok = kv4_page_ok(page, c.n_pages);
-    pg.load_v(c.pool + ((int64_t)(ok ? page : 0) * c.Hkv + h) * kv4_slab_bytes(HD), lane);
-    if (!ok) {
-#pragma unroll
-        for (int x = 0; x < HD / 64; ++x) pg.vs[x] = u32x4{0u, 0u, 0u, 0u};
-    }
+    pg.good_v = kv4_page_ok(page, c.n_pages) ? 0xffffffffu : 0u;
+    pg.load_v(kv4_slab_of<HD>(c, page, h), lane);
 }
 // bits of a NaN in both halves of a word, of either type
 #define KV4_NAN2 0x7fff7fffu
@@ -291,9 +319,10 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_few_kernel(Kv4
         kv4_fetch_k<HD>(pg, c, id, h, lane);
         kv4_fetch_v<HD>(pg, c, id, h, lane);
     }
-    for (int p = w; p < np; p += 4) {
-        const int next = __builtin_amdgcn_readlane(ids, p + 4 < np ? p + 4 : p);
+    // (the last page has a body of its own: a load under a condition would make every wait below one for all loads)
+    const auto step = [&](int p, auto more) {
         const int first = (p0 + p) * KV4_PAGE, seen[1] = {sees - first};
+        const int next = more() ? __builtin_amdgcn_readlane(ids, p + 4) : 0;
         f32x4 sc[1][4];
         bf16x8 ph[1][2], pl[1][2];
         kv4_scores<HD, F16, 1>(pg, q, sc);
@@ -302,18 +331,20 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_few_kernel(Kv4
             for (int x = 0; x < 4; ++x)
                 *reinterpret_cast<f32x4*>(keep + first + 4 * x) = f32x4{sc[0][0][x], sc[0][1][x], sc[0][2][x], sc[0][3][x]};
         }
-        if (p + 4 < np) kv4_fetch_k<HD>(pg, c, next, h, lane);
+        if constexpr (more()) kv4_fetch_k<HD>(pg, c, next, h, lane);
         if (least < first + KV4_PAGE) {
             kv4_hide_scores<1>(sc, seen, lane);
             kv4_hide_values<HD>(pg, s.ctx - first, lane);
         }
         kv4_softmax<HD, 1>(sc, st, a.c, ph, pl);
         kv4_values<HD, 1>(pg, ph, pl, st);
-        if (p + 4 < np) kv4_fetch_v<HD>(pg, c, next, h, lane);
-    }
+        if constexpr (more()) kv4_fetch_v<HD>(pg, c, next, h, lane);
+    };
+    int p = w;
+    for (; p + 4 < np; p += 4) step(p, std::true_type{});
+    if (p < np) step(p, std::false_type{});
     float l = st.l[0];
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+    l = kv4_group_sum(l);
     const int g = lane >> 4, cc = lane & 15;
     if (g == 0) { sm[w][0][cc] = st.m[0]; sm[w][1][cc] = l; }
 #pragma unroll
@@ -456,8 +487,7 @@ __global__ __launch_bounds__(256) void kv4_attn_many_kernel(Kv4View c, Kv4Rows b
     for (int n = 0; n < NC; ++n) {
         const int col = c0 + 16 * n + (lane & 15), j = col / a.group, head = h * a.group + col % a.group, g = lane >> 4;
         float l = st.l[n];
-        l += __shfl_xor(l, 16);
-        l += __shfl_xor(l, 32);
+        l = kv4_group_sum(l);
         if (col >= c1) continue;
         const float inv = l == 0.f ? 0.f : 1.0f / l;
         uint16_t* op = a.out + (int64_t)(s.start + j) * a.out_stride + head * HD + 16 * g;
