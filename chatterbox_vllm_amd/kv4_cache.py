@@ -20,6 +20,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch._C import _cuda_getCurrentRawStream as _raw_stream    # the handle alone: a Stream object costs 2 us a call
 
 from . import _capi
 
@@ -52,7 +53,7 @@ class KV4Batch:
         self._tensors = (seq_start, streams, ctx)                # keeps the addresses below alive
         self._c = _capi.T3Kv4Batch(seq_start.data_ptr(), streams.data_ptr(), ctx.data_ptr(), n, rows, self.max_rows, self.max_ctx)
         self._ref = C.byref(self._c)
-        self._work = {}                                          # (heads, with weights) -> bytes of the work buffer
+        self._work = {}                                          # heads (negative: with weights) -> bytes of the work buffer
 
 
 class KV4Cache:
@@ -78,10 +79,11 @@ class KV4Cache:
             raise ValueError("the pages of a layer must lie one behind the other")
         if pool.device.type != "cuda":
             raise ValueError(f"the pool must be on the GPU, got {pool.device}")
-        self.device = pool.device
+        self.device, self._index = pool.device, pool.device.index
         if block_table.dim() != 2 or block_table.numel() < 1:
             raise ValueError("block_table must be [streams, max_pages]")
         self._int32("block_table", block_table, block_table.numel())
+        self._scale = 1.0 / math.sqrt(head_dim)
         self.num_kv_heads, self.head_dim, self.pool, self.block_table = num_kv_heads, head_dim, pool, block_table
         self.num_layers, self.num_pages = pool.shape[0], pool.shape[1]
         self.num_streams, self.max_pages = block_table.shape
@@ -113,29 +115,28 @@ class KV4Cache:
         multiple of kv_heads.  ``scale`` defaults to head_dim ** -0.5.  ``weights`` (fp32 [streams, kv_heads, width], one layer of
         ``new_weights()``): the softmax weights of every entry are added to it.  Returns ``out``, by default a new tensor in which
         rows of no sequence are undefined."""
-        if q.dim() != 3 or q.shape[1] % self.num_kv_heads or q.shape[1] == 0:
+        heads = q.shape[1] if q.dim() == 3 else 0
+        if heads == 0 or heads % self.num_kv_heads:
             raise ValueError(f"q must be [rows, heads, {self.head_dim}] with heads a multiple of {self.num_kv_heads}, got {tuple(q.shape)}")
-        heads = q.shape[1]
         dtype = self._rows("q", q, batch, heads)
         if out is None:
-            out = torch.empty((q.shape[0], heads, self.head_dim), dtype=q.dtype, device=self.device)
+            out = torch.empty_like(q)                            # dense, or q's own row stride where q is
         elif self._rows("out", out, batch, heads) != dtype:
             raise ValueError("out must have q's type")
         w_ptr, w_stride = None, 0
         if weights is not None:
             self._weights(weights, 3)
             w_ptr, w_stride = weights.data_ptr(), weights.stride(1)
-        key = (heads, weights is not None)
-        size = batch._work.get(key)
+        size = batch._work.get(heads if weights is None else -heads)
         if size is None:
             size = self._lib.t3_op_attn_kv4_work_bytes(self._ref, batch._ref, heads, int(weights is not None))
             if size < 0:
                 _capi.check(self._lib, 1)
-            batch._work[key] = size
+            batch._work[heads if weights is None else -heads] = size
         # a buffer of this call's own: calls on other streams and captured graphs get others
         work = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
         self._run(self._lib.t3_op_attn_kv4, self._ref, batch._ref, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), heads,
-                  dtype, scale if scale is not None else 1.0 / math.sqrt(self.head_dim), w_ptr, w_stride,
+                  dtype, self._scale if scale is None else scale, w_ptr, w_stride,
                   work.data_ptr() if size else None, size, layer)
         return out
 
@@ -185,10 +186,12 @@ class KV4Cache:
 
     # -- checks ------------------------------------------------------------------------------------------------------
     def _run(self, fn, *args) -> None:
-        if torch.cuda.current_device() != self.device.index:
-            with torch.cuda.device(self.device):
+        if torch.cuda.current_device() != self._index:
+            with torch.cuda.device(self._index):
                 return self._run(fn, *args)
-        _capi.check(self._lib, fn(*args, torch.cuda.current_stream(self.device).cuda_stream))
+        status = fn(*args, _raw_stream(self._index))
+        if status:
+            _capi.check(self._lib, status)
 
     def _int32(self, name: str, t: torch.Tensor, size: int) -> None:
         if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() != size or size < 1 or t.device != self.device:
@@ -199,12 +202,13 @@ class KV4Cache:
             raise ValueError("the batch belongs to another cache")
 
     def _rows(self, name: str, t: torch.Tensor, batch: KV4Batch, heads: int) -> int:
-        self._batch(batch)
+        if batch.cache is not self:
+            self._batch(batch)
         dtype = _DTYPES.get(t.dtype)
-        if dtype is None or t.device != self.device or t.shape != (batch.rows, heads, self.head_dim):
+        if dtype is None or t.shape != (batch.rows, heads, self.head_dim) or t.device != self.device:
             raise ValueError(f"{name} must be bfloat16 or float16 [{batch.rows}, {heads}, {self.head_dim}] on {self.device}, "
                              f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-        if t.stride(2) != 1 or t.stride(1) != self.head_dim:
+        if t.stride()[1:] != (self.head_dim, 1):
             raise ValueError(f"the heads of a row of {name} must lie one behind the other, strides are {t.stride()}")
         return dtype
 
