@@ -9,7 +9,8 @@
 // fp16 queries enter as bf16 hi + lo (exact to 2^-16 of the value, fp16 has 11 bits), so one set of products serves both types.
 //
 //   p = exp2(s c - m),  c = scale log2(e),  m the running maximum of s c as rounded, l the running sum:  one pass, fp32.
-// Keeping m as the rounded product makes the factors between pages and chunks, exp2(m - m'), consistent at any size of s.
+// m follows the maximum in jumps: it stays while the maximum is at most 2^8 above it (p <= 2^8 costs fp32 and bf16 nothing), so the
+// sums are rarely rescaled.  Keeping m as the rounded product makes the factors between pages and chunks, exp2(m - m'), consistent at any size of s.
 //
 // Sequences of at most KV4_FEW_COLUMNS columns (decode steps, drafted tokens) are cut into chunks of their cache, a workgroup of
 // four waves each; a second launch joins the chunks in order.  The chunk length follows from the sequence's own length, so a
@@ -19,8 +20,13 @@
 #include <type_traits>
 
 #define KV4_FEW_COLUMNS 64        // rows x group up to which a sequence is cut along its cache
-#ifndef KV4_KEEP_COLUMNS
-#define KV4_KEEP_COLUMNS 16
+#define KV4_KEEP_COLUMNS 16       // columns up to which the scores are kept for the weights
+#define KV4_SLACK 8.f             // the reference moves when a maximum passes it by 2^8
+#ifndef MW64
+#define MW64 2
+#define MW128 2
+#define NC64 2
+#define NC128 2
 #endif
 #define KV4_NONE -1e30f           // running maximum before the first visible token
 
@@ -172,8 +178,8 @@ __device__ __forceinline__ void kv4_split(float p0, float p1, unsigned& hi, unsi
 }
 
 // Probabilities of one page from its scores; the state's sums move to the new maximum.  ph + pl: slot y of step x is token
-// 16 g + 8 x + y.
-template <int HD, int NC>
+// 16 g + 8 x + y; without LO, ph alone.
+template <int HD, int NC, bool LO>
 __device__ __forceinline__ void kv4_softmax(const f32x4 (&s)[NC][4], Kv4State<HD, NC>& st, float c, bf16x8 (&ph)[NC][2], bf16x8 (&pl)[NC][2]) {
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
@@ -182,8 +188,17 @@ __device__ __forceinline__ void kv4_softmax(const f32x4 (&s)[NC][4], Kv4State<HD
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) top = fmaxf(top, s[n][i][j]);
-        const float m = fmaxf(st.m[n], kv4_group_max(top) * c), alpha = __builtin_amdgcn_exp2f(st.m[n] - m);
-        st.m[n] = m;
+        top = kv4_group_max(top) * c;
+        const float m = top > st.m[n] + KV4_SLACK ? top : st.m[n];
+        if (__any(m != st.m[n])) {                                // a column that keeps its reference multiplies by one
+            const float alpha = __builtin_amdgcn_exp2f(st.m[n] - m);
+            st.m[n] = m;
+            st.l[n] *= alpha;
+#pragma unroll
+            for (int h = 0; h < HD / 64; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) st.o[n][h][e] *= alpha;
+        }
         float sum = 0.f;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -199,13 +214,9 @@ __device__ __forceinline__ void kv4_softmax(const f32x4 (&s)[NC][4], Kv4State<HD
                 hi[y / 2] = h; lo[y / 2] = l;
             }
             ph[n][x] = __builtin_bit_cast(bf16x8, hi);
-            pl[n][x] = __builtin_bit_cast(bf16x8, lo);
+            if constexpr (LO) pl[n][x] = __builtin_bit_cast(bf16x8, lo);
         }
-        st.l[n] = fmaf(st.l[n], alpha, sum);
-#pragma unroll
-        for (int h = 0; h < HD / 64; ++h)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) st.o[n][h][e] *= alpha;
+        st.l[n] += sum;
     }
 }
 
@@ -336,7 +347,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_few_kernel(Kv4
             kv4_hide_scores<1>(sc, seen, lane);
             kv4_hide_values<HD>(pg, s.ctx - first, lane);
         }
-        kv4_softmax<HD, 1>(sc, st, a.c, ph, pl);
+        kv4_softmax<HD, 1, true>(sc, st, a.c, ph, pl);
         kv4_values<HD, 1>(pg, ph, pl, st);
         if constexpr (more()) kv4_fetch_v<HD>(pg, c, next, h, lane);
     };
@@ -440,20 +451,89 @@ __global__ __launch_bounds__(256) void kv4_attn_join_kernel(Kv4View c, Kv4Rows b
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Many columns (prompts): one wave per NC tiles of 16 columns and key head, the whole cache up to what its last row sees.
+// Many columns (prompts): a workgroup of four waves takes 4 x NC tiles of 16 columns of a key head and walks the cache up to what
+// its last row sees.  Each page is turned into bf16 once per workgroup: a wave converts a quarter (one of K's four token tiles, a
+// quarter of V) and leaves it in LDS in operand order, 1 KiB per fragment and a lane's 16 bytes where the same lane of every
+// wave will read them, while the products of the page before run from the other half of the buffer: one barrier a page.
+// For bf16 rows P is rounded to bf16: each probability is off by at most 2^-8 of itself, independently, which adds an error of the
+// size of the output's own rounding (at most 1.42 times it in all, measured over flat to sharp scores) and halves the second
+// product (4095 rows x 32 heads: 386 us against 476 with hi + lo parts).  For fp16 rows P is hi + lo.
 // ------------------------------------------------------------------------------------------------------------------
+template <int HD> struct Kv4Stage {
+    u32x4 k, v;                                                   // at hd 64 a wave's part of K is 8 bytes
+    u32x2 vs;
+    unsigned ks, bad;
+    // wave w: token tile w of K; V at hd 128 the half (h, x) = (w / 2, w % 2), at hd 64 x = w / 2 and two of its four dim tiles
+    __device__ __forceinline__ void load(const Kv4View& c, int page, int h, int w, int lane) {
+        const int g = lane >> 4, r = lane & 15;
+        bad = kv4_page_ok(page, c.n_pages) ? 0u : 0xffffffffu;
+        const uint8_t* slab = kv4_slab_of<HD>(c, page, h);
+        if constexpr (HD == 64) {
+            const u32x2 t = *reinterpret_cast<const u32x2*>(slab + (w >> 1) * 1024 + lane * 16 + (w & 1) * 8);
+            k = u32x4{t[0], t[1], 0u, 0u};
+            v = *reinterpret_cast<const u32x4*>(slab + 32 * HD + (w >> 1) * 1024 + lane * 16);
+            vs = *reinterpret_cast<const u32x2*>(slab + 66 * HD + (r >> 3) * KV4_PAGE + 16 * g + 8 * (w >> 1));
+        } else {
+            k = *reinterpret_cast<const u32x4*>(slab + w * 1024 + lane * 16);
+            v = *reinterpret_cast<const u32x4*>(slab + 32 * HD + w * 1024 + lane * 16);
+            vs = *reinterpret_cast<const u32x2*>(slab + 66 * HD + (2 * (w >> 1) + (r >> 3)) * KV4_PAGE + 16 * g + 8 * (w & 1));
+        }
+        ks = slab[64 * HD + g * (HD / 4) / KV4_BLOCK * KV4_PAGE + 4 * r + w];
+    }
+    // tail: tokens of the page that exist
+    __device__ __forceinline__ void store(uint8_t* buf, int tail, int w, int lane) const {
+        const int x = HD == 64 ? w >> 1 : w & 1;
+        const float sc = kv4_scale((ks | bad) & 255u);
+#pragma unroll
+        for (int y = 0; y < HD / 32; ++y) {
+            const u32x4 a = {kv4_pair<0>(k[y], sc), kv4_pair<1>(k[y], sc), kv4_pair<2>(k[y], sc), kv4_pair<3>(k[y], sc)};
+            *reinterpret_cast<u32x4*>(buf + (w * (HD / 32) + y) * 1024 + lane * 16) = a;
+        }
+        u32x2 s = {vs[0] & ~bad, vs[1] & ~bad};
+        if (tail < KV4_PAGE) {
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+                const int mine = tail - 16 * (lane >> 4) - 8 * x - 4 * z;
+                s[z] &= mine >= 4 ? 0xffffffffu : mine <= 0 ? 0u : (1u << (8 * mine)) - 1u;
+            }
+        }
+        u32x4 a[4];
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+            const float s0 = kv4_scale(kv4_byte(s[z / 2], z % 2 * 2)), s1 = kv4_scale(kv4_byte(s[z / 2], z % 2 * 2 + 1));
+            const unsigned codes = HD == 64 && (w & 1) ? v[z] >> 8 : v[z];      // hd 64: dims 2, 3 move to where 0, 1 are
+            const unsigned t0 = kv4_pair<0>(codes, s0), t1 = kv4_pair<2>(codes, s1);
+            a[0][z] = __builtin_amdgcn_perm(t1, t0, 0x05040100u);
+            a[1][z] = __builtin_amdgcn_perm(t1, t0, 0x07060302u);
+            if constexpr (HD == 128) {
+                const unsigned u0 = kv4_pair<1>(codes, s0), u1 = kv4_pair<3>(codes, s1);
+                a[2][z] = __builtin_amdgcn_perm(u1, u0, 0x05040100u);
+                a[3][z] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
+            }
+        }
+        // fragment (h, x, e) of V
+        const int f = HD == 64 ? x * 4 + 2 * (w & 1) : w * 4;
+#pragma unroll
+        for (int e = 0; e < HD / 32; ++e) *reinterpret_cast<u32x4*>(buf + 128 * HD + (f + e) * 1024 + lane * 16) = a[e];
+    }
+};
+
 template <int HD, bool F16, int NC>
-__global__ __launch_bounds__(256) void kv4_attn_many_kernel(Kv4View c, Kv4Rows b, Kv4Attn a) {
-    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int h = blockIdx.y, H = c.Hkv * a.group;
+__global__ __launch_bounds__(256, HD == 64 ? MW64 : MW128) void kv4_attn_many_kernel(Kv4View c, Kv4Rows b, Kv4Attn a) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2][256 * HD];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
+    const int h = blockIdx.x, H = c.Hkv * a.group;
     const Kv4Seq s = kv4_seq_of(b, c, blockIdx.z);
     const int rows = s.n < b.max_rows ? s.n : b.max_rows, cols = rows * a.group;
     if (s.state == 1 || cols <= KV4_FEW_COLUMNS) return;
-    const int c0 = (blockIdx.x * 4 + w) * (16 * NC);
-    if (c0 >= cols) return;                                       // no barrier below: waves are on their own
-    const int c1 = cols < c0 + 16 * NC ? cols : c0 + 16 * NC;
-    if (s.state == 2) { kv4_fill_columns<HD>(a, s, h, c0, c1, lane, 64); return; }
-
+    // the last tiles see most: they start first
+    const int block = (cols + 64 * NC - 1) / (64 * NC) - 1 - (int)blockIdx.y;
+    if (block < 0) return;
+    const int c0 = (block * 4 + w) * (16 * NC), c1 = cols < c0 + 16 * NC ? cols : c0 + 16 * NC;
+    if (s.state == 2) {
+        if (c0 < cols) kv4_fill_columns<HD>(a, s, h, c0, c1, lane, 64);
+        return;
+    }
     Kv4Query<HD, F16> q[NC];
     int sees[NC], seen[NC];
 #pragma unroll
@@ -462,32 +542,72 @@ __global__ __launch_bounds__(256) void kv4_attn_many_kernel(Kv4View c, Kv4Rows b
         q[n].load(col < c1 ? a.q + (int64_t)(s.start + j) * a.q_stride + (h * a.group + col % a.group) * HD : nullptr, lane);
         sees[n] = col < c1 ? s.ctx - s.n + j + 1 : 0;
     }
-    const int least = s.ctx - s.n + c0 / a.group + 1, most = s.ctx - s.n + (c1 - 1) / a.group + 1;   // first and last row of the wave
+    // what the wave's first and last row see; a wave without columns sees nothing and only converts
+    const int base = s.ctx - s.n + 1, least = base + c0 / a.group, most = c0 < cols ? base + (c1 - 1) / a.group : 0;
+    const int end = block * (64 * NC) + 64 * NC, all = base + ((cols < end ? cols : end) - 1) / a.group;      // the workgroup's last row
     Kv4State<HD, NC> st;
     st.clear();
     const int32_t* bt = c.table + (int64_t)s.stream * c.max_pages;
-    for (int first = 0; first < most; first += KV4_PAGE) {
-        const int id = __builtin_amdgcn_readfirstlane(bt[first / KV4_PAGE]);
-        Kv4Page<HD> pg;
-        kv4_fetch_k<HD>(pg, c, id, h, lane);
-        kv4_fetch_v<HD>(pg, c, id, h, lane);
-#pragma unroll
-        for (int n = 0; n < NC; ++n) seen[n] = sees[n] - first;
-        f32x4 sc[NC][4];
-        bf16x8 ph[NC][2], pl[NC][2];
-        kv4_scores<HD, F16, NC>(pg, q, sc);
-        if (least < first + KV4_PAGE) {
-            kv4_hide_scores<NC>(sc, seen, lane);
-            kv4_hide_values<HD>(pg, s.ctx - first, lane);
+    const int pages = all > 0 ? (all + KV4_PAGE - 1) / KV4_PAGE : 0;
+    Kv4Stage<HD> stage;
+    if (pages > 0) {
+        stage.load(c, __builtin_amdgcn_readfirstlane(bt[0]), h, w, lane);
+        stage.store(lds[0], s.ctx, w, lane);
+    }
+    int id = pages > 1 ? __builtin_amdgcn_readfirstlane(bt[1]) : 0;
+    __syncthreads();
+    for (int p = 0; p < pages; ++p) {
+        const int first = p * KV4_PAGE;
+        const bool more = p + 1 < pages;
+        if (more) {
+            stage.load(c, id, h, w, lane);
+            id = __builtin_amdgcn_readfirstlane(bt[p + 2 < pages ? p + 2 : p]);
         }
-        kv4_softmax<HD, NC>(sc, st, a.c, ph, pl);
-        kv4_values<HD, NC>(pg, ph, pl, st);
+        if (first < most) {
+            const uint8_t* buf = lds[p & 1];
+            f32x4 sc[NC][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int n = 0; n < NC; ++n) sc[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int x = 0; x < HD / 32; ++x) {
+                    const bf16x8 af = *reinterpret_cast<const bf16x8*>(buf + (i * (HD / 32) + x) * 1024 + lane * 16);
+#pragma unroll
+                    for (int n = 0; n < NC; ++n) {
+                        sc[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, q[n].q[x], sc[n][i], 0, 0, 0);
+                        if constexpr (F16) sc[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, q[n].q[HD / 32 + x], sc[n][i], 0, 0, 0);
+                    }
+                }
+            }
+            if (least < first + KV4_PAGE) {
+#pragma unroll
+                for (int n = 0; n < NC; ++n) seen[n] = sees[n] - first;
+                kv4_hide_scores<NC>(sc, seen, lane);
+            }
+            bf16x8 ph[NC][2], pl[NC][2];
+            kv4_softmax<HD, NC, F16>(sc, st, a.c, ph, pl);
+#pragma unroll
+            for (int hh = 0; hh < HD / 64; ++hh)
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const bf16x8 af = *reinterpret_cast<const bf16x8*>(buf + 128 * HD + ((hh * 2 + x) * 4 + e) * 1024 + lane * 16);
+#pragma unroll
+                        for (int n = 0; n < NC; ++n) {
+                            st.o[n][hh][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, ph[n][x], st.o[n][hh][e], 0, 0, 0);
+                            if constexpr (F16) st.o[n][hh][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, pl[n][x], st.o[n][hh][e], 0, 0, 0);
+                        }
+                    }
+        }
+        if (more) stage.store(lds[(p + 1) & 1], s.ctx - first - KV4_PAGE, w, lane);
+        __syncthreads();
     }
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-        const int col = c0 + 16 * n + (lane & 15), j = col / a.group, head = h * a.group + col % a.group, g = lane >> 4;
-        float l = st.l[n];
-        l = kv4_group_sum(l);
+        const int col = c0 + 16 * n + (lane & 15), j = col / a.group, head = h * a.group + col % a.group;
+        const float l = kv4_group_sum(st.l[n]);
         if (col >= c1) continue;
         const float inv = l == 0.f ? 0.f : 1.0f / l;
         uint16_t* op = a.out + (int64_t)(s.start + j) * a.out_stride + head * HD + 16 * g;
@@ -650,13 +770,13 @@ extern "C" int64_t t3_op_attn_kv4_work_bytes(const t3_kv4_cache* cache, const t3
 
 template <int HD, bool F16>
 static int launch_attn(const Kv4View& c, const Kv4Rows& b, const Kv4Attn& a, float* weights, int64_t weights_stride, hipStream_t st) {
-    constexpr int NC = 4;
+    constexpr int NC = HD == 64 ? NC64 : NC128;
     const int64_t cols = (int64_t)b.max_rows * a.group;
     T3_LAUNCH((kv4_attn_few_kernel<HD, F16>), dim3(a.tiles * c.Hkv, b.n_seqs, a.chunks), dim3(256), 0, st, c, b, a);
     if (a.chunks > 1)
         T3_LAUNCH((kv4_attn_join_kernel<HD, F16>), dim3((cols < KV4_FEW_COLUMNS ? (int)cols : KV4_FEW_COLUMNS) * c.Hkv, b.n_seqs), dim3(256), 0, st, c, b, a);
     if (cols > KV4_FEW_COLUMNS)
-        T3_LAUNCH((kv4_attn_many_kernel<HD, F16, NC>), dim3((unsigned)((cols + 64 * NC - 1) / (64 * NC)), c.Hkv, b.n_seqs), dim3(256), 0, st, c, b, a);
+        T3_LAUNCH((kv4_attn_many_kernel<HD, F16, NC>), dim3(c.Hkv, (unsigned)((cols + 64 * NC - 1) / (64 * NC)), b.n_seqs), dim3(256), 0, st, c, b, a);
     if (weights) {
         const int64_t cap = (int64_t)c.max_pages * KV4_PAGE, most = b.max_ctx < cap ? b.max_ctx : cap;
         if (cols <= KV4_KEEP_COLUMNS)
@@ -677,7 +797,7 @@ extern "C" int t3_op_attn_kv4(const t3_kv4_cache* cache, const t3_kv4_batch* bat
     T3_REQUIRE(q_dev && out_dev, "attn_kv4: null argument");
     T3_REQUIRE(dtype == 0 || dtype == 1, "attn_kv4: dtype must be 0 (bf16) or 1 (fp16)");
     T3_REQUIRE(scale > 0.f && scale < 1e8f, "attn_kv4: scale must be positive");
-    T3_REQUIRE((int64_t)batch->max_rows * (H / cache->Hkv) <= (1 << 30), "attn_kv4: more than 2^30 rows x query heads of a key head");
+    T3_REQUIRE((int64_t)batch->max_rows * (H / cache->Hkv) <= (1 << 22), "attn_kv4: more than 2^22 rows x query heads of a key head");
     const int64_t width = (int64_t)H * cache->hd;
     T3_REQUIRE(q_stride >= width && out_stride >= width && q_stride % 8 == 0 && out_stride % 8 == 0 &&
                reinterpret_cast<uintptr_t>(q_dev) % 16 == 0 && reinterpret_cast<uintptr_t>(out_dev) % 16 == 0,

@@ -110,11 +110,13 @@ def attend(q, k, v, ctx, scale):
     return out, weights, size, bound
 
 
-def out_bound(ref, size, bound, ctx, dtype):
-    """|out - ref| may be: half a step of the output; each probability off by twice a score's error (its own and the sum's), by the
-    2^-17 that its two bf16 parts leave, and by the fp32 sums over ctx entries."""
+def out_bound(ref, size, bound, ctx, dtype, columns=1):
+    """|out - ref| may be: half a step of the output; each probability off by twice a score's error (its own and the sum's), by what
+    its rounding leaves (half a step of bf16 is 2^-8: one part, as bf16 sequences of more than 64 columns have it; 2^-16 in two), and
+    by the fp32 sums over ctx entries."""
     eps = torch.finfo(dtype).eps / 2
-    inner = size * (2 * bound * 2.0 ** -24 + 2.0 ** -17 + (ctx / 16 + 64) * 2.0 ** -24)
+    rounding = 2.0 ** -8 if dtype == torch.bfloat16 and columns > 64 else 2.0 ** -16
+    inner = size * (2 * bound * 2.0 ** -24 + rounding + (ctx / 16 + 64) * 2.0 ** -24)
     return eps * (ref.abs() + inner) + inner + torch.finfo(dtype).smallest_normal * 2 ** -7
 
 

@@ -48,7 +48,7 @@ def check_attend(m, cache, rows, ctx, group, dtype, with_weights, streams=None, 
         k, v = m.get(m.pool, streams[i], torch.arange(ctx[i]), layer)
         ref, p, size, bound = _kv4.attend(q[s[i]:s[i + 1]].double(), k, v, ctx[i], scale)
         err = (out[s[i]:s[i + 1]].cpu().double() - ref).abs()
-        tol = _kv4.out_bound(ref, size, bound, ctx[i], DT[dtype])
+        tol = _kv4.out_bound(ref, size, bound, ctx[i], DT[dtype], rows[i] * group)
         assert (err <= tol).all(), f"sequence {i} ({rows[i]} rows, {ctx[i]} entries): {(err / tol).max():.2f} of the bound"
         added[streams[i], :, :ctx[i]] += p
         slack[streams[i], :, :ctx[i]] += _kv4.weights_bound(p, torch.zeros_like(p), bound, ctx[i], rows[i] * group)
@@ -215,7 +215,7 @@ def test_sharp_and_flat_scores():
         out = cache.attend(q.to(DEV), cache.batch(i32([0, rows]), i32([0]), i32([t]), rows=rows)).cpu()
         assert torch.isnan(out[-3:]).all()
         ref, _, size, bound = _kv4.attend(q[:-3].double(), *(x[:t - 3] for x in m.get(m.pool, 0, torch.arange(t))), t - 3, 0.125)
-        assert ((out[:-3].double() - ref).abs() <= _kv4.out_bound(ref, size, bound, t, torch.bfloat16)).all()
+        assert ((out[:-3].double() - ref).abs() <= _kv4.out_bound(ref, size, bound, t, torch.bfloat16, rows)).all()
 
 
 def test_what_lies_behind_the_last_entry_does_not_matter():
@@ -275,7 +275,7 @@ def test_numbers_that_do_not_fit_give_nan_and_store_nothing():
         assert torch.isnan(out[[1, 2]]).all()
         for i in (0, 5, 6):
             ref, _, size, bound = _kv4.attend(q.cpu().double()[i * rows:(i + 1) * rows], *m.get(m.pool, streams[i], torch.arange(ctx[i])), ctx[i], 0.125)
-            assert ((out[i].double() - ref).abs() <= _kv4.out_bound(ref, size, bound, 200, torch.bfloat16)).all()
+            assert ((out[i].double() - ref).abs() <= _kv4.out_bound(ref, size, bound, 200, torch.bfloat16, rows)).all()
         assert not torch.isnan(w[[0, 1, 2, 5]]).any() and (w[2] == 0).all()
         k, v = cache.read(batch)
         k, v = k.view(n, rows, 2, 64), v.view(n, rows, 2, 64)
@@ -448,7 +448,7 @@ def test_a_stream_from_prompt_to_eviction_and_on(hd, kv, group):
             m.put(m.pool, st, torch.arange(ctx[i] - rows[i], ctx[i]), qkv[s[i]:s[i + 1], kv * group:-kv], qkv[s[i]:s[i + 1], -kv:], layer)
             kk, vv = m.get(m.pool, st, torch.arange(ctx[i]), layer)
             ref, p, size, bound = _kv4.attend(qkv[s[i]:s[i + 1], :kv * group].double(), kk, vv, ctx[i], hd ** -0.5)
-            assert ((out[s[i]:s[i + 1]] - ref).abs() <= _kv4.out_bound(ref, size, bound, ctx[i], torch.bfloat16)).all()
+            assert ((out[s[i]:s[i + 1]] - ref).abs() <= _kv4.out_bound(ref, size, bound, ctx[i], torch.bfloat16, rows[i] * group)).all()
             model_w[st, :, :ctx[i]] += p
             slack = max(slack, _kv4.weights_bound(p, p, bound, ctx[i], rows[i] * group).max().item())
 
