@@ -22,12 +22,6 @@
 #define KV4_FEW_COLUMNS 64        // rows x group up to which a sequence is cut along its cache
 #define KV4_KEEP_COLUMNS 16       // columns up to which the scores are kept for the weights
 #define KV4_SLACK 8.f             // the reference moves when a maximum passes it by 2^8
-#ifndef MW64
-#define MW64 2
-#define MW128 2
-#define NC64 2
-#define NC128 2
-#endif
 #define KV4_NONE -1e30f           // running maximum before the first visible token
 
 // A chunk is 16 pages: the four waves of its workgroup take four each.
@@ -177,10 +171,8 @@ __device__ __forceinline__ void kv4_split(float p0, float p1, unsigned& hi, unsi
     lo = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{p0 - bf_lo(hi), p1 - bf_hi(hi)}), bf16x2));
 }
 
-// Probabilities of one page from its scores; the state's sums move to the new maximum.  ph + pl: slot y of step x is token
-// 16 g + 8 x + y; without LO, ph alone.
-template <int HD, int NC, bool LO>
-__device__ __forceinline__ void kv4_softmax(const f32x4 (&s)[NC][4], Kv4State<HD, NC>& st, float c, bf16x8 (&ph)[NC][2], bf16x8 (&pl)[NC][2]) {
+// A page's softmax in two parts.  First the reference: it moves, and the sums with it, where a maximum has left it behind.
+template <int HD, int NC> __device__ __forceinline__ void kv4_reference(const f32x4 (&s)[NC][4], Kv4State<HD, NC>& st, float c) {
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
         float top = s[n][0][0];
@@ -199,6 +191,13 @@ __device__ __forceinline__ void kv4_softmax(const f32x4 (&s)[NC][4], Kv4State<HD
 #pragma unroll
                 for (int e = 0; e < 4; ++e) st.o[n][h][e] *= alpha;
         }
+    }
+}
+// Then the probabilities.  ph + pl: slot y of step x is token 16 g + 8 x + y; without LO, ph alone.
+template <int HD, int NC, bool LO>
+__device__ __forceinline__ void kv4_probabilities(const f32x4 (&s)[NC][4], Kv4State<HD, NC>& st, float c, bf16x8 (&ph)[NC][2], bf16x8 (&pl)[NC][2]) {
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
         float sum = 0.f;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -206,8 +205,8 @@ __device__ __forceinline__ void kv4_softmax(const f32x4 (&s)[NC][4], Kv4State<HD
 #pragma unroll
             for (int y = 0; y < 8; y += 2) {
                 const int e = 8 * x + y;                          // tokens 16 g + e, + e + 1
-                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[n][e & 3][e >> 2], c, -m));
-                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[n][(e & 3) + 1][e >> 2], c, -m));
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[n][e & 3][e >> 2], c, -st.m[n]));
+                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[n][(e & 3) + 1][e >> 2], c, -st.m[n]));
                 sum += p0 + p1;
                 unsigned h, l;
                 kv4_split(p0, p1, h, l);
@@ -347,7 +346,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_few_kernel(Kv4
             kv4_hide_scores<1>(sc, seen, lane);
             kv4_hide_values<HD>(pg, s.ctx - first, lane);
         }
-        kv4_softmax<HD, 1, true>(sc, st, a.c, ph, pl);
+        kv4_reference<HD, 1>(sc, st, a.c);
+        kv4_probabilities<HD, 1, true>(sc, st, a.c, ph, pl);
         kv4_values<HD, 1>(pg, ph, pl, st);
         if constexpr (more()) kv4_fetch_v<HD>(pg, c, next, h, lane);
     };
@@ -462,40 +462,44 @@ __global__ __launch_bounds__(256) void kv4_attn_join_kernel(Kv4View c, Kv4Rows b
 template <int HD> struct Kv4Stage {
     u32x4 k, v;                                                   // at hd 64 a wave's part of K is 8 bytes
     u32x2 vs;
-    unsigned ks, bad;
+    unsigned ks, bad_k, good_v;
     // wave w: token tile w of K; V at hd 128 the half (h, x) = (w / 2, w % 2), at hd 64 x = w / 2 and two of its four dim tiles
-    __device__ __forceinline__ void load(const Kv4View& c, int page, int h, int w, int lane) {
+    __device__ __forceinline__ void load_k(const Kv4View& c, int page, int h, int w, int lane) {
         const int g = lane >> 4, r = lane & 15;
-        bad = kv4_page_ok(page, c.n_pages) ? 0u : 0xffffffffu;
+        bad_k = kv4_page_ok(page, c.n_pages) ? 0u : 0xffffffffu;
         const uint8_t* slab = kv4_slab_of<HD>(c, page, h);
         if constexpr (HD == 64) {
             const u32x2 t = *reinterpret_cast<const u32x2*>(slab + (w >> 1) * 1024 + lane * 16 + (w & 1) * 8);
             k = u32x4{t[0], t[1], 0u, 0u};
-            v = *reinterpret_cast<const u32x4*>(slab + 32 * HD + (w >> 1) * 1024 + lane * 16);
-            vs = *reinterpret_cast<const u32x2*>(slab + 66 * HD + (r >> 3) * KV4_PAGE + 16 * g + 8 * (w >> 1));
         } else {
             k = *reinterpret_cast<const u32x4*>(slab + w * 1024 + lane * 16);
-            v = *reinterpret_cast<const u32x4*>(slab + 32 * HD + w * 1024 + lane * 16);
-            vs = *reinterpret_cast<const u32x2*>(slab + 66 * HD + (2 * (w >> 1) + (r >> 3)) * KV4_PAGE + 16 * g + 8 * (w & 1));
         }
         ks = slab[64 * HD + g * (HD / 4) / KV4_BLOCK * KV4_PAGE + 4 * r + w];
     }
-    // tail: tokens of the page that exist
-    __device__ __forceinline__ void store(uint8_t* buf, int tail, int w, int lane) const {
-        const int x = HD == 64 ? w >> 1 : w & 1;
-        const float sc = kv4_scale((ks | bad) & 255u);
+    __device__ __forceinline__ void load_v(const Kv4View& c, int page, int h, int w, int lane) {
+        const int g = lane >> 4, r = lane & 15;
+        good_v = kv4_page_ok(page, c.n_pages) ? 0xffffffffu : 0u;
+        const uint8_t* slab = kv4_slab_of<HD>(c, page, h);
+        const int part = HD == 64 ? w >> 1 : w;
+        v = *reinterpret_cast<const u32x4*>(slab + 32 * HD + part * 1024 + lane * 16);
+        vs = *reinterpret_cast<const u32x2*>(slab + 66 * HD + (HD == 64 ? r >> 3 : 2 * (w >> 1) + (r >> 3)) * KV4_PAGE + 16 * g + 8 * (HD == 64 ? part : w & 1));
+    }
+    __device__ __forceinline__ void store_k(uint8_t* buf, int w, int lane) const {
+        const float sc = kv4_scale((ks | bad_k) & 255u);
 #pragma unroll
         for (int y = 0; y < HD / 32; ++y) {
             const u32x4 a = {kv4_pair<0>(k[y], sc), kv4_pair<1>(k[y], sc), kv4_pair<2>(k[y], sc), kv4_pair<3>(k[y], sc)};
             *reinterpret_cast<u32x4*>(buf + (w * (HD / 32) + y) * 1024 + lane * 16) = a;
         }
-        u32x2 s = {vs[0] & ~bad, vs[1] & ~bad};
-        if (tail < KV4_PAGE) {
+    }
+    // tail: tokens of the page that exist; the scales of the others go to 0 (their bytes may be anything, and 0 * finite is 0)
+    __device__ __forceinline__ void store_v(uint8_t* buf, int tail, int w, int lane) const {
+        const int x = HD == 64 ? w >> 1 : w & 1;
+        u32x2 s;
 #pragma unroll
-            for (int z = 0; z < 2; ++z) {
-                const int mine = tail - 16 * (lane >> 4) - 8 * x - 4 * z;
-                s[z] &= mine >= 4 ? 0xffffffffu : mine <= 0 ? 0u : (1u << (8 * mine)) - 1u;
-            }
+        for (int z = 0; z < 2; ++z) {
+            const int mine = tail - 16 * (lane >> 4) - 8 * x - 4 * z;
+            s[z] = vs[z] & good_v & (mine >= 4 ? 0xffffffffu : mine <= 0 ? 0u : (1u << (8 * mine)) - 1u);
         }
         u32x4 a[4];
 #pragma unroll
@@ -514,20 +518,70 @@ template <int HD> struct Kv4Stage {
         // fragment (h, x, e) of V
         const int f = HD == 64 ? x * 4 + 2 * (w & 1) : w * 4;
 #pragma unroll
-        for (int e = 0; e < HD / 32; ++e) *reinterpret_cast<u32x4*>(buf + 128 * HD + (f + e) * 1024 + lane * 16) = a[e];
+        for (int e = 0; e < HD / 32; ++e) *reinterpret_cast<u32x4*>(buf + (f + e) * 1024 + lane * 16) = a[e];
     }
 };
 
+// The order wanted of a product's block: four fragments read ahead, and one more behind the products of each, so that no product
+// waits for LDS.  Nothing else is put between them: on this chip vector instructions do not run beside matrix ones, of the same or
+// of another wave (17.6 clocks a product, 27.5 with four fmas behind each), and every change from one to the other costs ~5 clocks.
+template <int FRAGMENTS, int PRODUCTS> __device__ __forceinline__ void kv4_interleave() {
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);           // LDS reads
+#pragma unroll
+    for (int f = 0; f < FRAGMENTS; ++f) {
+        __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS, 0);
+        if (f + 4 < FRAGMENTS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+}
+
+// S^T of a page from its fragments in LDS
 template <int HD, bool F16, int NC>
-__global__ __launch_bounds__(256, HD == 64 ? MW64 : MW128) void kv4_attn_many_kernel(Kv4View c, Kv4Rows b, Kv4Attn a) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[2][256 * HD];
+__device__ __forceinline__ void kv4_lds_scores(const uint8_t* kbuf, const Kv4Query<HD, F16> (&q)[NC], f32x4 (&s)[NC][4], int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int n = 0; n < NC; ++n) s[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < HD / 32; ++x) {                           // tiles inside steps: products of one sum lie 4 x NC apart
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bf16x8 af = *reinterpret_cast<const bf16x8*>(kbuf + (i * (HD / 32) + x) * 1024 + lane * 16);
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                s[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, q[n].q[x], s[n][i], 0, 0, 0);
+                if constexpr (F16) s[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, q[n].q[HD / 32 + x], s[n][i], 0, 0, 0);
+            }
+        }
+    }
+}
+template <int HD, bool LO, int NC>
+__device__ __forceinline__ void kv4_lds_values(const uint8_t* vbuf, const bf16x8 (&ph)[NC][2], const bf16x8 (&pl)[NC][2], Kv4State<HD, NC>& st, int lane) {
+#pragma unroll
+    for (int hh = 0; hh < HD / 64; ++hh)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bf16x8 af = *reinterpret_cast<const bf16x8*>(vbuf + ((hh * 2 + x) * 4 + e) * 1024 + lane * 16);
+#pragma unroll
+                for (int n = 0; n < NC; ++n) {
+                    st.o[n][hh][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, ph[n][x], st.o[n][hh][e], 0, 0, 0);
+                    if constexpr (LO) st.o[n][hh][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, pl[n][x], st.o[n][hh][e], 0, 0, 0);
+                }
+            }
+}
+
+template <int HD, bool F16, int NC>
+__global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_many_kernel(Kv4View c, Kv4Rows b, Kv4Attn a) {
+    __shared__ __attribute__((aligned(16))) uint8_t kbuf[2][128 * HD], vbuf[2][128 * HD];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
     const int h = blockIdx.x, H = c.Hkv * a.group;
     const Kv4Seq s = kv4_seq_of(b, c, blockIdx.z);
     const int rows = s.n < b.max_rows ? s.n : b.max_rows, cols = rows * a.group;
     if (s.state == 1 || cols <= KV4_FEW_COLUMNS) return;
     // the last tiles see most: they start first
-    const int block = (cols + 64 * NC - 1) / (64 * NC) - 1 - (int)blockIdx.y;
+    constexpr int COLS = 64 * NC;
+    const int block = (cols + COLS - 1) / COLS - 1 - (int)blockIdx.y;
     if (block < 0) return;
     const int c0 = (block * 4 + w) * (16 * NC), c1 = cols < c0 + 16 * NC ? cols : c0 + 16 * NC;
     if (s.state == 2) {
@@ -544,64 +598,54 @@ __global__ __launch_bounds__(256, HD == 64 ? MW64 : MW128) void kv4_attn_many_ke
     }
     // what the wave's first and last row see; a wave without columns sees nothing and only converts
     const int base = s.ctx - s.n + 1, least = base + c0 / a.group, most = c0 < cols ? base + (c1 - 1) / a.group : 0;
-    const int end = block * (64 * NC) + 64 * NC, all = base + ((cols < end ? cols : end) - 1) / a.group;      // the workgroup's last row
+    const int end = block * COLS + COLS, all = base + ((cols < end ? cols : end) - 1) / a.group;      // the workgroup's last row
     Kv4State<HD, NC> st;
     st.clear();
     const int32_t* bt = c.table + (int64_t)s.stream * c.max_pages;
     const int pages = all > 0 ? (all + KV4_PAGE - 1) / KV4_PAGE : 0;
+    const int mine = most > 0 ? (most + KV4_PAGE - 1) / KV4_PAGE : 0;        // pages that the wave looks at
+    const auto page_id = [&](int p) { return __builtin_amdgcn_readfirstlane(bt[p < pages ? p : pages - 1]); };
     Kv4Stage<HD> stage;
     if (pages > 0) {
-        stage.load(c, __builtin_amdgcn_readfirstlane(bt[0]), h, w, lane);
-        stage.store(lds[0], s.ctx, w, lane);
+        stage.load_k(c, page_id(0), h, w, lane);
+        stage.load_v(c, page_id(0), h, w, lane);
+        stage.store_k(kbuf[0], w, lane);
+        stage.store_v(vbuf[0], s.ctx, w, lane);
     }
-    int id = pages > 1 ? __builtin_amdgcn_readfirstlane(bt[1]) : 0;
+    int id = pages > 0 ? page_id(1) : 0;
     __syncthreads();
-    for (int p = 0; p < pages; ++p) {
+    int p = 0;
+    for (; p < mine; ++p) {
         const int first = p * KV4_PAGE;
-        const bool more = p + 1 < pages;
-        if (more) {
-            stage.load(c, id, h, w, lane);
-            id = __builtin_amdgcn_readfirstlane(bt[p + 2 < pages ? p + 2 : p]);
+        stage.load_k(c, id, h, w, lane);
+        stage.load_v(c, id, h, w, lane);
+        id = page_id(p + 2);
+        f32x4 sc[NC][4];
+        bf16x8 ph[NC][2], pl[NC][2];
+        kv4_lds_scores<HD, F16, NC>(kbuf[p & 1], q, sc, lane);
+        kv4_interleave<HD / 8, NC * (F16 ? 2 : 1)>();
+        if (least < first + KV4_PAGE) {
+#pragma unroll
+            for (int n = 0; n < NC; ++n) seen[n] = sees[n] - first;
+            kv4_hide_scores<NC>(sc, seen, lane);
         }
-        if (first < most) {
-            const uint8_t* buf = lds[p & 1];
-            f32x4 sc[NC][4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                for (int n = 0; n < NC; ++n) sc[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int x = 0; x < HD / 32; ++x) {
-                    const bf16x8 af = *reinterpret_cast<const bf16x8*>(buf + (i * (HD / 32) + x) * 1024 + lane * 16);
-#pragma unroll
-                    for (int n = 0; n < NC; ++n) {
-                        sc[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, q[n].q[x], sc[n][i], 0, 0, 0);
-                        if constexpr (F16) sc[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, q[n].q[HD / 32 + x], sc[n][i], 0, 0, 0);
-                    }
-                }
-            }
-            if (least < first + KV4_PAGE) {
-#pragma unroll
-                for (int n = 0; n < NC; ++n) seen[n] = sees[n] - first;
-                kv4_hide_scores<NC>(sc, seen, lane);
-            }
-            bf16x8 ph[NC][2], pl[NC][2];
-            kv4_softmax<HD, NC, F16>(sc, st, a.c, ph, pl);
-#pragma unroll
-            for (int hh = 0; hh < HD / 64; ++hh)
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const bf16x8 af = *reinterpret_cast<const bf16x8*>(buf + 128 * HD + ((hh * 2 + x) * 4 + e) * 1024 + lane * 16);
-#pragma unroll
-                        for (int n = 0; n < NC; ++n) {
-                            st.o[n][hh][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, ph[n][x], st.o[n][hh][e], 0, 0, 0);
-                            if constexpr (F16) st.o[n][hh][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, pl[n][x], st.o[n][hh][e], 0, 0, 0);
-                        }
-                    }
-        }
-        if (more) stage.store(lds[(p + 1) & 1], s.ctx - first - KV4_PAGE, w, lane);
+        kv4_reference<HD, NC>(sc, st, a.c);
+        kv4_probabilities<HD, NC, F16>(sc, st, a.c, ph, pl);
+        __builtin_amdgcn_sched_barrier(0);
+        kv4_lds_values<HD, F16, NC>(vbuf[p & 1], ph, pl, st, lane);
+        kv4_interleave<HD / 8, NC * (F16 ? 2 : 1)>();
+        __builtin_amdgcn_sched_barrier(0);
+        stage.store_k(kbuf[(p + 1) & 1], w, lane);
+        stage.store_v(vbuf[(p + 1) & 1], s.ctx - first - KV4_PAGE, w, lane);
+        __syncthreads();
+    }
+    // pages that only later waves of the workgroup see
+    for (; p < pages; ++p) {
+        stage.load_k(c, id, h, w, lane);
+        stage.load_v(c, id, h, w, lane);
+        id = page_id(p + 2);
+        stage.store_k(kbuf[(p + 1) & 1], w, lane);
+        stage.store_v(vbuf[(p + 1) & 1], s.ctx - (p + 1) * KV4_PAGE, w, lane);
         __syncthreads();
     }
 #pragma unroll
@@ -770,7 +814,9 @@ extern "C" int64_t t3_op_attn_kv4_work_bytes(const t3_kv4_cache* cache, const t3
 
 template <int HD, bool F16>
 static int launch_attn(const Kv4View& c, const Kv4Rows& b, const Kv4Attn& a, float* weights, int64_t weights_stride, hipStream_t st) {
-    constexpr int NC = HD == 64 ? NC64 : NC128;
+    // column tiles of a wave: at hd 128 two share each fragment's way through LDS (372 us; one, with eight waves a workgroup, 395); at
+    // hd 64 one leaves room for four waves a SIMD instead of two (4 x 2000 rows 70.6 us; two 78, four 98)
+    constexpr int NC = HD == 64 ? 1 : 2;
     const int64_t cols = (int64_t)b.max_rows * a.group;
     T3_LAUNCH((kv4_attn_few_kernel<HD, F16>), dim3(a.tiles * c.Hkv, b.n_seqs, a.chunks), dim3(256), 0, st, c, b, a);
     if (a.chunks > 1)
