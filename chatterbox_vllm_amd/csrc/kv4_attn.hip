@@ -29,18 +29,31 @@
 KV4_FN int kv4_chunks(int ctx) { return (int)(((int64_t)ctx + KV4_CHUNK_PAGES * KV4_PAGE - 1) / (KV4_CHUNK_PAGES * KV4_PAGE)); }
 
 struct Kv4Attn {
-    const uint16_t* q; int64_t q_stride;
-    uint16_t* out; int64_t out_stride;
+    const uint16_t* q; uint16_t* out;
+    unsigned q_stride, out_stride, inv;        // row strides in elements; ceil(2^32 / group), 0 for a group of one
     int group, tiles, chunks;     // query heads per key head; column tiles and chunks the state buffer holds per (sequence, key head)
     float c;                      // scale * log2(e)
     float* states;                // [sequence][key head][tile][chunk] x kv4_state_floats
-    f32x2* norm;                  // [rows][H]: m and 1 / l of each column, or null
+    // for the weights, or null.  Columns of a (sequence, key head) start at kv4_column(), tiles of 16 of them being whole:
+    f32x2* norm;                  // m and 1 / l of each column
+    uint8_t* frags;               // the queries of each tile as the product takes them: [hd / 32][64 lanes][16 bytes]
+    int slots;                    // tiles of a key head that these have room for
     float* scores;                // [sequence][key head][kept][width] raw scores of sequences of at most KV4_KEEP_COLUMNS columns, or null
     int kept; int64_t width;      // columns and entries that buffer has room for
+    // row of a column: col / group without a division (exact below 2^26, and there are at most 2^22 columns)
+    __device__ __forceinline__ int row(int col) const { return inv ? (int)__umulhi((unsigned)col, inv) : col; }
+    __device__ __forceinline__ const uint16_t* q_at(int row, int head_at) const { return q + (uint64_t)(unsigned)row * q_stride + head_at; }
+    __device__ __forceinline__ uint16_t* out_at(int row, int head_at) const { return out + (uint64_t)(unsigned)row * out_stride + head_at; }
 };
 // state of (chunk, tile): m[16], l[16], O[16][hd]
 template <int HD> __device__ __forceinline__ int64_t kv4_state_at(const Kv4Attn& a, int Hkv, int seq, int h, int tile, int chunk) {
     return ((((int64_t)seq * Hkv + h) * a.tiles + tile) * a.chunks + chunk) * (16 * (HD + 2));
+}
+
+// first column of a sequence and key head: sequences in order take disjoint tiles, for floor((a + b) / 16) + 1 >= floor(a / 16) +
+// ceil(b / 16), and never one outside the buffer
+__device__ __forceinline__ int64_t kv4_column(const Kv4Attn& a, int h, int seq, const Kv4Seq& s) {
+    return ((int64_t)h * a.slots + (s.start * a.group >> 4) + seq) * 16;
 }
 
 template <int HD> struct Kv4Page {
@@ -66,47 +79,62 @@ __device__ __forceinline__ unsigned kv4_byte(unsigned w, int i) { return w >> (8
 // Q of one column tile: step x of the product takes dims g hd/4 + 8 x .. + 7 of lane group g
 template <int HD, bool F16> struct Kv4Query {
     bf16x8 q[(F16 ? 2 : 1) * HD / 32];
-    __device__ __forceinline__ void load(const uint16_t* row, int lane) {          // null: a column that is none
-        const int g = lane >> 4;
+    __device__ __forceinline__ void set(int x, u32x4 w) {
+        if constexpr (F16) {
+            const f16x8 f = __builtin_bit_cast(f16x8, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const __bf16 hi = (__bf16)(float)f[e];
+                q[x][e] = hi;
+                q[HD / 32 + x][e] = (__bf16)((float)f[e] - (float)hi);
+            }
+        } else {
+            q[x] = __builtin_bit_cast(bf16x8, w);
+        }
+    }
+    // from a row (null: a column that is none), and, if wanted, on to where the weights' pass finds the tile
+    __device__ __forceinline__ void load(const uint16_t* row, int lane, uint8_t* keep) {
 #pragma unroll
         for (int x = 0; x < HD / 32; ++x) {
             u32x4 w = {0u, 0u, 0u, 0u};
-            if (row) w = *reinterpret_cast<const u32x4*>(row + g * (HD / 4) + 8 * x);
-            if constexpr (F16) {
-                const f16x8 f = __builtin_bit_cast(f16x8, w);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const __bf16 hi = (__bf16)(float)f[e];
-                    q[x][e] = hi;
-                    q[HD / 32 + x][e] = (__bf16)((float)f[e] - (float)hi);
-                }
-            } else {
-                q[x] = __builtin_bit_cast(bf16x8, w);
-            }
+            if (row) w = *reinterpret_cast<const u32x4*>(row + (lane >> 4) * (HD / 4) + 8 * x);
+            if (keep) *reinterpret_cast<u32x4*>(keep + x * 1024 + lane * 16) = w;
+            set(x, w);
         }
     }
 };
 
-// S^T of a page for NC column tiles: s[n][i][j] = token 16 g + 4 j + i, column lane & 15
-template <int HD, bool F16, int NC>
-__device__ __forceinline__ void kv4_scores(const Kv4Page<HD>& pg, const Kv4Query<HD, F16> (&q)[NC], f32x4 (&s)[NC][4]) {
+// K of a page as operands of the first product: tile i, step x
+template <int HD> __device__ __forceinline__ void kv4_operands(const Kv4Page<HD>& pg, bf16x8 (&kf)[4][HD / 32]) {
     const unsigned ks = pg.ks | pg.bad_k;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float sc = kv4_scale(kv4_byte(ks, i));
 #pragma unroll
-        for (int n = 0; n < NC; ++n) s[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
         for (int x = 0; x < HD / 32; ++x) {
             const unsigned w = HD == 64 ? pg.k[i / 2][i % 2 * 2 + x] : pg.k[HD == 64 ? 0 : i][x];
             const u32x4 a = {kv4_pair<0>(w, sc), kv4_pair<1>(w, sc), kv4_pair<2>(w, sc), kv4_pair<3>(w, sc)};
-            const bf16x8 af = __builtin_bit_cast(bf16x8, a);
+            kf[i][x] = __builtin_bit_cast(bf16x8, a);
+        }
+    }
+}
+
+// S^T of a page for NC column tiles: s[n][i][j] = token 16 g + 4 j + i, column lane & 15
+template <int HD, bool F16, int NC>
+__device__ __forceinline__ void kv4_scores(const Kv4Page<HD>& pg, const Kv4Query<HD, F16> (&q)[NC], f32x4 (&s)[NC][4]) {
+    bf16x8 kf[4][HD / 32];
+    kv4_operands<HD>(pg, kf);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int n = 0; n < NC; ++n) s[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < HD / 32; ++x)
 #pragma unroll
             for (int n = 0; n < NC; ++n) {
-                s[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, q[n].q[x], s[n][i], 0, 0, 0);
-                if constexpr (F16) s[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af, q[n].q[HD / 32 + x], s[n][i], 0, 0, 0);
+                s[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i][x], q[n].q[x], s[n][i], 0, 0, 0);
+                if constexpr (F16) s[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i][x], q[n].q[HD / 32 + x], s[n][i], 0, 0, 0);
             }
-        }
     }
 }
 
@@ -279,22 +307,26 @@ template <int HD> __device__ __forceinline__ void kv4_fetch_v(Kv4Page<HD>& pg, c
 // NaN into the rows of columns [c0, c1) of a sequence and key head
 template <int HD> __device__ void kv4_fill_columns(const Kv4Attn& a, const Kv4Seq& s, int h, int c0, int c1, int tid, int threads) {
     for (int i = tid; i < (c1 - c0) * (HD / 8); i += threads) {
-        const int col = c0 + i / (HD / 8), j = col / a.group, head = h * a.group + col % a.group;
+        const int col = c0 + i / (HD / 8), j = a.row(col), head = h * a.group + col - j * a.group;
         const u32x4 w = {KV4_NAN2, KV4_NAN2, KV4_NAN2, KV4_NAN2};
-        *reinterpret_cast<u32x4*>(a.out + (int64_t)(s.start + j) * a.out_stride + head * HD + i % (HD / 8) * 8) = w;
+        *reinterpret_cast<u32x4*>(a.out_at(s.start + j, head * HD + i % (HD / 8) * 8)) = w;
     }
 }
 
 // ------------------------------------------------------------------------------------------------------------------
 // Few columns: one workgroup per (chunk, tile of 16 columns and key head, sequence).
 // ------------------------------------------------------------------------------------------------------------------
+template <int HD> struct Kv4FewLds {
+    float m[4][2][16];
+    __attribute__((aligned(16))) float o[4][16][HD + 4];
+};
+
 template <int HD, bool F16>
-__global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_few_kernel(Kv4View c, Kv4Rows b, Kv4Attn a) {
-    __shared__ float sm[4][2][16];
-    __shared__ __attribute__((aligned(16))) float so[4][16][HD + 4];
+__device__ __forceinline__ void kv4_few_block(const Kv4View& c, const Kv4Rows& b, const Kv4Attn& a, Kv4FewLds<HD>& lds, int h, int tile, int seq, int chunk) {
+    float (&sm)[4][2][16] = lds.m;
+    float (&so)[4][16][HD + 4] = lds.o;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int h = blockIdx.x % c.Hkv, tile = blockIdx.x / c.Hkv, chunk = blockIdx.z, H = c.Hkv * a.group;
-    const Kv4Seq s = kv4_seq_of(b, c, blockIdx.y);
+    const Kv4Seq s = kv4_seq_of(b, c, seq);
     const int rows = s.n < b.max_rows ? s.n : b.max_rows;
     const int cols = rows * a.group;
     if (s.state == 1 || cols > KV4_FEW_COLUMNS || tile * 16 >= cols) return;
@@ -306,11 +338,12 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_few_kernel(Kv4
     const int chunks = kv4_chunks(s.ctx);
     if (chunk >= (chunks > 0 ? chunks : 1)) return;
 
-    const int col = tile * 16 + (lane & 15), j = col / a.group, head = h * a.group + col % a.group;
+    const int col = tile * 16 + (lane & 15), j = a.row(col), head = h * a.group + col - j * a.group;
     const int sees = col < cols ? s.ctx - s.n + j + 1 : 0;        // entries that this lane's column sees, may be <= 0
-    const int least = s.ctx - s.n + (tile * 16) / a.group + 1;    // what the tile's first row sees
+    const int least = s.ctx - s.n + a.row(tile * 16) + 1;    // what the tile's first row sees
     Kv4Query<HD, F16> q[1];
-    q[0].load(col < cols ? a.q + (int64_t)(s.start + j) * a.q_stride + head * HD : nullptr, lane);
+    q[0].load(col < cols ? a.q_at(s.start + j, head * HD) : nullptr, lane,
+              a.frags && cols > KV4_KEEP_COLUMNS && chunk == 0 && w == 0 ? a.frags + (kv4_column(a, h, seq, s) + tile * 16) * (2 * HD) : nullptr);
     Kv4State<HD, 1> st;
     st.clear();
 
@@ -322,7 +355,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_few_kernel(Kv4
     const int ids = lane < np ? bt[lane] : -1;
     // where the lane's 16 tokens' scores go, if they are wanted
     float* keep = a.scores && cols <= KV4_KEEP_COLUMNS && col < cols
-                      ? a.scores + ((int64_t)(blockIdx.y * c.Hkv + h) * a.kept + col) * a.width + 16 * (lane >> 4) : nullptr;
+                      ? a.scores + (((int64_t)seq * c.Hkv + h) * a.kept + col) * a.width + 16 * (lane >> 4) : nullptr;
     Kv4Page<HD> pg;
     if (w < np) {
         const int id = __builtin_amdgcn_readlane(ids, w);
@@ -384,20 +417,26 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_few_kernel(Kv4
             for (int e = 0; e < 8; ++e) o[e] = fmaf(so[x][k][d + e], f, o[e]);
         }
         if (chunks > 1) {
-            float* sp = a.states + kv4_state_at<HD>(a, c.Hkv, blockIdx.y, h, tile, chunk);
+            float* sp = a.states + kv4_state_at<HD>(a, c.Hkv, seq, h, tile, chunk);
             if (d == 0) { sp[k] = M; sp[16 + k] = L; }
 #pragma unroll
             for (int e = 0; e < 8; e += 4)
                 *reinterpret_cast<f32x4*>(sp + 32 + k * HD + d + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
         } else {
-            const int jj = kcol / a.group, hh = h * a.group + kcol % a.group;
+            const int jj = a.row(kcol), hh = h * a.group + kcol - jj * a.group;
             const float inv = L == 0.f ? 0.f : 1.0f / L;          // nothing seen: 0 (a NaN stays one)
             const u32x4 r = {kv4_pack2<F16>(o[0] * inv, o[1] * inv), kv4_pack2<F16>(o[2] * inv, o[3] * inv),
                              kv4_pack2<F16>(o[4] * inv, o[5] * inv), kv4_pack2<F16>(o[6] * inv, o[7] * inv)};
-            *reinterpret_cast<u32x4*>(a.out + (int64_t)(s.start + jj) * a.out_stride + hh * HD + d) = r;
-            if (a.norm && d == 0) a.norm[(int64_t)(s.start + jj) * H + hh] = f32x2{M, inv};
+            *reinterpret_cast<u32x4*>(a.out_at(s.start + jj, hh * HD + d)) = r;
+            if (a.norm && d == 0) a.norm[kv4_column(a, h, seq, s) + kcol] = f32x2{M, inv};
         }
     }
+}
+
+template <int HD, bool F16>
+__global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_few_kernel(Kv4View c, Kv4Rows b, Kv4Attn a) {
+    __shared__ Kv4FewLds<HD> lds;
+    kv4_few_block<HD, F16>(c, b, a, lds, blockIdx.x % c.Hkv, blockIdx.x / c.Hkv, blockIdx.y, blockIdx.z);
 }
 
 // Joins the chunks of a column.  A thread has 4 dims; 1024 / HD groups of threads walk the chunks side by side, group x the chunks
@@ -407,7 +446,7 @@ __global__ __launch_bounds__(256) void kv4_attn_join_kernel(Kv4View c, Kv4Rows b
     constexpr int T = HD / 4, GROUPS = 256 / T, step = 16 * (HD + 2);
     __shared__ float sm[GROUPS][2];
     __shared__ __attribute__((aligned(16))) f32x4 so[GROUPS][T];
-    const int h = blockIdx.x % c.Hkv, col = blockIdx.x / c.Hkv, H = c.Hkv * a.group;
+    const int h = blockIdx.x % c.Hkv, col = blockIdx.x / c.Hkv;
     const Kv4Seq s = kv4_seq_of(b, c, blockIdx.y);
     const int rows = s.n < b.max_rows ? s.n : b.max_rows, cols = rows * a.group;
     if (s.state || cols > KV4_FEW_COLUMNS || col >= cols) return;
@@ -443,11 +482,11 @@ __global__ __launch_bounds__(256) void kv4_attn_join_kernel(Kv4View c, Kv4Rows b
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = fmaf(so[x][t][e], f, o[e]);
     }
-    const int j = col / a.group, head = h * a.group + col % a.group;
+    const int j = a.row(col), head = h * a.group + col - j * a.group;
     const float inv = L == 0.f ? 0.f : 1.0f / L;
     const u32x2 r = {kv4_pack2<F16>(o[0] * inv, o[1] * inv), kv4_pack2<F16>(o[2] * inv, o[3] * inv)};
-    *reinterpret_cast<u32x2*>(a.out + (int64_t)(s.start + j) * a.out_stride + head * HD + 4 * t) = r;
-    if (a.norm && t == 0) a.norm[(int64_t)(s.start + j) * H + head] = f32x2{M, inv};
+    *reinterpret_cast<u32x2*>(a.out_at(s.start + j, head * HD + 4 * t)) = r;
+    if (a.norm && t == 0) a.norm[kv4_column(a, h, blockIdx.y, s) + col] = f32x2{M, inv};
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -571,17 +610,19 @@ __device__ __forceinline__ void kv4_lds_values(const uint8_t* vbuf, const bf16x8
             }
 }
 
+template <int HD> struct Kv4ManyLds { __attribute__((aligned(16))) uint8_t k[2][128 * HD], v[2][128 * HD]; };
+
 template <int HD, bool F16, int NC>
-__global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_many_kernel(Kv4View c, Kv4Rows b, Kv4Attn a) {
-    __shared__ __attribute__((aligned(16))) uint8_t kbuf[2][128 * HD], vbuf[2][128 * HD];
+__device__ __forceinline__ void kv4_many_block(const Kv4View& c, const Kv4Rows& b, const Kv4Attn& a, Kv4ManyLds<HD>& lds, int h, int turn, int seq) {
+    uint8_t (&kbuf)[2][128 * HD] = lds.k;
+    uint8_t (&vbuf)[2][128 * HD] = lds.v;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
-    const int h = blockIdx.x, H = c.Hkv * a.group;
-    const Kv4Seq s = kv4_seq_of(b, c, blockIdx.z);
+    const Kv4Seq s = kv4_seq_of(b, c, seq);
     const int rows = s.n < b.max_rows ? s.n : b.max_rows, cols = rows * a.group;
     if (s.state == 1 || cols <= KV4_FEW_COLUMNS) return;
     // the last tiles see most: they start first
     constexpr int COLS = 64 * NC;
-    const int block = (cols + COLS - 1) / COLS - 1 - (int)blockIdx.y;
+    const int block = (cols + COLS - 1) / COLS - 1 - turn;
     if (block < 0) return;
     const int c0 = (block * 4 + w) * (16 * NC), c1 = cols < c0 + 16 * NC ? cols : c0 + 16 * NC;
     if (s.state == 2) {
@@ -592,13 +633,14 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_many_kernel(Kv
     int sees[NC], seen[NC];
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-        const int col = c0 + 16 * n + (lane & 15), j = col / a.group;
-        q[n].load(col < c1 ? a.q + (int64_t)(s.start + j) * a.q_stride + (h * a.group + col % a.group) * HD : nullptr, lane);
+        const int col = c0 + 16 * n + (lane & 15), j = a.row(col);
+        q[n].load(col < c1 ? a.q_at(s.start + j, (h * a.group + col - j * a.group) * HD) : nullptr, lane,
+                  a.frags && c0 + 16 * n < c1 ? a.frags + (kv4_column(a, h, seq, s) + c0 + 16 * n) * (2 * HD) : nullptr);
         sees[n] = col < c1 ? s.ctx - s.n + j + 1 : 0;
     }
     // what the wave's first and last row see; a wave without columns sees nothing and only converts
-    const int base = s.ctx - s.n + 1, least = base + c0 / a.group, most = c0 < cols ? base + (c1 - 1) / a.group : 0;
-    const int end = block * COLS + COLS, all = base + ((cols < end ? cols : end) - 1) / a.group;      // the workgroup's last row
+    const int base = s.ctx - s.n + 1, least = base + a.row(c0), most = c0 < cols ? base + a.row(c1 - 1) : 0;
+    const int end = block * COLS + COLS, all = base + a.row((cols < end ? cols : end) - 1);      // the workgroup's last row
     Kv4State<HD, NC> st;
     st.clear();
     const int32_t* bt = c.table + (int64_t)s.stream * c.max_pages;
@@ -650,11 +692,11 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_many_kernel(Kv
     }
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-        const int col = c0 + 16 * n + (lane & 15), j = col / a.group, head = h * a.group + col % a.group;
+        const int col = c0 + 16 * n + (lane & 15), j = a.row(col), head = h * a.group + col - j * a.group;
         const float l = kv4_group_sum(st.l[n]);
         if (col >= c1) continue;
         const float inv = l == 0.f ? 0.f : 1.0f / l;
-        uint16_t* op = a.out + (int64_t)(s.start + j) * a.out_stride + head * HD + 16 * g;
+        uint16_t* op = a.out_at(s.start + j, head * HD + 16 * g);
 #pragma unroll
         for (int x = 0; x < HD / 64; ++x)
 #pragma unroll
@@ -664,7 +706,27 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_many_kernel(Kv
                                  kv4_pack2<F16>(o[0][jj + 1] * inv, o[1][jj + 1] * inv), kv4_pack2<F16>(o[2][jj + 1] * inv, o[3][jj + 1] * inv)};
                 *reinterpret_cast<u32x4*>(op + 64 * x + 4 * jj) = r;
             }
-        if (a.norm && g == 0) a.norm[(int64_t)(s.start + j) * H + head] = f32x2{st.m[n], inv};
+        if (a.norm && g == 0) a.norm[kv4_column(a, h, seq, s) + col] = f32x2{st.m[n], inv};
+    }
+}
+
+// Both in one launch, for a batch that may hold sequences of either kind: the long blocks start first.
+template <int HD, bool F16, int NC>
+__global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_mixed_kernel(Kv4View c, Kv4Rows b, Kv4Attn a, int turns) {
+    __shared__ union { Kv4ManyLds<HD> many; Kv4FewLds<HD> few; } lds;
+    const unsigned many = (unsigned)c.Hkv * turns * b.n_seqs;
+    unsigned x = blockIdx.x;
+    if (x < many) {
+        const int h = x % c.Hkv;
+        x /= c.Hkv;
+        kv4_many_block<HD, F16, NC>(c, b, a, lds.many, h, x % turns, x / turns);
+    } else {
+        x -= many;
+        const int h = x % c.Hkv;
+        x /= c.Hkv;
+        const int tile = x % a.tiles;
+        x /= a.tiles;
+        kv4_few_block<HD, F16>(c, b, a, lds.few, h, tile, x % b.n_seqs, x / b.n_seqs);
     }
 }
 
@@ -688,7 +750,7 @@ template <typename Fn> __device__ __forceinline__ bool kv4_of_stream(const Kv4Ro
 
 // Every sequence of the call has its scores kept: a thread four entries.
 __global__ __launch_bounds__(256) void kv4_weights_kept_kernel(Kv4View c, Kv4Rows b, Kv4Attn a, float* weights, int64_t weights_stride) {
-    const int lane = threadIdx.x & 63, h = blockIdx.y, H = c.Hkv * a.group, seq = blockIdx.z, stream = b.stream[seq];
+    const int lane = threadIdx.x & 63, h = blockIdx.y, seq = blockIdx.z, stream = b.stream[seq];
     if (stream < 0 || stream >= c.n_streams) return;
     const int first = (blockIdx.x * 256 + threadIdx.x) * 4;
     f32x4 mine = {0.f, 0.f, 0.f, 0.f};
@@ -698,8 +760,8 @@ __global__ __launch_bounds__(256) void kv4_weights_kept_kernel(Kv4View c, Kv4Row
         const int rows = s.n < b.max_rows ? s.n : b.max_rows, cols = rows * a.group;
         const float* sp = a.scores + (int64_t)(i * c.Hkv + h) * a.kept * a.width + first;
         for (int col = 0; col < cols; ++col) {
-            const int j = col / a.group, seen = s.ctx - s.n + j + 1 - first;
-            const f32x2 norm = a.norm[(int64_t)(s.start + j) * H + h * a.group + col % a.group];
+            const int j = a.row(col), seen = s.ctx - s.n + j + 1 - first;
+            const f32x2 norm = a.norm[kv4_column(a, h, i, s) + col];
             const f32x4 x = *reinterpret_cast<const f32x4*>(sp + col * a.width);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -715,14 +777,16 @@ __global__ __launch_bounds__(256) void kv4_weights_kept_kernel(Kv4View c, Kv4Row
         if (mine[e] != 0.f && first + e < weights_stride) wp[e] += mine[e];
 }
 
+// Some have not: a workgroup per (page, key head, stream).  A wave keeps the page's keys as operands, takes every fourth column tile
+// (the next one's queries are under way meanwhile) and sums over its tiles and their columns; the waves are added in order.
 template <int HD, bool F16>
-__global__ __launch_bounds__(256) void kv4_weights_kernel(Kv4View c, Kv4Rows b, Kv4Attn a, float* weights, int64_t weights_stride) {
-    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int h = blockIdx.y, H = c.Hkv * a.group, seq = blockIdx.z, p = blockIdx.x * 4 + w, first = p * KV4_PAGE;
+__global__ __launch_bounds__(256, 2) void kv4_weights_kernel(Kv4View c, Kv4Rows b, Kv4Attn a, float* weights, int64_t weights_stride) {
+    __shared__ float part[4][KV4_PAGE];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
+    const int h = blockIdx.y, seq = blockIdx.z, p = blockIdx.x, first = p * KV4_PAGE;
     const int stream = b.stream[seq];
     if (stream < 0 || stream >= c.n_streams) return;
-    const int32_t* bt = c.table + (int64_t)stream * c.max_pages;
-    Kv4Page<HD> pg;
+    bf16x8 kf[4][HD / 32];
     bool have = false;
     float mine = 0.f;                                             // of token first + lane
     const bool own = kv4_of_stream(b, seq, stream, lane, [&](int i) {
@@ -731,38 +795,71 @@ __global__ __launch_bounds__(256) void kv4_weights_kernel(Kv4View c, Kv4Rows b, 
         const int rows = s.n < b.max_rows ? s.n : b.max_rows, cols = rows * a.group;
         if (a.scores && cols <= KV4_KEEP_COLUMNS) {
             const float* sp = a.scores + (int64_t)(i * c.Hkv + h) * a.kept * a.width + first + lane;
-            for (int col = 0; col < cols; ++col) {
-                const int j = col / a.group;
-                const f32x2 norm = a.norm[(int64_t)(s.start + j) * H + h * a.group + col % a.group];
+            for (int col = 0; w == 0 && col < cols; ++col) {
+                const int j = a.row(col);
+                const f32x2 norm = a.norm[kv4_column(a, h, i, s) + col];
                 const float v = __builtin_amdgcn_exp2f(fmaf(sp[col * a.width], a.c, -norm[0]));
                 mine += first + lane < s.ctx - s.n + j + 1 ? v * norm[1] : 0.f;
             }
             return;
         }
         if (!have) {
-            kv4_fetch_k<HD>(pg, c, __builtin_amdgcn_readfirstlane(bt[p]), h, lane);
+            Kv4Page<HD> pg;
+            kv4_fetch_k<HD>(pg, c, __builtin_amdgcn_readfirstlane(c.table[(int64_t)stream * c.max_pages + p]), h, lane);
+            kv4_operands<HD>(pg, kf);
             have = true;
         }
         float sum[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) sum[e] = 0.f;
         // rows before the first that sees this page add nothing
-        int j0 = first - (s.ctx - s.n);
-        j0 = j0 < 0 ? 0 : j0;
-        for (int c0 = j0 * a.group / 16 * 16; c0 < cols; c0 += 16) {
-            const int col = c0 + (lane & 15), j = col / a.group, head = h * a.group + col % a.group;
-            Kv4Query<HD, F16> q[1];
-            q[0].load(col < cols ? a.q + (int64_t)(s.start + j) * a.q_stride + head * HD : nullptr, lane);
-            f32x2 norm = {0.f, 0.f};
-            if (col < cols) norm = a.norm[(int64_t)(s.start + j) * H + head];
-            const int seen = col < cols ? s.ctx - s.n + j + 1 - first : 0;
-            f32x4 sc[1][4];
-            kv4_scores<HD, F16, 1>(pg, q, sc);
+        const int base = s.ctx - s.n + 1, j0 = first + 1 - base;
+        const int t0 = j0 > 0 ? j0 * a.group / 16 : 0, tiles = (cols + 15) / 16;
+        // the tiles' queries as the pass above left them (54 cache lines' lookups a load become 16) and their columns' norms
+        const int64_t column = kv4_column(a, h, i, s);
+        const uint8_t* qp = a.frags + column * (2 * HD) + lane * 16;
+        const f32x2* np = a.norm + column + (lane & 15);
+        struct Tile { u32x4 q[HD / 32]; f32x2 norm; int col; } even, odd;
+        const auto fetch = [&](Tile& t, int tile) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float v = __builtin_amdgcn_exp2f(fmaf(sc[0][e & 3][e >> 2], a.c, -norm[0]));
-                sum[e] += 16 * (lane >> 4) + e < seen ? v * norm[1] : 0.f;
+            for (int x = 0; x < HD / 32; ++x) t.q[x] = *reinterpret_cast<const u32x4*>(qp + (int64_t)tile * (32 * HD) + x * 1024);
+            t.norm = np[tile * 16];
+            t.col = tile * 16 + (lane & 15);
+        };
+        const auto add = [&](const Tile& t) {
+            Kv4Query<HD, F16> q;
+#pragma unroll
+            for (int x = 0; x < HD / 32; ++x) q.set(x, t.q[x]);
+            const int seen = t.col < cols ? base + a.row(t.col) - first - 16 * g : 0;      // of the lane's 16 tokens
+            f32x4 sc[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int x = 0; x < HD / 32; ++x)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i][x], q.q[x], sc[i], 0, 0, 0);
+                    if constexpr (F16) sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i][x], q.q[HD / 32 + x], sc[i], 0, 0, 0);
+                }
+            if (__all(seen >= 16)) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    sum[e] = fmaf(__builtin_amdgcn_exp2f(fmaf(sc[e & 3][e >> 2], a.c, -t.norm[0])), t.norm[1], sum[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float v = __builtin_amdgcn_exp2f(fmaf(sc[e & 3][e >> 2], a.c, -t.norm[0]));
+                    sum[e] = e < seen ? fmaf(v, t.norm[1], sum[e]) : sum[e];
+                }
             }
+        };
+        int tile = t0 + w;
+        if (tile < tiles) fetch(even, tile);
+        for (; tile < tiles; tile += 8) {
+            fetch(odd, tile + 4 < tiles ? tile + 4 : tile);
+            add(even);
+            fetch(even, tile + 8 < tiles ? tile + 8 : tile);
+            if (tile + 4 < tiles) add(odd);
         }
         // over the 16 columns; lane r of a group takes token 16 g + r
 #pragma unroll
@@ -774,18 +871,22 @@ __global__ __launch_bounds__(256) void kv4_weights_kernel(Kv4View c, Kv4Rows b, 
             mine += (lane & 15) == e ? sum[e] : 0.f;
         }
     });
+    if (!own) return;                                             // the same in all waves
+    part[w][lane] = mine;
+    __syncthreads();
     const int64_t t = first + lane;
-    if (own && t < weights_stride) {
+    if (w == 0 && t < weights_stride) {
+        const float all = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
         float* wp = weights + ((int64_t)stream * c.Hkv + h) * weights_stride + t;
-        if (mine != 0.f) *wp += mine;
+        if (all != 0.f) *wp += all;
     }
 }
 
 // ------------------------------------------------------------------------------------------------------------------
 // Entry points
 // ------------------------------------------------------------------------------------------------------------------
-// the work buffer: chunk states | kept scores | m and 1 / l
-struct Kv4Work { int64_t states, scores, norm, width; int tiles, chunks, kept; };
+// the work buffer: chunk states | kept scores | m and 1 / l | queries
+struct Kv4Work { int64_t states, scores, norm, frags, width; int tiles, chunks, kept, slots; };
 static Kv4Work plan_work(const t3_kv4_cache* c, const t3_kv4_batch* b, int H, bool weights) {
     Kv4Work w{};
     const int64_t cols = (int64_t)b->max_rows * (H / c->Hkv), few = cols < KV4_FEW_COLUMNS ? cols : KV4_FEW_COLUMNS;
@@ -797,7 +898,9 @@ static Kv4Work plan_work(const t3_kv4_cache* c, const t3_kv4_batch* b, int H, bo
         w.kept = (int)(few < KV4_KEEP_COLUMNS ? few : KV4_KEEP_COLUMNS);
         w.width = (most + KV4_PAGE - 1) / KV4_PAGE * KV4_PAGE;
         w.scores = pairs * w.kept * w.width * 4;
-        w.norm = (int64_t)b->rows * H * 8;
+        w.slots = (int)((int64_t)b->rows * (H / c->Hkv) / 16) + b->n_seqs + 1;
+        w.norm = (int64_t)c->Hkv * w.slots * 16 * 8;
+        w.frags = cols > KV4_KEEP_COLUMNS ? (int64_t)c->Hkv * w.slots * 16 * c->hd * 2 : 0;
     }
     return w;
 }
@@ -809,7 +912,7 @@ static int check_heads(const t3_kv4_cache* c, int H) {
 extern "C" int64_t t3_op_attn_kv4_work_bytes(const t3_kv4_cache* cache, const t3_kv4_batch* batch, int32_t H, int32_t with_weights) {
     if (kv4_check_cache(cache, 0, 1, nullptr) || kv4_check_batch(batch) || check_heads(cache, H)) return -1;
     const Kv4Work w = plan_work(cache, batch, H, with_weights != 0);
-    return (w.states + w.scores + w.norm + 15) / 16 * 16;
+    return w.states + w.scores + w.norm + w.frags;
 }
 
 template <int HD, bool F16>
@@ -818,17 +921,21 @@ static int launch_attn(const Kv4View& c, const Kv4Rows& b, const Kv4Attn& a, flo
     // hd 64 one leaves room for four waves a SIMD instead of two (4 x 2000 rows 70.6 us; two 78, four 98)
     constexpr int NC = HD == 64 ? 1 : 2;
     const int64_t cols = (int64_t)b.max_rows * a.group;
-    T3_LAUNCH((kv4_attn_few_kernel<HD, F16>), dim3(a.tiles * c.Hkv, b.n_seqs, a.chunks), dim3(256), 0, st, c, b, a);
+    if (cols <= KV4_FEW_COLUMNS) {
+        T3_LAUNCH((kv4_attn_few_kernel<HD, F16>), dim3(a.tiles * c.Hkv, b.n_seqs, a.chunks), dim3(256), 0, st, c, b, a);
+    } else {
+        const int64_t turns = (cols + 64 * NC - 1) / (64 * NC), blocks = c.Hkv * (int64_t)b.n_seqs * (turns + (int64_t)a.tiles * a.chunks);
+        T3_REQUIRE(blocks <= INT32_MAX, "attn_kv4: too many sequences of that many rows in one call");
+        T3_LAUNCH((kv4_attn_mixed_kernel<HD, F16, NC>), dim3((unsigned)blocks), dim3(256), 0, st, c, b, a, (int)turns);
+    }
     if (a.chunks > 1)
         T3_LAUNCH((kv4_attn_join_kernel<HD, F16>), dim3((cols < KV4_FEW_COLUMNS ? (int)cols : KV4_FEW_COLUMNS) * c.Hkv, b.n_seqs), dim3(256), 0, st, c, b, a);
-    if (cols > KV4_FEW_COLUMNS)
-        T3_LAUNCH((kv4_attn_many_kernel<HD, F16, NC>), dim3(c.Hkv, (unsigned)((cols + 64 * NC - 1) / (64 * NC)), b.n_seqs), dim3(256), 0, st, c, b, a);
     if (weights) {
         const int64_t cap = (int64_t)c.max_pages * KV4_PAGE, most = b.max_ctx < cap ? b.max_ctx : cap;
         if (cols <= KV4_KEEP_COLUMNS)
             T3_LAUNCH(kv4_weights_kept_kernel, dim3((unsigned)((most + 1023) / 1024), c.Hkv, b.n_seqs), dim3(256), 0, st, c, b, a, weights, weights_stride);
         else
-            T3_LAUNCH((kv4_weights_kernel<HD, F16>), dim3((unsigned)((most + 4 * KV4_PAGE - 1) / (4 * KV4_PAGE)), c.Hkv, b.n_seqs), dim3(256), 0, st,
+            T3_LAUNCH((kv4_weights_kernel<HD, F16>), dim3((unsigned)((most + KV4_PAGE - 1) / KV4_PAGE), c.Hkv, b.n_seqs), dim3(256), 0, st,
                   c, b, a, weights, weights_stride);
     }
     T3_HIP_CHECK(hipGetLastError());
@@ -844,18 +951,21 @@ extern "C" int t3_op_attn_kv4(const t3_kv4_cache* cache, const t3_kv4_batch* bat
     T3_REQUIRE(dtype == 0 || dtype == 1, "attn_kv4: dtype must be 0 (bf16) or 1 (fp16)");
     T3_REQUIRE(scale > 0.f && scale < 1e8f, "attn_kv4: scale must be positive");
     T3_REQUIRE((int64_t)batch->max_rows * (H / cache->Hkv) <= (1 << 22), "attn_kv4: more than 2^22 rows x query heads of a key head");
+    T3_REQUIRE((int64_t)batch->rows * (H / cache->Hkv) <= (1 << 30), "attn_kv4: more than 2^30 rows x query heads of a key head in one call");
     const int64_t width = (int64_t)H * cache->hd;
     T3_REQUIRE(q_stride >= width && out_stride >= width && q_stride % 8 == 0 && out_stride % 8 == 0 &&
                reinterpret_cast<uintptr_t>(q_dev) % 16 == 0 && reinterpret_cast<uintptr_t>(out_dev) % 16 == 0,
                "attn_kv4: rows must be 16-byte aligned and must not overlap");
+    T3_REQUIRE(q_stride <= INT32_MAX && out_stride <= INT32_MAX, "attn_kv4: row stride of more than 2^31 elements");
     T3_REQUIRE(!weights_dev || weights_stride >= batch->max_ctx, "attn_kv4: weights_stride must be at least max_ctx");
     const int64_t needed = t3_op_attn_kv4_work_bytes(cache, batch, H, weights_dev != nullptr);
     T3_REQUIRE(needed == 0 || (work_dev && work_bytes >= needed && reinterpret_cast<uintptr_t>(work_dev) % 16 == 0),
                "attn_kv4: the work buffer is too small or not 16-byte aligned");
     Kv4Attn a{};
-    a.q = static_cast<const uint16_t*>(q_dev); a.q_stride = q_stride;
-    a.out = static_cast<uint16_t*>(out_dev); a.out_stride = out_stride;
+    a.q = static_cast<const uint16_t*>(q_dev); a.q_stride = (unsigned)q_stride;
+    a.out = static_cast<uint16_t*>(out_dev); a.out_stride = (unsigned)out_stride;
     a.group = H / cache->Hkv;
+    a.inv = a.group == 1 ? 0u : (unsigned)(((1ull << 32) + a.group - 1) / a.group);
     a.c = scale * 1.44269504088896340736f;
     const Kv4Work w = plan_work(cache, batch, H, weights_dev != nullptr);
     uint8_t* work = static_cast<uint8_t*>(work_dev);
@@ -863,6 +973,8 @@ extern "C" int t3_op_attn_kv4(const t3_kv4_cache* cache, const t3_kv4_batch* bat
     a.states = reinterpret_cast<float*>(work);
     a.scores = w.scores ? reinterpret_cast<float*>(work + w.states) : nullptr;
     a.norm = weights_dev ? reinterpret_cast<f32x2*>(work + w.states + w.scores) : nullptr;
+    a.frags = w.frags ? work + w.states + w.scores + w.norm : nullptr;
+    a.slots = w.slots;
     const Kv4View c = kv4_view(cache, layer);
     const Kv4Rows b = kv4_rows(batch);
     if (cache->hd == 64) return dtype ? launch_attn<64, true>(c, b, a, weights_dev, weights_stride, st) : launch_attn<64, false>(c, b, a, weights_dev, weights_stride, st);
