@@ -20,13 +20,19 @@
 #include <type_traits>
 
 #define KV4_FEW_COLUMNS 64        // rows x group up to which a sequence is cut along its cache
-#define KV4_KEEP_COLUMNS 16       // columns up to which the scores are kept for the weights
 #define KV4_SLACK 8.f             // the reference moves when a maximum passes it by 2^8
 #define KV4_NONE -1e30f           // running maximum before the first visible token
 
 // A chunk is 16 pages: the four waves of its workgroup take four each.
 #define KV4_CHUNK_PAGES 16
 KV4_FN int kv4_chunks(int ctx) { return (int)(((int64_t)ctx + KV4_CHUNK_PAGES * KV4_PAGE - 1) / (KV4_CHUNK_PAGES * KV4_PAGE)); }
+
+// Where weights are wanted, the scores of a (sequence, key head) of few columns are kept if they are at most KV4_KEEP values (4 MiB).
+#ifndef KV4_KEEP
+#define KV4_KEEP (1 << 20)
+#endif
+KV4_FN int64_t kv4_kept_width(int64_t ctx) { return (ctx + KV4_PAGE - 1) / KV4_PAGE * KV4_PAGE; }
+KV4_FN bool kv4_kept(int cols, int ctx) { return cols <= KV4_FEW_COLUMNS && cols * kv4_kept_width(ctx) <= KV4_KEEP; }
 
 struct Kv4Attn {
     const uint16_t* q; uint16_t* out;
@@ -38,8 +44,8 @@ struct Kv4Attn {
     f32x2* norm;                  // m and 1 / l of each column
     uint8_t* frags;               // the queries of each tile as the product takes them: [hd / 32][64 lanes][16 bytes]
     int slots;                    // tiles of a key head that these have room for
-    float* scores;                // [sequence][key head][kept][width] raw scores of sequences of at most KV4_KEEP_COLUMNS columns, or null
-    int kept; int64_t width;      // columns and entries that buffer has room for
+    float* scores;                // [sequence][key head][room]: raw scores [column][kv4_kept_width], or null
+    int64_t room;
     // row of a column: col / group without a division (exact below 2^26, and there are at most 2^22 columns)
     __device__ __forceinline__ int row(int col) const { return inv ? (int)__umulhi((unsigned)col, inv) : col; }
     __device__ __forceinline__ const uint16_t* q_at(int row, int head_at) const { return q + (uint64_t)(unsigned)row * q_stride + head_at; }
@@ -343,7 +349,7 @@ __device__ __forceinline__ void kv4_few_block(const Kv4View& c, const Kv4Rows& b
     const int least = s.ctx - s.n + a.row(tile * 16) + 1;    // what the tile's first row sees
     Kv4Query<HD, F16> q[1];
     q[0].load(col < cols ? a.q_at(s.start + j, head * HD) : nullptr, lane,
-              a.frags && cols > KV4_KEEP_COLUMNS && chunk == 0 && w == 0 ? a.frags + (kv4_column(a, h, seq, s) + tile * 16) * (2 * HD) : nullptr);
+              a.frags && !kv4_kept(cols, s.ctx) && chunk == 0 && w == 0 ? a.frags + (kv4_column(a, h, seq, s) + tile * 16) * (2 * HD) : nullptr);
     Kv4State<HD, 1> st;
     st.clear();
 
@@ -354,8 +360,8 @@ __device__ __forceinline__ void kv4_few_block(const Kv4View& c, const Kv4Rows& b
     const int32_t* bt = c.table + (int64_t)s.stream * c.max_pages + p0;
     const int ids = lane < np ? bt[lane] : -1;
     // where the lane's 16 tokens' scores go, if they are wanted
-    float* keep = a.scores && cols <= KV4_KEEP_COLUMNS && col < cols
-                      ? a.scores + (((int64_t)seq * c.Hkv + h) * a.kept + col) * a.width + 16 * (lane >> 4) : nullptr;
+    float* keep = a.scores && col < cols && kv4_kept(cols, s.ctx)
+                      ? a.scores + ((int64_t)seq * c.Hkv + h) * a.room + col * kv4_kept_width(s.ctx) + 16 * (lane >> 4) : nullptr;
     Kv4Page<HD> pg;
     if (w < np) {
         const int id = __builtin_amdgcn_readlane(ids, w);
@@ -748,21 +754,27 @@ template <typename Fn> __device__ __forceinline__ bool kv4_of_stream(const Kv4Ro
     return true;
 }
 
-// Every sequence of the call has its scores kept: a thread four entries.
+// Every sequence of the call has its scores kept.  A thread has four entries; with GROUPS = 4 the workgroup's waves take every
+// fourth column each of the same entries and are added in order (the order of the single one while there are at most 4 columns).
+template <int GROUPS>
 __global__ __launch_bounds__(256) void kv4_weights_kept_kernel(Kv4View c, Kv4Rows b, Kv4Attn a, float* weights, int64_t weights_stride) {
-    const int lane = threadIdx.x & 63, h = blockIdx.y, seq = blockIdx.z, stream = b.stream[seq];
+    __shared__ f32x4 part[GROUPS][64];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = blockIdx.y, seq = blockIdx.z, stream = b.stream[seq];
     if (stream < 0 || stream >= c.n_streams) return;
-    const int first = (blockIdx.x * 256 + threadIdx.x) * 4;
+    const int first = (GROUPS == 1 ? blockIdx.x * 256 + threadIdx.x : blockIdx.x * 64 + lane) * 4;
     f32x4 mine = {0.f, 0.f, 0.f, 0.f};
     const bool own = kv4_of_stream(b, seq, stream, lane, [&](int i) {
         const Kv4Seq s = kv4_seq_of(b, c, i);
         if (s.state || first >= s.ctx) return;
         const int rows = s.n < b.max_rows ? s.n : b.max_rows, cols = rows * a.group;
-        const float* sp = a.scores + (int64_t)(i * c.Hkv + h) * a.kept * a.width + first;
-        for (int col = 0; col < cols; ++col) {
-            const int j = a.row(col), seen = s.ctx - s.n + j + 1 - first;
-            const f32x2 norm = a.norm[kv4_column(a, h, i, s) + col];
-            const f32x4 x = *reinterpret_cast<const f32x4*>(sp + col * a.width);
+        const int64_t width = kv4_kept_width(s.ctx);
+        const float* sp = a.scores + ((int64_t)i * c.Hkv + h) * a.room + first;
+        const f32x2* norms = a.norm + kv4_column(a, h, i, s);
+#pragma unroll 4
+        for (int col = GROUPS == 1 ? 0 : w; col < cols; col += GROUPS) {
+            const int seen = s.ctx - s.n + a.row(col) + 1 - first;
+            const f32x2 norm = norms[col];
+            const f32x4 x = *reinterpret_cast<const f32x4*>(sp + col * width);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float v = __builtin_amdgcn_exp2f(fmaf(x[e], a.c, -norm[0]));
@@ -770,7 +782,14 @@ __global__ __launch_bounds__(256) void kv4_weights_kept_kernel(Kv4View c, Kv4Row
             }
         }
     });
-    if (!own) return;
+    if (!own) return;                                             // the same in all waves
+    if constexpr (GROUPS > 1) {
+        part[w][lane] = mine;
+        __syncthreads();
+        if (w) return;
+#pragma unroll
+        for (int x = 1; x < GROUPS; ++x) mine += part[x][lane];
+    }
     float* wp = weights + ((int64_t)stream * c.Hkv + h) * weights_stride + first;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -793,12 +812,13 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_kernel(Kv4View c, Kv4Rows 
         const Kv4Seq s = kv4_seq_of(b, c, i);
         if (s.state || first >= s.ctx) return;
         const int rows = s.n < b.max_rows ? s.n : b.max_rows, cols = rows * a.group;
-        if (a.scores && cols <= KV4_KEEP_COLUMNS) {
-            const float* sp = a.scores + (int64_t)(i * c.Hkv + h) * a.kept * a.width + first + lane;
-            for (int col = 0; w == 0 && col < cols; ++col) {
+        if (kv4_kept(cols, s.ctx)) {
+            const int64_t width = kv4_kept_width(s.ctx);
+            const float* sp = a.scores + ((int64_t)i * c.Hkv + h) * a.room + first + lane;
+            for (int col = w; col < cols; col += 4) {
                 const int j = a.row(col);
                 const f32x2 norm = a.norm[kv4_column(a, h, i, s) + col];
-                const float v = __builtin_amdgcn_exp2f(fmaf(sp[col * a.width], a.c, -norm[0]));
+                const float v = __builtin_amdgcn_exp2f(fmaf(sp[col * width], a.c, -norm[0]));
                 mine += first + lane < s.ctx - s.n + j + 1 ? v * norm[1] : 0.f;
             }
             return;
@@ -886,7 +906,7 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_kernel(Kv4View c, Kv4Rows 
 // Entry points
 // ------------------------------------------------------------------------------------------------------------------
 // the work buffer: chunk states | kept scores | m and 1 / l | queries
-struct Kv4Work { int64_t states, scores, norm, frags, width; int tiles, chunks, kept, slots; };
+struct Kv4Work { int64_t states, scores, norm, frags, room; int tiles, chunks, slots; };
 static Kv4Work plan_work(const t3_kv4_cache* c, const t3_kv4_batch* b, int H, bool weights) {
     Kv4Work w{};
     const int64_t cols = (int64_t)b->max_rows * (H / c->Hkv), few = cols < KV4_FEW_COLUMNS ? cols : KV4_FEW_COLUMNS;
@@ -895,12 +915,12 @@ static Kv4Work plan_work(const t3_kv4_cache* c, const t3_kv4_batch* b, int H, bo
     w.chunks = kv4_chunks((int)most);
     w.states = w.chunks > 1 ? pairs * w.tiles * w.chunks * (16 * (c->hd + 2)) * 4 : 0;
     if (weights) {
-        w.kept = (int)(few < KV4_KEEP_COLUMNS ? few : KV4_KEEP_COLUMNS);
-        w.width = (most + KV4_PAGE - 1) / KV4_PAGE * KV4_PAGE;
-        w.scores = pairs * w.kept * w.width * 4;
+        const int64_t every = few * kv4_kept_width(most);
+        w.room = every < KV4_KEEP ? every : KV4_KEEP;
+        w.scores = pairs * w.room * 4;
         w.slots = (int)((int64_t)b->rows * (H / c->Hkv) / 16) + b->n_seqs + 1;
         w.norm = (int64_t)c->Hkv * w.slots * 16 * 8;
-        w.frags = cols > KV4_KEEP_COLUMNS ? (int64_t)c->Hkv * w.slots * 16 * c->hd * 2 : 0;
+        w.frags = cols > few || every > KV4_KEEP ? (int64_t)c->Hkv * w.slots * 16 * c->hd * 2 : 0;
     }
     return w;
 }
@@ -932,8 +952,10 @@ static int launch_attn(const Kv4View& c, const Kv4Rows& b, const Kv4Attn& a, flo
         T3_LAUNCH((kv4_attn_join_kernel<HD, F16>), dim3((cols < KV4_FEW_COLUMNS ? (int)cols : KV4_FEW_COLUMNS) * c.Hkv, b.n_seqs), dim3(256), 0, st, c, b, a);
     if (weights) {
         const int64_t cap = (int64_t)c.max_pages * KV4_PAGE, most = b.max_ctx < cap ? b.max_ctx : cap;
-        if (cols <= KV4_KEEP_COLUMNS)
-            T3_LAUNCH(kv4_weights_kept_kernel, dim3((unsigned)((most + 1023) / 1024), c.Hkv, b.n_seqs), dim3(256), 0, st, c, b, a, weights, weights_stride);
+        if (!a.frags && cols <= 4)
+            T3_LAUNCH(kv4_weights_kept_kernel<1>, dim3((unsigned)((most + 1023) / 1024), c.Hkv, b.n_seqs), dim3(256), 0, st, c, b, a, weights, weights_stride);
+        else if (!a.frags)
+            T3_LAUNCH(kv4_weights_kept_kernel<4>, dim3((unsigned)((most + 255) / 256), c.Hkv, b.n_seqs), dim3(256), 0, st, c, b, a, weights, weights_stride);
         else
             T3_LAUNCH((kv4_weights_kernel<HD, F16>), dim3((unsigned)((most + KV4_PAGE - 1) / KV4_PAGE), c.Hkv, b.n_seqs), dim3(256), 0, st,
                   c, b, a, weights, weights_stride);
@@ -969,7 +991,7 @@ extern "C" int t3_op_attn_kv4(const t3_kv4_cache* cache, const t3_kv4_batch* bat
     a.c = scale * 1.44269504088896340736f;
     const Kv4Work w = plan_work(cache, batch, H, weights_dev != nullptr);
     uint8_t* work = static_cast<uint8_t*>(work_dev);
-    a.tiles = w.tiles; a.chunks = w.chunks; a.kept = w.kept; a.width = w.width;
+    a.tiles = w.tiles; a.chunks = w.chunks; a.room = w.room;
     a.states = reinterpret_cast<float*>(work);
     a.scores = w.scores ? reinterpret_cast<float*>(work + w.states) : nullptr;
     a.norm = weights_dev ? reinterpret_cast<f32x2*>(work + w.states + w.scores) : nullptr;
