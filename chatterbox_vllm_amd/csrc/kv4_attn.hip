@@ -23,7 +23,9 @@
 #define KV4_SLACK 8.f             // the reference moves when a maximum passes it by 2^8
 #define KV4_NONE -1e30f           // running maximum before the first visible token
 
-// A chunk is 16 pages: the four waves of its workgroup take four each.
+// A chunk is 16 pages: the four waves of its workgroup take four each.  (8 waves: 64 x 12 heads of 64 over 1.4k entries 13.2 -> 14.9 us,
+// 16 heads of 128 over up to 32k 77 -> 107; 32 pages: one sequence of 4k 13.5 -> 18.5, the long one 76.)
+#define KV4_FEW_WAVES 4
 #define KV4_CHUNK_PAGES 16
 KV4_FN int kv4_chunks(int ctx) { return (int)(((int64_t)ctx + KV4_CHUNK_PAGES * KV4_PAGE - 1) / (KV4_CHUNK_PAGES * KV4_PAGE)); }
 
@@ -62,22 +64,29 @@ __device__ __forceinline__ int64_t kv4_column(const Kv4Attn& a, int h, int seq, 
     return ((int64_t)h * a.slots + (s.start * a.group >> 4) + seq) * 16;
 }
 
+// Pages that one workgroup alone looks at are fetched past the caches (16 x 32 heads over up to 32k entries 88 -> 77 us); those that
+// several column tiles share are not (drafts of 40 columns 17.9 us, 18.7 so).
+template <bool ONCE, typename T> __device__ __forceinline__ T kv4_read_once(const T* p) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(p);
+    else return *p;
+}
+
 template <int HD> struct Kv4Page {
     u32x4 k[HD / 32], v[HD / 32], vs[HD / 64];
     unsigned ks;
     unsigned bad_k, good_v;                                       // all ones or all zeros, the same in every lane
-    __device__ __forceinline__ void load_k(const uint8_t* slab, int lane) {
+    template <bool ONCE> __device__ __forceinline__ void load_k(const uint8_t* slab, int lane) {
         const int g = lane >> 4, r = lane & 15;
 #pragma unroll
-        for (int x = 0; x < HD / 32; ++x) k[x] = *reinterpret_cast<const u32x4*>(slab + x * 1024 + lane * 16);
-        ks = *reinterpret_cast<const unsigned*>(slab + 64 * HD + g * (HD / 4) / KV4_BLOCK * KV4_PAGE + 4 * r);
+        for (int x = 0; x < HD / 32; ++x) k[x] = kv4_read_once<ONCE>(reinterpret_cast<const u32x4*>(slab + x * 1024 + lane * 16));
+        ks = kv4_read_once<ONCE>(reinterpret_cast<const unsigned*>(slab + 64 * HD + g * (HD / 4) / KV4_BLOCK * KV4_PAGE + 4 * r));
     }
-    __device__ __forceinline__ void load_v(const uint8_t* slab, int lane) {
+    template <bool ONCE> __device__ __forceinline__ void load_v(const uint8_t* slab, int lane) {
         const int g = lane >> 4, r = lane & 15;
 #pragma unroll
-        for (int x = 0; x < HD / 32; ++x) v[x] = *reinterpret_cast<const u32x4*>(slab + 32 * HD + x * 1024 + lane * 16);
+        for (int x = 0; x < HD / 32; ++x) v[x] = kv4_read_once<ONCE>(reinterpret_cast<const u32x4*>(slab + 32 * HD + x * 1024 + lane * 16));
 #pragma unroll
-        for (int x = 0; x < HD / 64; ++x) vs[x] = *reinterpret_cast<const u32x4*>(slab + 66 * HD + (2 * x + (r >> 3)) * KV4_PAGE + 16 * g);
+        for (int x = 0; x < HD / 64; ++x) vs[x] = kv4_read_once<ONCE>(reinterpret_cast<const u32x4*>(slab + 66 * HD + (2 * x + (r >> 3)) * KV4_PAGE + 16 * g));
     }
 };
 __device__ __forceinline__ unsigned kv4_byte(unsigned w, int i) { return w >> (8 * i) & 255u; }
@@ -299,13 +308,13 @@ template <bool F16> __device__ __forceinline__ unsigned kv4_pack2(float lo, floa
 template <int HD> __device__ __forceinline__ const uint8_t* kv4_slab_of(const Kv4View& c, int page, int h) {
     return c.pool + ((int64_t)(kv4_page_ok(page, c.n_pages) ? page : 0) * c.Hkv + h) * kv4_slab_bytes(HD);
 }
-template <int HD> __device__ __forceinline__ void kv4_fetch_k(Kv4Page<HD>& pg, const Kv4View& c, int page, int h, int lane) {
+template <int HD, bool ONCE> __device__ __forceinline__ void kv4_fetch_k(Kv4Page<HD>& pg, const Kv4View& c, int page, int h, int lane) {
     pg.bad_k = kv4_page_ok(page, c.n_pages) ? 0u : 0xffffffffu;
-    pg.load_k(kv4_slab_of<HD>(c, page, h), lane);
+    pg.template load_k<ONCE>(kv4_slab_of<HD>(c, page, h), lane);
 }
-template <int HD> __device__ __forceinline__ void kv4_fetch_v(Kv4Page<HD>& pg, const Kv4View& c, int page, int h, int lane) {
+template <int HD, bool ONCE> __device__ __forceinline__ void kv4_fetch_v(Kv4Page<HD>& pg, const Kv4View& c, int page, int h, int lane) {
     pg.good_v = kv4_page_ok(page, c.n_pages) ? 0xffffffffu : 0u;
-    pg.load_v(kv4_slab_of<HD>(c, page, h), lane);
+    pg.template load_v<ONCE>(kv4_slab_of<HD>(c, page, h), lane);
 }
 // bits of a NaN in both halves of a word, of either type
 #define KV4_NAN2 0x7fff7fffu
@@ -323,14 +332,14 @@ template <int HD> __device__ void kv4_fill_columns(const Kv4Attn& a, const Kv4Se
 // Few columns: one workgroup per (chunk, tile of 16 columns and key head, sequence).
 // ------------------------------------------------------------------------------------------------------------------
 template <int HD> struct Kv4FewLds {
-    float m[4][2][16];
-    __attribute__((aligned(16))) float o[4][16][HD + 4];
+    float m[KV4_FEW_WAVES][2][16];
+    __attribute__((aligned(16))) float o[KV4_FEW_WAVES][16][HD + 4];
 };
 
-template <int HD, bool F16>
+template <int HD, bool F16, bool ONCE>
 __device__ __forceinline__ void kv4_few_block(const Kv4View& c, const Kv4Rows& b, const Kv4Attn& a, Kv4FewLds<HD>& lds, int h, int tile, int seq, int chunk) {
-    float (&sm)[4][2][16] = lds.m;
-    float (&so)[4][16][HD + 4] = lds.o;
+    float (&sm)[KV4_FEW_WAVES][2][16] = lds.m;
+    float (&so)[KV4_FEW_WAVES][16][HD + 4] = lds.o;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Kv4Seq s = kv4_seq_of(b, c, seq);
     const int rows = s.n < b.max_rows ? s.n : b.max_rows;
@@ -338,7 +347,7 @@ __device__ __forceinline__ void kv4_few_block(const Kv4View& c, const Kv4Rows& b
     if (s.state == 1 || cols > KV4_FEW_COLUMNS || tile * 16 >= cols) return;
     const int c1 = cols < tile * 16 + 16 ? cols : tile * 16 + 16;
     if (s.state == 2) {
-        if (chunk == 0) kv4_fill_columns<HD>(a, s, h, tile * 16, c1, tid, 256);
+        if (chunk == 0) kv4_fill_columns<HD>(a, s, h, tile * 16, c1, tid, 64 * KV4_FEW_WAVES);
         return;
     }
     const int chunks = kv4_chunks(s.ctx);
@@ -365,13 +374,13 @@ __device__ __forceinline__ void kv4_few_block(const Kv4View& c, const Kv4Rows& b
     Kv4Page<HD> pg;
     if (w < np) {
         const int id = __builtin_amdgcn_readlane(ids, w);
-        kv4_fetch_k<HD>(pg, c, id, h, lane);
-        kv4_fetch_v<HD>(pg, c, id, h, lane);
+        kv4_fetch_k<HD, ONCE>(pg, c, id, h, lane);
+        kv4_fetch_v<HD, ONCE>(pg, c, id, h, lane);
     }
     // (the last page has a body of its own: a load under a condition would make every wait below one for all loads)
     const auto step = [&](int p, auto more) {
         const int first = (p0 + p) * KV4_PAGE, seen[1] = {sees - first};
-        const int next = more() ? __builtin_amdgcn_readlane(ids, p + 4) : 0;
+        const int next = more() ? __builtin_amdgcn_readlane(ids, p + KV4_FEW_WAVES) : 0;
         f32x4 sc[1][4];
         bf16x8 ph[1][2], pl[1][2];
         kv4_scores<HD, F16, 1>(pg, q, sc);
@@ -380,7 +389,7 @@ __device__ __forceinline__ void kv4_few_block(const Kv4View& c, const Kv4Rows& b
             for (int x = 0; x < 4; ++x)
                 *reinterpret_cast<f32x4*>(keep + first + 4 * x) = f32x4{sc[0][0][x], sc[0][1][x], sc[0][2][x], sc[0][3][x]};
         }
-        if constexpr (more()) kv4_fetch_k<HD>(pg, c, next, h, lane);
+        if constexpr (more()) kv4_fetch_k<HD, ONCE>(pg, c, next, h, lane);
         if (least < first + KV4_PAGE) {
             kv4_hide_scores<1>(sc, seen, lane);
             kv4_hide_values<HD>(pg, s.ctx - first, lane);
@@ -388,10 +397,10 @@ __device__ __forceinline__ void kv4_few_block(const Kv4View& c, const Kv4Rows& b
         kv4_reference<HD, 1>(sc, st, a.c);
         kv4_probabilities<HD, 1, true>(sc, st, a.c, ph, pl);
         kv4_values<HD, 1>(pg, ph, pl, st);
-        if constexpr (more()) kv4_fetch_v<HD>(pg, c, next, h, lane);
+        if constexpr (more()) kv4_fetch_v<HD, ONCE>(pg, c, next, h, lane);
     };
     int p = w;
-    for (; p + 4 < np; p += 4) step(p, std::true_type{});
+    for (; p + KV4_FEW_WAVES < np; p += KV4_FEW_WAVES) step(p, std::true_type{});
     if (p < np) step(p, std::false_type{});
     float l = st.l[0];
     l = kv4_group_sum(l);
@@ -405,18 +414,18 @@ __device__ __forceinline__ void kv4_few_block(const Kv4View& c, const Kv4Rows& b
             *reinterpret_cast<f32x4*>(&so[w][cc][64 * x + 16 * g + 4 * jj]) = v;
         }
     __syncthreads();
-    // the four waves in order; a thread 8 dims of a column
-    for (int i = tid; i < 16 * (HD / 8); i += 256) {
+    // the waves in order; a thread 8 dims of a column
+    for (int i = tid; i < 16 * (HD / 8); i += 64 * KV4_FEW_WAVES) {
         const int k = i / (HD / 8), d = i % (HD / 8) * 8, kcol = tile * 16 + k;
         if (kcol >= c1) continue;
         float M = sm[0][0][k];
 #pragma unroll
-        for (int x = 1; x < 4; ++x) M = fmaxf(M, sm[x][0][k]);
+        for (int x = 1; x < KV4_FEW_WAVES; ++x) M = fmaxf(M, sm[x][0][k]);
         float L = 0.f, o[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[e] = 0.f;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
+        for (int x = 0; x < KV4_FEW_WAVES; ++x) {
             const float f = __builtin_amdgcn_exp2f(sm[x][0][k] - M);
             L = fmaf(sm[x][1][k], f, L);
 #pragma unroll
@@ -439,10 +448,10 @@ __device__ __forceinline__ void kv4_few_block(const Kv4View& c, const Kv4Rows& b
     }
 }
 
-template <int HD, bool F16>
-__global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_few_kernel(Kv4View c, Kv4Rows b, Kv4Attn a) {
+template <int HD, bool F16, bool ONCE>
+__global__ __launch_bounds__(64 * KV4_FEW_WAVES, HD == 64 ? 4 : 2) void kv4_attn_few_kernel(Kv4View c, Kv4Rows b, Kv4Attn a) {
     __shared__ Kv4FewLds<HD> lds;
-    kv4_few_block<HD, F16>(c, b, a, lds, blockIdx.x % c.Hkv, blockIdx.x / c.Hkv, blockIdx.y, blockIdx.z);
+    kv4_few_block<HD, F16, ONCE>(c, b, a, lds, blockIdx.x % c.Hkv, blockIdx.x / c.Hkv, blockIdx.y, blockIdx.z);
 }
 
 // Joins the chunks of a column.  A thread has 4 dims; 1024 / HD groups of threads walk the chunks side by side, group x the chunks
@@ -732,7 +741,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_mixed_kernel(K
         x /= c.Hkv;
         const int tile = x % a.tiles;
         x /= a.tiles;
-        kv4_few_block<HD, F16>(c, b, a, lds.few, h, tile, x % b.n_seqs, x / b.n_seqs);
+        kv4_few_block<HD, F16, false>(c, b, a, lds.few, h, tile, x % b.n_seqs, x / b.n_seqs);
     }
 }
 
@@ -825,7 +834,7 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_kernel(Kv4View c, Kv4Rows 
         }
         if (!have) {
             Kv4Page<HD> pg;
-            kv4_fetch_k<HD>(pg, c, __builtin_amdgcn_readfirstlane(c.table[(int64_t)stream * c.max_pages + p]), h, lane);
+            kv4_fetch_k<HD, false>(pg, c, __builtin_amdgcn_readfirstlane(c.table[(int64_t)stream * c.max_pages + p]), h, lane);
             kv4_operands<HD>(pg, kf);
             have = true;
         }
@@ -942,7 +951,9 @@ static int launch_attn(const Kv4View& c, const Kv4Rows& b, const Kv4Attn& a, flo
     constexpr int NC = HD == 64 ? 1 : 2;
     const int64_t cols = (int64_t)b.max_rows * a.group;
     if (cols <= KV4_FEW_COLUMNS) {
-        T3_LAUNCH((kv4_attn_few_kernel<HD, F16>), dim3(a.tiles * c.Hkv, b.n_seqs, a.chunks), dim3(256), 0, st, c, b, a);
+        const dim3 grid(a.tiles * c.Hkv, b.n_seqs, a.chunks);
+        if (a.tiles == 1) T3_LAUNCH((kv4_attn_few_kernel<HD, F16, true>), grid, dim3(64 * KV4_FEW_WAVES), 0, st, c, b, a);
+        else T3_LAUNCH((kv4_attn_few_kernel<HD, F16, false>), grid, dim3(64 * KV4_FEW_WAVES), 0, st, c, b, a);
     } else {
         const int64_t turns = (cols + 64 * NC - 1) / (64 * NC), blocks = c.Hkv * (int64_t)b.n_seqs * (turns + (int64_t)a.tiles * a.chunks);
         T3_REQUIRE(blocks <= INT32_MAX, "attn_kv4: too many sequences of that many rows in one call");
