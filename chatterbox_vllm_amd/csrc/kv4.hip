@@ -37,49 +37,91 @@ __device__ __forceinline__ unsigned kv4_codes8(const float x[8], float scale) {
     return r;
 }
 
-template <int HD, bool F16>
-__global__ __launch_bounds__(256) void kv4_append_kernel(Kv4View c, Kv4Rows b, const uint16_t* __restrict__ k,
-                                                         const uint16_t* __restrict__ v, int64_t k_stride, int64_t v_stride) {
-    constexpr int T = HD / 8;                                    // threads of one (row, head)
-    const Kv4Seq s = kv4_seq_of(b, c, blockIdx.y);
-    if (s.state) return;
-    const int n = s.n < b.max_rows ? s.n : b.max_rows;
-    const int64_t items = (int64_t)n * c.Hkv * T, step = (int64_t)gridDim.x * 256;
-    // all lanes of a wave walk together: the butterflies below read every lane of a (row, head)
-    for (int64_t i0 = (int64_t)blockIdx.x * 256; i0 < items; i0 += step) {
-        const int64_t i = i0 + threadIdx.x;
-        const int ch = (int)(i % T) * 8, h = (int)(i / T % c.Hkv);
-        const int64_t j = i / ((int64_t)T * c.Hkv);
-        const int64_t slot = (int64_t)s.ctx - s.n + j;
-        bool put = i < items && slot >= 0;
-        int page = -1;
-        if (put) page = c.table[(int64_t)s.stream * c.max_pages + slot / KV4_PAGE];
-        put = put && kv4_page_ok(page, c.n_pages);
-        float kx[8], vx[8];
+// A wave takes the rows of one (page, key head).  Rows that fill the page build its slab in shared memory, which leaves in 16-byte
+// stores; others are stored from where they are, two bytes of V at a time, since their neighbours may be someone else's.
+struct Kv4Slice { int64_t first, slot; int lo, hi, page; };      // slot of row 0; of token 0; tokens [lo, hi) are rows; page id
+
+__device__ __forceinline__ int kv4_slices(int n) { return (int)(((int64_t)n + KV4_PAGE - 2) / KV4_PAGE) + 1; }
+__device__ __forceinline__ Kv4Slice kv4_slice(const Kv4View& c, const Kv4Seq& s, int n, int64_t x) {
+    Kv4Slice r;
+    r.first = (int64_t)s.ctx - s.n;
+    r.slot = ((r.first >> 6) + x) * KV4_PAGE;
+    const int64_t lo = r.first - r.slot, hi = r.first + n - r.slot;
+    r.lo = lo > 0 ? (int)lo : 0;
+    r.hi = hi < KV4_PAGE ? (int)hi : KV4_PAGE;                   // not above lo: no row of the sequence
+    r.page = r.slot >= 0 && r.lo < r.hi && s.state == 0 ? c.table[(int64_t)s.stream * c.max_pages + r.slot / KV4_PAGE] : -1;
+    return r;
+}
+
+template <int HD, bool F16> struct Kv4AppendItem {               // 8 dims of one row and head
+    float kx[8], vx[8];
+    __device__ __forceinline__ void load(const uint16_t* k, const uint16_t* v, bool in) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) { kx[e] = 0.f; vx[e] = 0.f; }
-        if (put) {
-            kv4_load8<F16>(k + (s.start + j) * k_stride + h * HD + ch, kx);
-            kv4_load8<F16>(v + (s.start + j) * v_stride + h * HD + ch, vx);
-        }
+        if (in) { kv4_load8<F16>(k, kx); kv4_load8<F16>(v, vx); }
+    }
+    // (all lanes of the row and head: the butterflies read every one)
+    template <typename P> __device__ __forceinline__ void store(P slab, int t, int ch, bool in) const {
         unsigned ka = kv4_absmax_bits(kx), va = kv4_absmax_bits(vx);
         ka = kv4_lane_max(kv4_lane_max(ka, 1), 2);               // of the block of 32
         va = kv4_lane_max(kv4_lane_max(va, 1), 2);
         unsigned any = ka > va ? ka : va;                        // of the entry
 #pragma unroll
-        for (int o = 4; o < T; o <<= 1) any = kv4_lane_max(any, o);
+        for (int o = 4; o < HD / 8; o <<= 1) any = kv4_lane_max(any, o);
         const bool bad = any >= 0x7f800000u;                     // a NaN or an infinity somewhere in the entry
-        if (!put) continue;
+        if (!in) return;
         const int kb = kv4_scale_byte(ka), vb = kv4_scale_byte(va);
         const unsigned kc = bad ? 0u : kv4_codes8(kx, kv4_scale(kb)), vc = bad ? 0u : kv4_codes8(vx, kv4_scale(vb));
-        uint8_t* slab = c.pool + ((int64_t)page * c.Hkv + h) * kv4_slab_bytes(HD);
-        const int t = (int)(slot % KV4_PAGE);
         *reinterpret_cast<unsigned*>(slab + kv4_k_at(HD, t, ch)) = kc;
         *reinterpret_cast<uint16_t*>(slab + kv4_v_at(HD, t, ch)) = (uint16_t)vc;
         *reinterpret_cast<uint16_t*>(slab + kv4_v_at(HD, t, ch + 4)) = (uint16_t)(vc >> 16);
         if (ch % KV4_BLOCK == 0) {
             slab[kv4_ks_at(HD, t, ch)] = (uint8_t)(bad ? KV4_NAN_SCALE : kb);
             slab[kv4_vs_at(HD, t, ch)] = (uint8_t)(bad ? KV4_MIN_SCALE : vb);
+        }
+    }
+};
+
+template <int HD, bool F16>
+__global__ __launch_bounds__(256) void kv4_append_kernel(Kv4View c, Kv4Rows b, const uint16_t* __restrict__ k,
+                                                         const uint16_t* __restrict__ v, int64_t k_stride, int64_t v_stride) {
+    constexpr int T = HD / 8, STEP = 64 / T, SLAB = KV4_PAGE * (HD + HD / 16);   // lanes and rows a step
+    __shared__ __attribute__((aligned(16))) uint8_t slabs[4][SLAB];
+    const Kv4Seq s = kv4_seq_of(b, c, blockIdx.y);
+    if (s.state) return;
+    const int n = s.n < b.max_rows ? s.n : b.max_rows, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ch = lane % T * 8, heads = (c.Hkv + 3) / 4;
+    const int x0 = blockIdx.x / heads, h = (blockIdx.x - x0 * heads) * 4 + w, slices = kv4_slices(n);
+    if (h >= c.Hkv) return;
+    for (int64_t x = x0; x < slices; x += gridDim.x / heads) {
+        const Kv4Slice r = kv4_slice(c, s, n, x);
+        if (!kv4_page_ok(r.page, c.n_pages)) continue;
+        const int64_t row = s.start + r.slot - r.first;          // of token 0
+        const uint16_t* kp = k + row * k_stride + h * HD + ch;
+        const uint16_t* vp = v + row * v_stride + h * HD + ch;
+        uint8_t* slab = c.pool + ((int64_t)r.page * c.Hkv + h) * SLAB;
+        if (r.lo == 0 && r.hi == KV4_PAGE) {
+#pragma unroll
+            for (int t0 = 0; t0 < KV4_PAGE; t0 += 4 * STEP) {
+                Kv4AppendItem<HD, F16> a[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int t = t0 + j * STEP + lane / T;
+                    a[j].load(kp + t * k_stride, vp + t * v_stride, true);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) a[j].store(slabs[w], t0 + j * STEP + lane / T, ch, true);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            for (int q = lane; q < SLAB / 16; q += 64) reinterpret_cast<u32x4*>(slab)[q] = reinterpret_cast<const u32x4*>(slabs[w])[q];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        } else {
+            for (int t0 = r.lo; t0 < r.hi; t0 += STEP) {
+                const int t = t0 + lane / T;
+                Kv4AppendItem<HD, F16> a;
+                a.load(kp + t * k_stride, vp + t * v_stride, t < r.hi);
+                a.store(slab, t, ch, t < r.hi);
+            }
         }
     }
 }
@@ -107,56 +149,262 @@ template <bool F16> __device__ __forceinline__ u32x4 kv4_values8(unsigned codes,
 template <int HD, bool F16>
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4View c, Kv4Rows b, int64_t layer_stride, uint16_t* __restrict__ k,
                                                        uint16_t* __restrict__ v) {
-    constexpr int T = HD / 8;
+    constexpr int T = HD / 8, STEP = 64 / T, SLAB = KV4_PAGE * (HD + HD / 16);
+    __shared__ __attribute__((aligned(16))) uint8_t slabs[4][SLAB];
     const Kv4Seq s = kv4_seq_of(b, c, blockIdx.y);
     if (s.state == 1) return;
     const uint8_t* pool = c.pool + (int64_t)blockIdx.z * layer_stride;
-    const int n = s.n < b.max_rows ? s.n : b.max_rows;
-    const int64_t items = (int64_t)n * c.Hkv * T, step = (int64_t)gridDim.x * 256;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += step) {
-        const int ch = (int)(i % T) * 8, h = (int)(i / T % c.Hkv);
-        const int64_t j = i / ((int64_t)T * c.Hkv), slot = (int64_t)s.ctx - s.n + j;
-        const int64_t at = (((int64_t)blockIdx.z * b.rows + s.start + j) * c.Hkv + h) * HD + ch;
-        const u32x4 zero = {0u, 0u, 0u, 0u};
-        u32x4 ko = zero, vo = zero;
-        bool nan = s.state == 2;
-        if (!nan && slot >= 0) {
-            const int page = c.table[(int64_t)s.stream * c.max_pages + slot / KV4_PAGE];
-            nan = !kv4_page_ok(page, c.n_pages);
-            const uint8_t* slab = pool + ((int64_t)(nan ? 0 : page) * c.Hkv + h) * kv4_slab_bytes(HD);
-            const int t = (int)(slot % KV4_PAGE);
-            const unsigned kc = *reinterpret_cast<const unsigned*>(slab + kv4_k_at(HD, t, ch));
-            const unsigned vc = *reinterpret_cast<const uint16_t*>(slab + kv4_v_at(HD, t, ch)) |
-                                (unsigned)*reinterpret_cast<const uint16_t*>(slab + kv4_v_at(HD, t, ch + 4)) << 16;
-            const unsigned kb = slab[kv4_ks_at(HD, t, ch)], vb = slab[kv4_vs_at(HD, t, ch)];
-            nan = nan || kb == KV4_NAN_SCALE;
-            ko = kv4_values8<F16>(kc, kb, nan);
-            vo = kv4_values8<F16>(vc, vb, nan);
-        } else if (nan) {
-            ko = kv4_values8<F16>(0u, 0u, true);
-            vo = ko;
+    const int n = s.n < b.max_rows ? s.n : b.max_rows, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ch = lane % T * 8, heads = (c.Hkv + 3) / 4;
+    const int x0 = blockIdx.x / heads, h = (blockIdx.x - x0 * heads) * 4 + w, slices = kv4_slices(n);
+    if (h >= c.Hkv) return;
+    for (int64_t x = x0; x < slices; x += gridDim.x / heads) {
+        const Kv4Slice r = kv4_slice(c, s, n, x);
+        const bool ok = kv4_page_ok(r.page, c.n_pages), none = s.state == 0 && r.slot < 0;   // none: entries before the first
+        if (ok) {
+            const uint8_t* slab = pool + ((int64_t)r.page * c.Hkv + h) * SLAB;
+            u32x4 in[(SLAB + 1023) / 1024];
+#pragma unroll
+            for (int q = 0; q < SLAB / 1024; ++q) in[q] = reinterpret_cast<const u32x4*>(slab)[q * 64 + lane];
+            if (lane < SLAB % 1024 / 16) in[SLAB / 1024] = reinterpret_cast<const u32x4*>(slab)[SLAB / 1024 * 64 + lane];
+#pragma unroll
+            for (int q = 0; q < SLAB / 1024; ++q) reinterpret_cast<u32x4*>(slabs[w])[q * 64 + lane] = in[q];
+            if (lane < SLAB % 1024 / 16) reinterpret_cast<u32x4*>(slabs[w])[SLAB / 1024 * 64 + lane] = in[SLAB / 1024];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
-        *reinterpret_cast<u32x4*>(k + at) = ko;
-        *reinterpret_cast<u32x4*>(v + at) = vo;
+        const int64_t at = (((int64_t)blockIdx.z * b.rows + s.start + r.slot - r.first) * c.Hkv + h) * HD + ch;
+        for (int t0 = r.lo; t0 < r.hi; t0 += STEP) {
+            const int t = t0 + lane / T;
+            if (t >= r.hi) continue;
+            u32x4 ko = {0u, 0u, 0u, 0u}, vo = ko;
+            if (ok) {
+                const uint8_t* slab = slabs[w];
+                const unsigned kc = *reinterpret_cast<const unsigned*>(slab + kv4_k_at(HD, t, ch));
+                const unsigned vc = *reinterpret_cast<const uint16_t*>(slab + kv4_v_at(HD, t, ch)) |
+                                    (unsigned)*reinterpret_cast<const uint16_t*>(slab + kv4_v_at(HD, t, ch + 4)) << 16;
+                const unsigned kb = slab[kv4_ks_at(HD, t, ch)], vb = slab[kv4_vs_at(HD, t, ch)];
+                ko = kv4_values8<F16>(kc, kb, kb == KV4_NAN_SCALE);
+                vo = kv4_values8<F16>(vc, vb, kb == KV4_NAN_SCALE);
+            } else if (!none) {
+                ko = kv4_values8<F16>(0u, 0u, true);
+                vo = ko;
+            }
+            *reinterpret_cast<u32x4*>(k + at + (int64_t)t * c.Hkv * HD) = ko;
+            *reinterpret_cast<u32x4*>(v + at + (int64_t)t * c.Hkv * HD) = vo;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Eviction, two launches.
-//
-// Choice: one workgroup per (entry, key head, layer).  Of the c entries, [0, sink) and [c - recent, c) stay; among the others
-// the `need` largest weights are found exactly by four rounds of an 8-bit radix histogram over order-preserving keys (ties go to
-// the lower index, so the result is a set that any correct sort would give), then the kept indices are written in order.
-// Move: one workgroup per (destination page, key head, entry and layer) gathers its 64 tokens' bytes.
+// Eviction.  Of an entry's ctx tokens [0, sink) and [ctx - recent, ctx) stay; of the others the `need` largest weights, ties to
+// the lower index, so that the set is what any correct sort would give.  Per (entry, key head, layer) on its own:
+//   T = the largest key with at least `need` candidate keys >= T, found from the highest bit in which they differ down;
+//   what is above T stays, and the first need - |above T| of those equal to it.
 // ------------------------------------------------------------------------------------------------------------------
-#define KV4_CHOOSE_THREADS 1024
-
 struct Kv4Evict {
     const int32_t* src; const int32_t* dst; const int32_t* ctx;
     float* weights; int64_t weights_stride;
     int32_t* new_ctx; int32_t* kept;
     int n, max_ctx, keep, sink, recent;
 };
+struct Kv4Entry { int src, dst, ctx; bool ok; };
+
+// the entry's numbers; not ok: they fit neither the cache nor the call
+__device__ __forceinline__ Kv4Entry kv4_entry(const Kv4View& c, const Kv4Evict& e, int i) {
+    Kv4Entry x{e.src[i], e.dst[i], e.ctx[i], true};
+    x.ok = x.src >= 0 && x.src < c.n_streams && x.dst >= 0 && x.dst < c.n_streams && x.src != x.dst && x.ctx >= 0 && x.ctx <= e.max_ctx &&
+           x.ctx <= (int64_t)c.max_pages * KV4_PAGE;
+    return x;
+}
+// this thread's share of what else refuses an entry: its destination taken by an entry before it or read by any, pages outside the
+// pool, pages that are both read and written
+template <int THREADS> __device__ __forceinline__ bool kv4_entry_bad(const Kv4View& c, const Kv4Evict& e, const Kv4Entry& x, int i, int left) {
+    const int tid = threadIdx.x;
+    bool bad = false;
+    for (int o = tid; o < e.n; o += THREADS) bad = bad || (o < i && e.dst[o] == x.dst) || e.src[o] == x.dst;
+    const int32_t* sp = c.table + (int64_t)x.src * c.max_pages;
+    const int32_t* dp = c.table + (int64_t)x.dst * c.max_pages;
+    const int ns = (x.ctx + KV4_PAGE - 1) / KV4_PAGE, nd = (left + KV4_PAGE - 1) / KV4_PAGE;
+    for (int o = tid >> 4; o < ns; o += THREADS >> 4) {
+        const int page = sp[o];
+        bad = bad || !kv4_page_ok(page, c.n_pages);
+        for (int d = tid & 15; d < nd; d += 16) bad = bad || dp[d] == page;
+    }
+    for (int d = tid; d < nd; d += THREADS) bad = bad || !kv4_page_ok(dp[d], c.n_pages);
+    return bad;
+}
+template <int THREADS> __device__ __forceinline__ void kv4_refuse(const Kv4Evict& e, int32_t* kept, int i, bool first) {
+    for (int j = threadIdx.x; j < e.keep; j += THREADS) kept[j] = -1;
+    if (first && threadIdx.x == 0) e.new_ctx[i] = -1;
+}
+// what is behind the kept ones
+template <int THREADS> __device__ __forceinline__ void kv4_clear_rest(const Kv4Evict& e, int32_t* kept, float* wd, int left) {
+    for (int j = left + threadIdx.x; j < e.keep; j += THREADS) kept[j] = -1;
+    for (int64_t j = left + threadIdx.x; j < e.weights_stride; j += THREADS) wd[j] = 0.f;
+}
+
+// One wave writes one page of the destination: token t becomes old[t] of the source for t < n, nothing behind.  page_of(old): the
+// source's page.  K moves in pieces of one token and lane group (hd / 8 bytes), V in two bytes from each of eight tokens, scales
+// bytewise; all of a lane's loads are in flight together.
+template <int HD, typename PageOf>
+__device__ __forceinline__ void kv4_move_page(uint8_t* pool, int Hkv, int h, const int* old, int n, int to_page, PageOf page_of) {
+    typedef typename std::conditional<HD == 64, u32x2, u32x4>::type piece_t;
+    const int t = threadIdx.x & 63;
+    const auto slab = [&](int page) { return pool + ((int64_t)page * Hkv + h) * kv4_slab_bytes(HD); };
+    uint8_t* to = slab(to_page);
+    const bool has = t < n;
+    const int mine = has ? old[t] : old[0];
+    const uint8_t* p = slab(page_of(mine));
+    const int at = mine % KV4_PAGE;
+    piece_t k[4];
+    uint8_t sc[HD / 16];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) k[g] = *reinterpret_cast<const piece_t*>(p + kv4_k_at(HD, at, g * (HD / 4)));
+#pragma unroll
+    for (int x = 0; x < HD / 16; ++x) sc[x] = p[64 * HD + x * KV4_PAGE + at];
+    const int t0 = t % 8 * 8;
+    u32x4 v[HD / 32];
+#pragma unroll
+    for (int x = 0; x < HD / 32; ++x) v[x] = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const bool some = t0 + j < n;
+        const int o = some ? old[t0 + j] : old[0];
+        const uint8_t* q = slab(page_of(o)) + kv4_v_at(HD, o % KV4_PAGE, t / 8 * 4);
+#pragma unroll
+        for (int x = 0; x < HD / 32; ++x) {                      // dims t / 8 * 4 + 32 x
+            const unsigned two = *reinterpret_cast<const uint16_t*>(q + (x / 2) * 2048 + (x & 1) * 128);
+            v[x][j / 2] |= (some ? two : 0u) << (16 * (j & 1));
+        }
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) *reinterpret_cast<piece_t*>(to + kv4_k_at(HD, t, g * (HD / 4))) = has ? k[g] : piece_t{};
+#pragma unroll
+    for (int x = 0; x < HD / 32; ++x) *reinterpret_cast<u32x4*>(to + kv4_v_at(HD, t0, t / 8 * 4) + (x / 2) * 2048 + (x & 1) * 128) = v[x];
+#pragma unroll
+    for (int x = 0; x < HD / 16; ++x) to[64 * HD + x * KV4_PAGE + t] = has ? sc[x] : (uint8_t)KV4_MIN_SCALE;
+}
+
+// Entries of at most THREADS * PER tokens, choice and move in one launch: a thread keeps PER weights in registers (wave w has tokens
+// 64 PER w on, lanes side by side), a step of the search is PER ballots and one exchange of the waves' counts.
+template <int HD, int THREADS, int PER>
+__global__ __launch_bounds__(THREADS) void kv4_evict_kernel(Kv4View c, Kv4Evict e, int64_t layer_stride) {
+    constexpr int WAVES = THREADS / 64, MOST = THREADS * PER;
+    __shared__ int list[MOST];
+    __shared__ int pages[2][MOST / KV4_PAGE];                    // source, destination
+    __shared__ unsigned lim[2][WAVES];
+    __shared__ __attribute__((aligned(16))) int cnt[2][WAVES];
+    __shared__ int ends[3][WAVES];
+    const int h = blockIdx.x, i = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int32_t* kept = e.kept + (((int64_t)layer * e.n + i) * c.Hkv + h) * e.keep;
+    const bool first = h == 0 && layer == 0;
+    const Kv4Entry x = kv4_entry(c, e, i);
+    if (!x.ok) { kv4_refuse<THREADS>(e, kept, i, first); return; }
+    const int ctx = x.ctx, left = ctx < e.keep ? ctx : e.keep;
+    const float* ws = e.weights + (((int64_t)layer * c.n_streams + x.src) * c.Hkv + h) * e.weights_stride;
+    float* wd = e.weights + (((int64_t)layer * c.n_streams + x.dst) * c.Hkv + h) * e.weights_stride;
+    const int base = w * 64 * PER + lane;
+    float wt[PER];
+#pragma unroll
+    for (int p = 0; p < PER; ++p) wt[p] = base + 64 * p < ctx ? ws[base + 64 * p] : 0.f;
+    for (int o = tid; o < (ctx + KV4_PAGE - 1) / KV4_PAGE; o += THREADS) pages[0][o] = c.table[(int64_t)x.src * c.max_pages + o];
+    for (int o = tid; o < (left + KV4_PAGE - 1) / KV4_PAGE; o += THREADS) pages[1][o] = c.table[(int64_t)x.dst * c.max_pages + o];
+    if (__syncthreads_or(kv4_entry_bad<THREADS>(c, e, x, i, left))) { kv4_refuse<THREADS>(e, kept, i, first); return; }
+
+    const bool all = ctx <= e.keep;
+    const int a = all ? ctx : e.sink, z = all ? ctx : ctx - e.recent, need = all ? 0 : e.keep - e.sink - e.recent;
+    unsigned key[PER], T = 0;                                    // 0: no candidate, or a NaN
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+        const int t = base + 64 * p;
+        key[p] = t >= a && t < z ? kv4_weight_key(__float_as_uint(wt[p])) : 0u;
+    }
+    if (need > 0) {                                              // 0 < need < z - a
+        unsigned lo = ~0u, hi = 0u;
+#pragma unroll
+        for (int p = 0; p < PER; ++p) {
+            const int t = base + 64 * p;
+            if (t >= a && t < z) { lo = lo < key[p] ? lo : key[p]; hi = hi > key[p] ? hi : key[p]; }
+        }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const unsigned l2 = (unsigned)__shfl_xor((int)lo, o), h2 = (unsigned)__shfl_xor((int)hi, o);
+            lo = lo < l2 ? lo : l2;
+            hi = hi > h2 ? hi : h2;
+        }
+        if (lane == 0) { lim[0][w] = lo; lim[1][w] = hi; }
+        __syncthreads();
+#pragma unroll
+        for (int o = 0; o < WAVES; ++o) { lo = lo < lim[0][o] ? lo : lim[0][o]; hi = hi > lim[1][o] ? hi : lim[1][o]; }
+        int bit = __builtin_amdgcn_readfirstlane(lo == hi ? -1 : 31 - __clz((int)(lo ^ hi)));
+        T = __builtin_amdgcn_readfirstlane(bit < 0 ? hi : bit == 31 ? 0u : hi >> (bit + 1) << (bit + 1));
+        for (; bit >= 0; --bit) {
+            const unsigned next = T | 1u << bit;
+            int n = 0;
+#pragma unroll
+            for (int p = 0; p < PER; ++p) n += __popcll(__ballot(key[p] >= next));
+            int* shared = cnt[bit & 1];                          // the other one is still being read
+            if (lane == 0) shared[w] = n;
+            __syncthreads();
+            n = 0;
+#pragma unroll
+            for (int o = 0; o < WAVES; ++o) n += shared[o];
+            n = __builtin_amdgcn_readfirstlane(n);
+            if (n >= need) T = next;
+            if (n == need) break;                                // exactly those
+        }
+    }
+    // places, in the order of the tokens: first the waves' counts, then each wave's own
+    int n_stay = 0, n_above = 0, n_tied = 0;
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+        const int t = base + 64 * p;
+        const bool in = t >= a && t < z && need > 0, sure = t < ctx && (t < a || t >= z);
+        n_above += __popcll(__ballot(in && key[p] > T));
+        n_tied += __popcll(__ballot(in && key[p] == T));
+        n_stay += __popcll(__ballot(sure));
+    }
+    if (lane == 0) { ends[0][w] = n_stay + n_above; ends[1][w] = n_above; ends[2][w] = n_tied; }
+    __syncthreads();
+    int room = need, out = 0;                                    // tied ones that stay; kept before this wave
+#pragma unroll
+    for (int o = 0; o < WAVES; ++o) room -= ends[1][o];
+    for (int o = 0; o < w; ++o) {
+        const int n = ends[2][o] < room ? ends[2][o] : room;
+        out += ends[0][o] + n;
+        room -= n;
+    }
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+        const int t = base + 64 * p;
+        const bool in = t >= a && t < z && need > 0, sure = t < ctx && (t < a || t >= z);
+        const bool tie = in && key[p] == T;
+        const uint64_t ties = __ballot(tie);
+        const int rank = __builtin_amdgcn_mbcnt_hi((unsigned)(ties >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)ties, 0));
+        const bool stay = sure || (in && key[p] > T) || (tie && rank < room);
+        const uint64_t stays = __ballot(stay);
+        const int at = out + __builtin_amdgcn_mbcnt_hi((unsigned)(stays >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)stays, 0));
+        if (stay) { kept[at] = t; wd[at] = wt[p]; list[at] = t; }
+        out += __popcll(stays);
+        const int n = __popcll(ties);
+        room -= n < room ? n : room;
+    }
+    kv4_clear_rest<THREADS>(e, kept, wd, left);
+    if (first && tid == 0) e.new_ctx[i] = left;
+    __syncthreads();
+    uint8_t* pool = c.pool + (int64_t)layer * layer_stride;
+    for (int pg = w; pg * KV4_PAGE < left; pg += WAVES) {
+        const int n = left - pg * KV4_PAGE;
+        kv4_move_page<HD>(pool, c.Hkv, h, list + pg * KV4_PAGE, n < KV4_PAGE ? n : KV4_PAGE, pages[1][pg],
+                          [&](int old) { return pages[0][old / KV4_PAGE]; });
+    }
+}
+
+// Longer entries: the weights are read again for each of four rounds of an 8-bit radix histogram and once for the places; the pages
+// are moved by a launch of their own, which has workgroups for all of them.
+#define KV4_CHOOSE_THREADS 1024
 
 // sum over the workgroup's threads before this one; total in *all
 __device__ __forceinline__ int kv4_prefix(int v, int* wave_sums, int* all) {
@@ -178,32 +426,14 @@ __global__ __launch_bounds__(KV4_CHOOSE_THREADS) void kv4_choose_kernel(Kv4View 
     __shared__ int wave_sums[KV4_CHOOSE_THREADS / 64];
     __shared__ int pick[2];
     const int h = blockIdx.x, i = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x;
-    const int src = e.src[i], dst = e.dst[i], ctx = e.ctx[i];
     int32_t* kept = e.kept + (((int64_t)layer * e.n + i) * c.Hkv + h) * e.keep;
-
-    // what refuses the entry; every workgroup of the entry comes to the same answer
-    bool bad = src < 0 || src >= c.n_streams || dst < 0 || dst >= c.n_streams || src == dst || ctx < 0 || ctx > e.max_ctx ||
-               ctx > (int64_t)c.max_pages * KV4_PAGE;
-    const int left = ctx < e.keep ? ctx : e.keep;
-    for (int o = tid; o < e.n; o += KV4_CHOOSE_THREADS) bad = bad || (o < i && e.dst[o] == dst) || e.src[o] == dst;
-    if (!bad) {
-        const int32_t* sp = c.table + (int64_t)src * c.max_pages;
-        const int32_t* dp = c.table + (int64_t)dst * c.max_pages;
-        const int ns = (ctx + KV4_PAGE - 1) / KV4_PAGE, nd = (left + KV4_PAGE - 1) / KV4_PAGE;
-        for (int o = tid; o < ns; o += KV4_CHOOSE_THREADS) {
-            const int page = sp[o];
-            bad = bad || !kv4_page_ok(page, c.n_pages);
-            for (int d = 0; d < nd; ++d) bad = bad || dp[d] == page;
-        }
-        for (int d = tid; d < nd; d += KV4_CHOOSE_THREADS) bad = bad || !kv4_page_ok(dp[d], c.n_pages);
-    }
-    if (__syncthreads_or(bad)) {
-        for (int j = tid; j < e.keep; j += KV4_CHOOSE_THREADS) kept[j] = -1;
-        if (h == 0 && layer == 0 && tid == 0) e.new_ctx[i] = -1;
-        return;
-    }
-    const float* w = e.weights + (((int64_t)layer * c.n_streams + src) * c.Hkv + h) * e.weights_stride;
-    float* wd = e.weights + (((int64_t)layer * c.n_streams + dst) * c.Hkv + h) * e.weights_stride;
+    const bool first = h == 0 && layer == 0;
+    const Kv4Entry x = kv4_entry(c, e, i);
+    if (!x.ok) { kv4_refuse<KV4_CHOOSE_THREADS>(e, kept, i, first); return; }
+    const int ctx = x.ctx, left = ctx < e.keep ? ctx : e.keep;
+    if (__syncthreads_or(kv4_entry_bad<KV4_CHOOSE_THREADS>(c, e, x, i, left))) { kv4_refuse<KV4_CHOOSE_THREADS>(e, kept, i, first); return; }
+    const float* w = e.weights + (((int64_t)layer * c.n_streams + x.src) * c.Hkv + h) * e.weights_stride;
+    float* wd = e.weights + (((int64_t)layer * c.n_streams + x.dst) * c.Hkv + h) * e.weights_stride;
 
     unsigned least = 0;                                          // the smallest key that stays
     int ties = 0;                                                // how many of that key stay
@@ -247,55 +477,23 @@ __global__ __launch_bounds__(KV4_CHOOSE_THREADS) void kv4_choose_kernel(Kv4View 
         tied += n_tied;
         out += n_out;
     }
-    for (int j = left + tid; j < e.keep; j += KV4_CHOOSE_THREADS) kept[j] = -1;
-    for (int64_t j = left + tid; j < e.weights_stride; j += KV4_CHOOSE_THREADS) wd[j] = 0.f;
-    if (h == 0 && layer == 0 && tid == 0) e.new_ctx[i] = left;
+    kv4_clear_rest<KV4_CHOOSE_THREADS>(e, kept, wd, left);
+    if (first && tid == 0) e.new_ctx[i] = left;
 }
 
 template <int HD>
 __global__ __launch_bounds__(256) void kv4_move_kernel(Kv4View c, Kv4Evict e, int64_t layer_stride) {
-    __shared__ const uint8_t* from[KV4_PAGE];                    // slab of the old entry that becomes token t, null: none
-    __shared__ uint8_t old_t[KV4_PAGE];
-    const int h = blockIdx.y % c.Hkv, i = blockIdx.y / c.Hkv, layer = blockIdx.z, tid = threadIdx.x;
-    const int left = e.new_ctx[i], j0 = blockIdx.x * KV4_PAGE;
-    if (j0 >= left) return;                                      // covers a refused entry (-1)
-    uint8_t* pool = c.pool + (int64_t)layer * layer_stride;
-    const int32_t* kept = e.kept + (((int64_t)layer * e.n + i) * c.Hkv + h) * e.keep;
-    constexpr int slab_bytes = KV4_PAGE * (HD + HD / 16);
-    if (tid < KV4_PAGE) {
-        const int old = j0 + tid < left ? kept[j0 + tid] : -1;
-        from[tid] = old < 0 ? nullptr
-                            : pool + ((int64_t)c.table[(int64_t)e.src[i] * c.max_pages + old / KV4_PAGE] * c.Hkv + h) * slab_bytes;
-        old_t[tid] = (uint8_t)(old < 0 ? 0 : old % KV4_PAGE);
-    }
+    __shared__ int lists[4][KV4_PAGE];
+    const int h = blockIdx.y % c.Hkv, i = blockIdx.y / c.Hkv, layer = blockIdx.z, lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pg = blockIdx.x * 4 + w;
+    const int n = e.new_ctx[i] - pg * KV4_PAGE;                  // not positive for a refused entry (-1)
+    const int32_t* kept = e.kept + (((int64_t)layer * e.n + i) * c.Hkv + h) * e.keep + pg * KV4_PAGE;
+    if (lane < n) lists[w][lane] = kept[lane];
     __syncthreads();
-    uint8_t* to = pool + ((int64_t)c.table[(int64_t)e.dst[i] * c.max_pages + blockIdx.x] * c.Hkv + h) * slab_bytes;
-    // K: pieces of one token and lane group, hd / 8 bytes
-    typedef typename std::conditional<HD == 64, u32x2, u32x4>::type piece_t;
-    {
-        const int t = tid & 63, d = (tid >> 6) * (HD / 4);
-        const uint8_t* p = from[t];
-        piece_t x = {};
-        if (p) x = *reinterpret_cast<const piece_t*>(p + kv4_k_at(HD, old_t[t], d));
-        *reinterpret_cast<piece_t*>(to + kv4_k_at(HD, t, d)) = x;
-    }
-    // V: four dims of eight tokens, 16 bytes; two bytes from each
-    for (int q = tid; q < 2 * HD; q += 256) {
-        const int t0 = q % 8 * 8, d = q / 8 * 4;
-        u32x4 x = {0u, 0u, 0u, 0u};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint8_t* p = from[t0 + j];
-            if (p) x[j / 2] |= (unsigned)*reinterpret_cast<const uint16_t*>(p + kv4_v_at(HD, old_t[t0 + j], d)) << (16 * (j & 1));
-        }
-        *reinterpret_cast<u32x4*>(to + kv4_v_at(HD, t0, d)) = x;
-    }
-    // scales: K's blocks, then V's, which follow them
-    for (int q = tid; q < 4 * HD; q += 256) {
-        const int t = q % KV4_PAGE, d = q / KV4_PAGE * KV4_BLOCK;
-        const uint8_t* p = from[t];
-        to[kv4_ks_at(HD, t, d)] = p ? p[kv4_ks_at(HD, old_t[t], d)] : (uint8_t)KV4_MIN_SCALE;
-    }
+    if (n <= 0) return;
+    const int32_t* sp = c.table + (int64_t)e.src[i] * c.max_pages;
+    kv4_move_page<HD>(c.pool + (int64_t)layer * layer_stride, c.Hkv, h, lists[w], n < KV4_PAGE ? n : KV4_PAGE,
+                      c.table[(int64_t)e.dst[i] * c.max_pages + pg], [&](int old) { return sp[old / KV4_PAGE]; });
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -332,10 +530,10 @@ extern "C" int64_t t3_op_kv4_page_bytes(int32_t Hkv, int32_t hd) {
     return (hd == 64 || hd == 128) && Hkv >= 1 && Hkv <= 1024 ? (int64_t)Hkv * kv4_slab_bytes(hd) : 0;
 }
 
-// workgroups along the rows of a sequence: one per 256 threads' work, capped (the kernels stride over the rest)
-static int row_groups(const t3_kv4_cache* c, const t3_kv4_batch* b) {
-    const int64_t g = ((int64_t)b->max_rows * c->Hkv * (c->hd / 8) + 255) / 256;
-    return (int)(g < 4096 ? g : 4096);
+// workgroups along the pages of a sequence, four key heads each; capped (the kernels stride over the rest)
+static int page_groups(const t3_kv4_cache* c, const t3_kv4_batch* b) {
+    const int64_t heads = (c->Hkv + 3) / 4, slices = ((int64_t)b->max_rows + KV4_PAGE - 2) / KV4_PAGE + 1;
+    return (int)(heads * (slices < 16384 ? slices : 16384));
 }
 
 extern "C" int t3_op_kv4_append(const t3_kv4_cache* cache, const t3_kv4_batch* batch, const void* k_dev, const void* v_dev,
@@ -348,7 +546,7 @@ extern "C" int t3_op_kv4_append(const t3_kv4_cache* cache, const t3_kv4_batch* b
     T3_REQUIRE(k_stride >= width && v_stride >= width && k_stride % 8 == 0 && v_stride % 8 == 0 &&
                reinterpret_cast<uintptr_t>(k_dev) % 16 == 0 && reinterpret_cast<uintptr_t>(v_dev) % 16 == 0,
                "kv4_append: rows must be 16-byte aligned and must not overlap");
-    const dim3 grid(row_groups(cache, batch), batch->n_seqs);
+    const dim3 grid(page_groups(cache, batch), batch->n_seqs);
     const Kv4View c = kv4_view(cache, layer);
     const Kv4Rows b = kv4_rows(batch);
     const uint16_t* k = static_cast<const uint16_t*>(k_dev);
@@ -368,7 +566,7 @@ extern "C" int t3_op_kv4_read(const t3_kv4_cache* cache, const t3_kv4_batch* bat
     T3_REQUIRE(k_dev && v_dev, "kv4_read: null argument");
     T3_REQUIRE(dtype == 0 || dtype == 1, "kv4_read: dtype must be 0 (bf16) or 1 (fp16)");
     T3_REQUIRE(reinterpret_cast<uintptr_t>(k_dev) % 16 == 0 && reinterpret_cast<uintptr_t>(v_dev) % 16 == 0, "kv4_read: rows must be 16-byte aligned");
-    const dim3 grid(row_groups(cache, batch), batch->n_seqs, n_layers);
+    const dim3 grid(page_groups(cache, batch), batch->n_seqs, n_layers);
     const Kv4View c = kv4_view(cache, layer);
     const Kv4Rows b = kv4_rows(batch);
     uint16_t* k = static_cast<uint16_t*>(k_dev);
@@ -380,6 +578,15 @@ extern "C" int t3_op_kv4_read(const t3_kv4_cache* cache, const t3_kv4_batch* bat
     else T3_LAUNCH((kv4_read_kernel<128, true>), grid, dim3(256), 0, st, c, b, ls, k, v);
     T3_HIP_CHECK(hipGetLastError());
     return 0;
+}
+
+#ifndef KV4_HELD_MOST
+#define KV4_HELD_MOST 8192
+#endif
+template <int HD> static void kv4_evict_held(const Kv4View& c, const Kv4Evict& e, int layers, int64_t layer_stride, hipStream_t st) {
+    const dim3 grid(c.Hkv, e.n, layers);
+    if (e.max_ctx <= 2048) T3_LAUNCH((kv4_evict_kernel<HD, 256, 8>), grid, dim3(256), 0, st, c, e, layer_stride);
+    else T3_LAUNCH((kv4_evict_kernel<HD, 1024, 8>), grid, dim3(1024), 0, st, c, e, layer_stride);
 }
 
 extern "C" int t3_op_kv4_evict(const t3_kv4_cache* cache, const t3_kv4_evict_desc* d, void* stream) {
@@ -394,11 +601,16 @@ extern "C" int t3_op_kv4_evict(const t3_kv4_cache* cache, const t3_kv4_evict_des
     const Kv4View c = kv4_view(cache, d->layer);
     const Kv4Evict e{d->src_dev, d->dst_dev, d->ctx_dev, d->weights_dev, d->weights_stride, d->new_ctx_dev, d->kept_dev,
                      d->n, d->max_ctx, d->keep, d->sink, d->recent};
-    T3_LAUNCH(kv4_choose_kernel, dim3(cache->Hkv, d->n, d->n_layers), dim3(KV4_CHOOSE_THREADS), 0, st, c, e);
-    const int most = d->keep < d->max_ctx ? d->keep : d->max_ctx;
-    const dim3 grid((most + KV4_PAGE - 1) / KV4_PAGE, cache->Hkv * d->n, d->n_layers);
-    if (cache->hd == 64) T3_LAUNCH(kv4_move_kernel<64>, grid, dim3(256), 0, st, c, e, cache->layer_stride);
-    else T3_LAUNCH(kv4_move_kernel<128>, grid, dim3(256), 0, st, c, e, cache->layer_stride);
+    if (d->max_ctx <= KV4_HELD_MOST) {
+        if (cache->hd == 64) kv4_evict_held<64>(c, e, d->n_layers, cache->layer_stride, st);
+        else kv4_evict_held<128>(c, e, d->n_layers, cache->layer_stride, st);
+    } else {
+        T3_LAUNCH(kv4_choose_kernel, dim3(cache->Hkv, d->n, d->n_layers), dim3(KV4_CHOOSE_THREADS), 0, st, c, e);
+        const int most = d->keep < d->max_ctx ? d->keep : d->max_ctx;
+        const dim3 grid((most + 4 * KV4_PAGE - 1) / (4 * KV4_PAGE), cache->Hkv * d->n, d->n_layers);
+        if (cache->hd == 64) T3_LAUNCH(kv4_move_kernel<64>, grid, dim3(256), 0, st, c, e, cache->layer_stride);
+        else T3_LAUNCH(kv4_move_kernel<128>, grid, dim3(256), 0, st, c, e, cache->layer_stride);
+    }
     T3_HIP_CHECK(hipGetLastError());
     return 0;
 }

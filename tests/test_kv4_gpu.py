@@ -397,6 +397,41 @@ def test_evict_long_and_nan_entries():
     assert torch.isnan(cache.read(cache.batch(i32([0, 5]), i32([1]), i32([5]), rows=5))[0][3, 1]).all()
 
 
+@pytest.mark.parametrize("pages,ctx", [(32, [2048, 2047, 1025, 64, 513, 1, 0]), (33, [2049, 2048, 300]), (128, [8192, 8191, 4097, 640]), (129, [8193, 130])])
+@pytest.mark.parametrize("keep,sink,recent", [(500, 34, 100), (1, 0, 0), (1500, 0, 0), (1024, 1000, 24)])
+def test_evict_at_every_length(pages, ctx, keep, sink, recent):
+    """The choice for entries up to and past each number that the threads of a workgroup hold: weights that differ everywhere, in one
+    bit alone, not at all, in sign and exponent, infinite ones, NaN, and ties that reach over all waves."""
+    n, kv = len(ctx), 8
+    m = _kv4.Model(64, kv, 1, 2 * n * pages, 2 * n, pages, seed=20)
+    m.pool.random_(0, 200, generator=torch.Generator().manual_seed(21))
+    g = torch.Generator().manual_seed(22)
+    width = pages * 64
+    w = torch.rand(1, 2 * n, kv, width, generator=g)
+    w[:, :, 1] = (w[:, :, 1] * 3).floor()
+    w[:, :, 2] = 0.75
+    w[:, :, 3] = torch.where(w[:, :, 3] < 0.5, torch.tensor(1.0), torch.tensor(1.0 + 2.0 ** -23))
+    w[:, :, 4] = torch.exp((w[:, :, 4] - 0.5) * 160) * torch.where(torch.rand(2 * n, width, generator=g) < 0.3, -1.0, 1.0)
+    w[:, :, 5, ::7], w[:, :, 5, 1::5], w[:, :, 5, 2::11] = math.inf, math.nan, -3e38
+    w[:, :, 6] = math.nan
+    w[:, :, 7] = torch.arange(width) / 7.0
+    cache = device_cache(m)
+    dw = w.to(DEV)
+    new, kept = cache.evict(i32(list(range(n))), i32([n + i for i in range(n)]), i32(ctx), keep, sink, recent, dw)
+    left = [min(t, keep) for t in ctx]
+    assert new.tolist() == left
+    after = dw.cpu()
+    stays = {(i, h): _kv4.choose(w[0, i, h].tolist(), ctx[i], keep, sink, recent) for i in range(n) for h in range(kv)}
+    for (i, h), stay in stays.items():
+        assert kept[0, i, h].tolist() == stay + [-1] * (keep - left[i])
+        assert torch.equal(torch.nan_to_num(after[0, n + i, h], 9.5), torch.nan_to_num(torch.cat([w[0, i, h][stay], torch.zeros(width - left[i])]), 9.5))
+    old_k, old_v = cache.read(cache.batch(i32([sum(ctx[:i]) for i in range(n + 1)]), i32(list(range(n))), i32(ctx), rows=sum(ctx)))
+    new_k, new_v = cache.read(cache.batch(i32([sum(left[:i]) for i in range(n + 1)]), i32([n + i for i in range(n)]), i32(left), rows=sum(left)))
+    for (i, h), stay in stays.items():
+        for a, b in ((old_k, new_k), (old_v, new_v)):
+            assert torch.equal(a[sum(ctx[:i]):][stay, h], b[sum(left[:i]):sum(left[:i + 1]), h])
+
+
 def test_evict_refuses_entry_by_entry():
     m = _kv4.Model(64, 2, 1, 40, 12, 3, seed=17)
     for i in range(12):
