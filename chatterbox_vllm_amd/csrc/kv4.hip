@@ -217,21 +217,22 @@ __device__ __forceinline__ Kv4Entry kv4_entry(const Kv4View& c, const Kv4Evict& 
            x.ctx <= (int64_t)c.max_pages * KV4_PAGE;
     return x;
 }
-// this thread's share of what else refuses an entry: its destination taken by an entry before it or read by any, pages outside the
-// pool, pages that are both read and written
-template <int THREADS> __device__ __forceinline__ bool kv4_entry_bad(const Kv4View& c, const Kv4Evict& e, const Kv4Entry& x, int i, int left) {
+// this thread's share of what else refuses an entry: its destination taken by an entry before it or read by any; pages (sp: of its
+// source, dp: of its destination) outside the pool, or both read and written
+template <int THREADS> __device__ __forceinline__ bool kv4_entry_taken(const Kv4Evict& e, const Kv4Entry& x, int i) {
+    bool bad = false;
+    for (int o = threadIdx.x; o < e.n; o += THREADS) bad = bad || (o < i && e.dst[o] == x.dst) || e.src[o] == x.dst;
+    return bad;
+}
+template <int THREADS> __device__ __forceinline__ bool kv4_pages_bad(const int32_t* sp, const int32_t* dp, int ns, int nd, int n_pages) {
     const int tid = threadIdx.x;
     bool bad = false;
-    for (int o = tid; o < e.n; o += THREADS) bad = bad || (o < i && e.dst[o] == x.dst) || e.src[o] == x.dst;
-    const int32_t* sp = c.table + (int64_t)x.src * c.max_pages;
-    const int32_t* dp = c.table + (int64_t)x.dst * c.max_pages;
-    const int ns = (x.ctx + KV4_PAGE - 1) / KV4_PAGE, nd = (left + KV4_PAGE - 1) / KV4_PAGE;
     for (int o = tid >> 4; o < ns; o += THREADS >> 4) {
         const int page = sp[o];
-        bad = bad || !kv4_page_ok(page, c.n_pages);
+        bad = bad || !kv4_page_ok(page, n_pages);
         for (int d = tid & 15; d < nd; d += 16) bad = bad || dp[d] == page;
     }
-    for (int d = tid; d < nd; d += THREADS) bad = bad || !kv4_page_ok(dp[d], c.n_pages);
+    for (int d = tid; d < nd; d += THREADS) bad = bad || !kv4_page_ok(dp[d], n_pages);
     return bad;
 }
 template <int THREADS> __device__ __forceinline__ void kv4_refuse(const Kv4Evict& e, int32_t* kept, int i, bool first) {
@@ -245,161 +246,203 @@ template <int THREADS> __device__ __forceinline__ void kv4_clear_rest(const Kv4E
 }
 
 // One wave writes one page of the destination: token t becomes old[t] of the source for t < n, nothing behind.  page_of(old): the
-// source's page.  K moves in pieces of one token and lane group (hd / 8 bytes), V in two bytes from each of eight tokens, scales
-// bytewise; all of a lane's loads are in flight together.
-template <int HD, typename PageOf>
-__device__ __forceinline__ void kv4_move_page(uint8_t* pool, int Hkv, int h, const int* old, int n, int to_page, PageOf page_of) {
+// source's page.  K moves in pieces of one token and lane group (hd / 8 bytes), V in two bytes from each of eight tokens, whose
+// addresses the lanes leave each other in `where`, scales bytewise; all of a lane's loads are in flight together.
+template <int HD, typename Index, typename PageOf>
+__device__ __forceinline__ void kv4_move_page(uint8_t* pool, int Hkv, int h, const Index* old, int n, int to_page, const uint8_t** where,
+                                              PageOf page_of) {
     typedef typename std::conditional<HD == 64, u32x2, u32x4>::type piece_t;
-    const int t = threadIdx.x & 63;
+    const int t = threadIdx.x & 63, t0 = t % 8 * 8, d = t / 8 * 4;
     const auto slab = [&](int page) { return pool + ((int64_t)page * Hkv + h) * kv4_slab_bytes(HD); };
     uint8_t* to = slab(to_page);
     const bool has = t < n;
-    const int mine = has ? old[t] : old[0];
+    const int mine = old[has ? t : 0], at = mine % KV4_PAGE;
     const uint8_t* p = slab(page_of(mine));
-    const int at = mine % KV4_PAGE;
+    where[t] = p + kv4_v_at(HD, at, 0);
     piece_t k[4];
     uint8_t sc[HD / 16];
 #pragma unroll
     for (int g = 0; g < 4; ++g) k[g] = *reinterpret_cast<const piece_t*>(p + kv4_k_at(HD, at, g * (HD / 4)));
 #pragma unroll
     for (int x = 0; x < HD / 16; ++x) sc[x] = p[64 * HD + x * KV4_PAGE + at];
-    const int t0 = t % 8 * 8;
-    u32x4 v[HD / 32];
-#pragma unroll
-    for (int x = 0; x < HD / 32; ++x) v[x] = u32x4{0u, 0u, 0u, 0u};
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    uint16_t two[8][HD / 32];                                    // dims d + 32 x of token t0 + j
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const bool some = t0 + j < n;
-        const int o = some ? old[t0 + j] : old[0];
-        const uint8_t* q = slab(page_of(o)) + kv4_v_at(HD, o % KV4_PAGE, t / 8 * 4);
+        const uint8_t* q = where[t0 + j] + d * 4;
 #pragma unroll
-        for (int x = 0; x < HD / 32; ++x) {                      // dims t / 8 * 4 + 32 x
-            const unsigned two = *reinterpret_cast<const uint16_t*>(q + (x / 2) * 2048 + (x & 1) * 128);
-            v[x][j / 2] |= (some ? two : 0u) << (16 * (j & 1));
-        }
+        for (int x = 0; x < HD / 32; ++x) two[j][x] = *reinterpret_cast<const uint16_t*>(q + (x / 2) * 2048 + (x & 1) * 128);
     }
 #pragma unroll
     for (int g = 0; g < 4; ++g) *reinterpret_cast<piece_t*>(to + kv4_k_at(HD, t, g * (HD / 4))) = has ? k[g] : piece_t{};
 #pragma unroll
-    for (int x = 0; x < HD / 32; ++x) *reinterpret_cast<u32x4*>(to + kv4_v_at(HD, t0, t / 8 * 4) + (x / 2) * 2048 + (x & 1) * 128) = v[x];
-#pragma unroll
     for (int x = 0; x < HD / 16; ++x) to[64 * HD + x * KV4_PAGE + t] = has ? sc[x] : (uint8_t)KV4_MIN_SCALE;
+    const int some = n - t0;
+#pragma unroll
+    for (int x = 0; x < HD / 32; ++x) {
+        u32x4 v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const unsigned both = two[2 * j][x] | (unsigned)two[2 * j + 1][x] << 16;
+            v[j] = 2 * j + 1 < some ? both : 2 * j < some ? both & 0xffffu : 0u;
+        }
+        *reinterpret_cast<u32x4*>(to + kv4_v_at(HD, t0, d) + (x / 2) * 2048 + (x & 1) * 128) = v;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
-// Entries of at most THREADS * PER tokens, choice and move in one launch: a thread keeps PER weights in registers (wave w has tokens
-// 64 PER w on, lanes side by side), a step of the search is PER ballots and one exchange of the waves' counts.
+// sum over the lanes before and including this one
+__device__ __forceinline__ int kv4_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);          // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);          // lane 15 of rows 0 and 2, then lane 31, to what follows
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+    return x;
+}
+__device__ __forceinline__ unsigned kv4_or_scan(unsigned x) {
+    x |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false);
+    x |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false);
+    x |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false);
+    x |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false);
+    x |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false);
+    x |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false);
+    return x;
+}
+// a barrier for shared memory alone: stores to global memory stay in flight
+__device__ __forceinline__ void kv4_lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// Entries of at most THREADS * PER tokens, choice and move in one launch.  The weights go through shared memory to threads that have
+// PER neighbouring ones.  The bits that all candidates share are skipped; a histogram of the next 8 gives the bin of T, and so on
+// within it, until a bin stays whole: two rounds for weights that differ.  Every wave reads the histogram for itself.
 template <int HD, int THREADS, int PER>
 __global__ __launch_bounds__(THREADS) void kv4_evict_kernel(Kv4View c, Kv4Evict e, int64_t layer_stride) {
     constexpr int WAVES = THREADS / 64, MOST = THREADS * PER;
-    __shared__ int list[MOST];
-    __shared__ int pages[2][MOST / KV4_PAGE];                    // source, destination
-    __shared__ unsigned lim[2][WAVES];
-    __shared__ __attribute__((aligned(16))) int cnt[2][WAVES];
-    __shared__ int ends[3][WAVES];
+    __shared__ __attribute__((aligned(16))) float weight[MOST];
+    __shared__ uint16_t list[MOST];
+    __shared__ int32_t pages[2][MOST / KV4_PAGE];                // source, destination
+    __shared__ __attribute__((aligned(16))) int hist[4 * 256];   // a round each
+    __shared__ const uint8_t* where[WAVES][64];
+    __shared__ unsigned differ[WAVES];
+    __shared__ int ends[WAVES], refused;
     const int h = blockIdx.x, i = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     int32_t* kept = e.kept + (((int64_t)layer * e.n + i) * c.Hkv + h) * e.keep;
     const bool first = h == 0 && layer == 0;
     const Kv4Entry x = kv4_entry(c, e, i);
-    if (!x.ok) { kv4_refuse<THREADS>(e, kept, i, first); return; }
-    const int ctx = x.ctx, left = ctx < e.keep ? ctx : e.keep;
-    const float* ws = e.weights + (((int64_t)layer * c.n_streams + x.src) * c.Hkv + h) * e.weights_stride;
-    float* wd = e.weights + (((int64_t)layer * c.n_streams + x.dst) * c.Hkv + h) * e.weights_stride;
-    const int base = w * 64 * PER + lane;
-    float wt[PER];
-#pragma unroll
-    for (int p = 0; p < PER; ++p) wt[p] = base + 64 * p < ctx ? ws[base + 64 * p] : 0.f;
-    for (int o = tid; o < (ctx + KV4_PAGE - 1) / KV4_PAGE; o += THREADS) pages[0][o] = c.table[(int64_t)x.src * c.max_pages + o];
-    for (int o = tid; o < (left + KV4_PAGE - 1) / KV4_PAGE; o += THREADS) pages[1][o] = c.table[(int64_t)x.dst * c.max_pages + o];
-    if (__syncthreads_or(kv4_entry_bad<THREADS>(c, e, x, i, left))) { kv4_refuse<THREADS>(e, kept, i, first); return; }
-
+    const int ctx = x.ok ? x.ctx : 0, left = ctx < e.keep ? ctx : e.keep;
+    const int ns = (ctx + KV4_PAGE - 1) / KV4_PAGE, nd = (left + KV4_PAGE - 1) / KV4_PAGE;
     const bool all = ctx <= e.keep;
     const int a = all ? ctx : e.sink, z = all ? ctx : ctx - e.recent, need = all ? 0 : e.keep - e.sink - e.recent;
-    unsigned key[PER], T = 0;                                    // 0: no candidate, or a NaN
+    const int src = x.ok ? x.src : 0, dst = x.ok ? x.dst : 0;
+    const float* ws = e.weights + (((int64_t)layer * c.n_streams + src) * c.Hkv + h) * e.weights_stride;
+    float* wd = e.weights + (((int64_t)layer * c.n_streams + dst) * c.Hkv + h) * e.weights_stride;
+    const float one = need > 0 ? ws[a] : 0.f;
+    {
+        float wt[PER];
 #pragma unroll
-    for (int p = 0; p < PER; ++p) {
-        const int t = base + 64 * p;
-        key[p] = t >= a && t < z ? kv4_weight_key(__float_as_uint(wt[p])) : 0u;
+        for (int p = 0; p < PER; ++p) wt[p] = tid + THREADS * p < ctx ? ws[tid + THREADS * p] : 0.f;
+        if (tid < ns) pages[0][tid] = c.table[(int64_t)src * c.max_pages + tid];
+        if (tid < nd) pages[1][tid] = c.table[(int64_t)dst * c.max_pages + tid];
+        for (int o = tid; o < 1024; o += THREADS) hist[o] = 0;
+        if (tid == 0) refused = !x.ok;
+#pragma unroll
+        for (int p = 0; p < PER; ++p) weight[tid + THREADS * p] = wt[p];
     }
-    if (need > 0) {                                              // 0 < need < z - a
-        unsigned lo = ~0u, hi = 0u;
-#pragma unroll
-        for (int p = 0; p < PER; ++p) {
-            const int t = base + 64 * p;
-            if (t >= a && t < z) { lo = lo < key[p] ? lo : key[p]; hi = hi > key[p] ? hi : key[p]; }
-        }
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const unsigned l2 = (unsigned)__shfl_xor((int)lo, o), h2 = (unsigned)__shfl_xor((int)hi, o);
-            lo = lo < l2 ? lo : l2;
-            hi = hi > h2 ? hi : h2;
-        }
-        if (lane == 0) { lim[0][w] = lo; lim[1][w] = hi; }
-        __syncthreads();
-#pragma unroll
-        for (int o = 0; o < WAVES; ++o) { lo = lo < lim[0][o] ? lo : lim[0][o]; hi = hi > lim[1][o] ? hi : lim[1][o]; }
-        int bit = __builtin_amdgcn_readfirstlane(lo == hi ? -1 : 31 - __clz((int)(lo ^ hi)));
-        T = __builtin_amdgcn_readfirstlane(bit < 0 ? hi : bit == 31 ? 0u : hi >> (bit + 1) << (bit + 1));
-        for (; bit >= 0; --bit) {
-            const unsigned next = T | 1u << bit;
-            int n = 0;
-#pragma unroll
-            for (int p = 0; p < PER; ++p) n += __popcll(__ballot(key[p] >= next));
-            int* shared = cnt[bit & 1];                          // the other one is still being read
-            if (lane == 0) shared[w] = n;
-            __syncthreads();
-            n = 0;
-#pragma unroll
-            for (int o = 0; o < WAVES; ++o) n += shared[o];
-            n = __builtin_amdgcn_readfirstlane(n);
-            if (n >= need) T = next;
-            if (n == need) break;                                // exactly those
-        }
-    }
-    // places, in the order of the tokens: first the waves' counts, then each wave's own
-    int n_stay = 0, n_above = 0, n_tied = 0;
-#pragma unroll
-    for (int p = 0; p < PER; ++p) {
-        const int t = base + 64 * p;
-        const bool in = t >= a && t < z && need > 0, sure = t < ctx && (t < a || t >= z);
-        n_above += __popcll(__ballot(in && key[p] > T));
-        n_tied += __popcll(__ballot(in && key[p] == T));
-        n_stay += __popcll(__ballot(sure));
-    }
-    if (lane == 0) { ends[0][w] = n_stay + n_above; ends[1][w] = n_above; ends[2][w] = n_tied; }
+    const bool taken = kv4_entry_taken<THREADS>(e, x, i);
     __syncthreads();
-    int room = need, out = 0;                                    // tied ones that stay; kept before this wave
+    if (taken || kv4_pages_bad<THREADS>(pages[0], pages[1], ns, nd, c.n_pages)) refused = 1;
+
+    // this thread's: tokens base .. base + PER - 1; bit p of `cand`: one to choose from
+    const int base = tid * PER;
+    const unsigned ref = kv4_weight_key(__float_as_uint(one));
+    unsigned key[PER], cand = 0, diff = 0;
 #pragma unroll
-    for (int o = 0; o < WAVES; ++o) room -= ends[1][o];
-    for (int o = 0; o < w; ++o) {
-        const int n = ends[2][o] < room ? ends[2][o] : room;
-        out += ends[0][o] + n;
-        room -= n;
+    for (int p = 0; p < PER; p += 4) {
+        const f32x4 f = *reinterpret_cast<const f32x4*>(weight + base + p);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const bool in = base + p + q >= a && base + p + q < z;   // (none where nothing is to be chosen and all stay)
+            key[p + q] = kv4_weight_key(__float_as_uint(f[q]));
+            cand |= in ? 1u << (p + q) : 0u;
+            diff |= in ? key[p + q] ^ ref : 0u;
+        }
     }
+    diff = kv4_or_scan(diff);
+    if (lane == 63) differ[w] = diff;
+    __syncthreads();
+    if (refused) {
+        for (int j = tid; j < e.keep; j += THREADS) kept[j] = -1;
+        if (first && tid == 0) e.new_ctx[i] = -1;
+        return;
+    }
+    diff = 0;
+#pragma unroll
+    for (int o = 0; o < WAVES; ++o) diff |= differ[o];
+
+    // T, and how many of those equal to it stay
+    int bits = __builtin_amdgcn_readfirstlane(diff ? 32 - __clz((int)diff) : 0), want = need;
+    unsigned T = __builtin_amdgcn_readfirstlane(bits == 32 ? 0u : ref >> bits << bits);
+    if (need == 0) T = ~0u;                                      // (no weight's key) none of the candidates
+    else {                                                       // 0 < need < z - a
+        for (int* hr = hist; bits > 0; hr += 256) {
+            const int low = bits > 8 ? bits - 8 : 0;             // bits [low, bits)
+            const unsigned mask = (1u << (bits - low)) - 1;
+#pragma unroll
+            for (int p = 0; p < PER; ++p)
+                if ((cand >> p & 1u) && (bits == 32 || key[p] >> bits == T >> bits)) atomicAdd(&hr[key[p] >> low & mask], 1);
+            kv4_lds_barrier();
+            const int4 b4 = *reinterpret_cast<const int4*>(hr + 4 * (63 - lane));   // from the top
+            const int b[4] = {b4.x, b4.y, b4.z, b4.w};
+            const int sum = b[0] + b[1] + b[2] + b[3], upto = kv4_scan(sum);
+            int above = upto - sum, bin = 4 * (63 - lane) + 3, here = b[3];
+            const uint64_t at = __ballot(above < want && upto >= want);
+#pragma unroll
+            for (int o = 2; o >= 0; --o)
+                if (above + here < want) { above += here; here = b[o]; bin = 4 * (63 - lane) + o; }
+            const int from = __ffsll((unsigned long long)at) - 1;
+            T |= (unsigned)__builtin_amdgcn_readlane(bin, from) << low;
+            want -= __builtin_amdgcn_readlane(above, from);
+            if (__builtin_amdgcn_readlane(here, from) == want) break;
+            bits = low;
+        }
+    }
+    // places in the order of the tokens, from the numbers of (those that stay) | (those equal to T) << 16
+    unsigned stay = 0, tied = 0;
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
-        const int t = base + 64 * p;
-        const bool in = t >= a && t < z && need > 0, sure = t < ctx && (t < a || t >= z);
-        const bool tie = in && key[p] == T;
-        const uint64_t ties = __ballot(tie);
-        const int rank = __builtin_amdgcn_mbcnt_hi((unsigned)(ties >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)ties, 0));
-        const bool stay = sure || (in && key[p] > T) || (tie && rank < room);
-        const uint64_t stays = __ballot(stay);
-        const int at = out + __builtin_amdgcn_mbcnt_hi((unsigned)(stays >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)stays, 0));
-        if (stay) { kept[at] = t; wd[at] = wt[p]; list[at] = t; }
-        out += __popcll(stays);
-        const int n = __popcll(ties);
-        room -= n < room ? n : room;
+        const bool in = cand >> p & 1u;
+        stay |= (in ? key[p] > T : base + p < ctx) ? 1u << p : 0u;
+        tied |= in && key[p] == T ? 1u << p : 0u;
     }
-    kv4_clear_rest<THREADS>(e, kept, wd, left);
-    if (first && tid == 0) e.new_ctx[i] = left;
-    __syncthreads();
+    const int mine = __popc(stay) | __popc(tied) << 16, upto = kv4_scan(mine);
+    if (lane == 63) ends[w] = upto;
+    kv4_lds_barrier();
+    int before = upto - mine;
+#pragma unroll
+    for (int o = 0; o < WAVES; ++o) before += o < w ? ends[o] : 0;
+    int room = want - (before >> 16), out = (before & 0xffff) + (room < 0 ? want : before >> 16);
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+        const bool tie = tied >> p & 1u;
+        if ((stay >> p & 1u) || (tie && room > 0)) list[out++] = (uint16_t)(base + p);
+        room -= tie;
+    }
+    kv4_lds_barrier();
     uint8_t* pool = c.pool + (int64_t)layer * layer_stride;
-    for (int pg = w; pg * KV4_PAGE < left; pg += WAVES) {
+    for (int pg = w; pg < nd; pg += WAVES) {
         const int n = left - pg * KV4_PAGE;
-        kv4_move_page<HD>(pool, c.Hkv, h, list + pg * KV4_PAGE, n < KV4_PAGE ? n : KV4_PAGE, pages[1][pg],
+        kv4_move_page<HD>(pool, c.Hkv, h, list + pg * KV4_PAGE, n < KV4_PAGE ? n : KV4_PAGE, pages[1][pg], where[w],
                           [&](int old) { return pages[0][old / KV4_PAGE]; });
     }
+    for (int j = tid; j < e.keep; j += THREADS) kept[j] = j < left ? list[j] : -1;
+    for (int64_t j = tid; j < e.weights_stride; j += THREADS) wd[j] = j < left ? weight[list[j]] : 0.f;
+    if (first && tid == 0) e.new_ctx[i] = left;
 }
 
 // Longer entries: the weights are read again for each of four rounds of an 8-bit radix histogram and once for the places; the pages
@@ -431,7 +474,9 @@ __global__ __launch_bounds__(KV4_CHOOSE_THREADS) void kv4_choose_kernel(Kv4View 
     const Kv4Entry x = kv4_entry(c, e, i);
     if (!x.ok) { kv4_refuse<KV4_CHOOSE_THREADS>(e, kept, i, first); return; }
     const int ctx = x.ctx, left = ctx < e.keep ? ctx : e.keep;
-    if (__syncthreads_or(kv4_entry_bad<KV4_CHOOSE_THREADS>(c, e, x, i, left))) { kv4_refuse<KV4_CHOOSE_THREADS>(e, kept, i, first); return; }
+    if (__syncthreads_or(kv4_entry_taken<KV4_CHOOSE_THREADS>(e, x, i) ||
+                         kv4_pages_bad<KV4_CHOOSE_THREADS>(c.table + (int64_t)x.src * c.max_pages, c.table + (int64_t)x.dst * c.max_pages,
+                                                           (ctx + KV4_PAGE - 1) / KV4_PAGE, (left + KV4_PAGE - 1) / KV4_PAGE, c.n_pages))) { kv4_refuse<KV4_CHOOSE_THREADS>(e, kept, i, first); return; }
     const float* w = e.weights + (((int64_t)layer * c.n_streams + x.src) * c.Hkv + h) * e.weights_stride;
     float* wd = e.weights + (((int64_t)layer * c.n_streams + x.dst) * c.Hkv + h) * e.weights_stride;
 
@@ -484,6 +529,7 @@ __global__ __launch_bounds__(KV4_CHOOSE_THREADS) void kv4_choose_kernel(Kv4View 
 template <int HD>
 __global__ __launch_bounds__(256) void kv4_move_kernel(Kv4View c, Kv4Evict e, int64_t layer_stride) {
     __shared__ int lists[4][KV4_PAGE];
+    __shared__ const uint8_t* where[4][KV4_PAGE];
     const int h = blockIdx.y % c.Hkv, i = blockIdx.y / c.Hkv, layer = blockIdx.z, lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pg = blockIdx.x * 4 + w;
     const int n = e.new_ctx[i] - pg * KV4_PAGE;                  // not positive for a refused entry (-1)
@@ -493,7 +539,7 @@ __global__ __launch_bounds__(256) void kv4_move_kernel(Kv4View c, Kv4Evict e, in
     if (n <= 0) return;
     const int32_t* sp = c.table + (int64_t)e.src[i] * c.max_pages;
     kv4_move_page<HD>(c.pool + (int64_t)layer * layer_stride, c.Hkv, h, lists[w], n < KV4_PAGE ? n : KV4_PAGE,
-                      c.table[(int64_t)e.dst[i] * c.max_pages + pg], [&](int old) { return sp[old / KV4_PAGE]; });
+                      c.table[(int64_t)e.dst[i] * c.max_pages + pg], where[w], [&](int old) { return sp[old / KV4_PAGE]; });
 }
 
 // ------------------------------------------------------------------------------------------------------------------
