@@ -29,15 +29,15 @@
 
 KV4_FN int kv4_slab_bytes(int hd) { return KV4_PAGE * (hd + hd / 16); }
 // byte of the code of token t (0..63), dim d; the low nibble is the even dim
-KV4_FN int kv4_k_at(int hd, int t, int d) {
-    const int q = hd / 4, two = 128 / hd;                       // dims per lane group; tokens per 16 bytes
+KV4_FN int kv4_k_at(int hd, unsigned t, unsigned d) {
+    const unsigned q = hd / 4, two = 128 / hd;                       // dims per lane group; tokens per 16 bytes
     return (t % 4 / two) * 1024 + ((d / q) * 16 + t / 4) * 16 + (t % 4 % two) * 8 + d % q / 2;
 }
-KV4_FN int kv4_v_at(int hd, int t, int d) {
+KV4_FN int kv4_v_at(int hd, unsigned t, unsigned d) {
     return 32 * hd + (d / 64 * 2 + t / 8 % 2) * 1024 + ((t / 16) * 16 + d % 64 / 4) * 16 + t % 8 * 2 + d % 4 / 2;
 }
-KV4_FN int kv4_ks_at(int hd, int t, int d) { return 64 * hd + d / KV4_BLOCK * KV4_PAGE + t; }
-KV4_FN int kv4_vs_at(int hd, int t, int d) { return 66 * hd + d / KV4_BLOCK * KV4_PAGE + t; }
+KV4_FN int kv4_ks_at(int hd, unsigned t, unsigned d) { return 64 * hd + d / KV4_BLOCK * KV4_PAGE + t; }
+KV4_FN int kv4_vs_at(int hd, unsigned t, unsigned d) { return 66 * hd + d / KV4_BLOCK * KV4_PAGE + t; }
 
 // The batch of a call: sequence i owns rows [start, start + n) of the row tensors; they are entries ctx - n .. ctx - 1 of
 // `stream`.  state: 0 = in order, 1 = to be skipped (stream < 0, or no rows), 2 = refused: numbers that do not fit the cache or

@@ -153,7 +153,7 @@ class KV4Cache:
         shape = (batch.rows, self.num_kv_heads, self.head_dim)
         shape = shape if n_layers is None else (layers, *shape)
         k = torch.empty(shape, dtype=dtype, device=self.device)
-        v = torch.empty(shape, dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
         self._run(self._lib.t3_op_kv4_read, self._ref, batch._ref, k.data_ptr(), v.data_ptr(), _DTYPES[dtype], layer, layers)
         return k, v
 
@@ -163,7 +163,7 @@ class KV4Cache:
         """Moves stream src[i] (ctx[i] entries) into the pages of stream dst[i], shortened to its first ``sink``, its last
         ``recent`` and its most attended other entries, ``keep`` in all; per layer and key head by ``weights`` (fp32
         [n_layers, streams, kv_heads, width], as ``new_weights()`` makes it; dst's rows are rewritten).  Covers layers
-        layer .. layer + n_layers - 1, by default all from ``layer`` on.  src keeps its pages.  Returns the new lengths [n] (-1: the
+        layer .. layer + n_layers - 1, by default all from ``layer`` on.  src keeps its pages.  Returns the new lengths, as ctx (-1: the
         entry was refused, see include/t3_hip.h) and the old index of every kept entry [n_layers, n, kv_heads, keep] (-1 behind
         the last)."""
         n = src.numel()
@@ -175,7 +175,7 @@ class KV4Cache:
         self._weights(weights, 4)
         if weights.shape[0] != layers:
             raise ValueError(f"weights must have {layers} layers, got {weights.shape[0]}")
-        new_ctx = torch.empty(n, dtype=torch.int32, device=self.device)
+        new_ctx = torch.empty_like(ctx)
         kept = torch.empty((layers, n, self.num_kv_heads, keep), dtype=torch.int32, device=self.device)
         width = weights.shape[3]
         d = _capi.T3Kv4EvictDesc(src.data_ptr(), dst.data_ptr(), ctx.data_ptr(), weights.data_ptr(), width, new_ctx.data_ptr(),
