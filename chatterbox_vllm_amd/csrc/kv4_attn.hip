@@ -41,9 +41,11 @@ struct Kv4Attn {
     unsigned q_stride, out_stride, inv;        // row strides in elements; ceil(2^32 / group), 0 for a group of one
     int group, tiles, chunks;     // query heads per key head; column tiles and chunks the state buffer holds per (sequence, key head)
     float c;                      // scale * log2(e)
-    float* states;                // [sequence][key head][tile][chunk] x kv4_state_floats
+    // of sequences of few columns, by (sequence, key head, tile): O before its division by l [chunk][16][hd], m and l [16][chunk]
+    float* states;
+    f32x2* ml;
     // for the weights, or null.  Columns of a (sequence, key head) start at kv4_column(), tiles of 16 of them being whole:
-    f32x2* norm;                  // m and 1 / l of each column
+    f32x2* norm;                  // m and 1 / l of each column, where scores are formed again
     uint8_t* frags;               // the queries of each tile as the product takes them: [hd / 32][64 lanes][16 bytes]
     int slots;                    // tiles of a key head that these have room for
     float* scores;                // [sequence][key head][room]: raw scores [column][kv4_kept_width], or null
@@ -53,9 +55,8 @@ struct Kv4Attn {
     __device__ __forceinline__ const uint16_t* q_at(int row, int head_at) const { return q + (uint64_t)(unsigned)row * q_stride + head_at; }
     __device__ __forceinline__ uint16_t* out_at(int row, int head_at) const { return out + (uint64_t)(unsigned)row * out_stride + head_at; }
 };
-// state of (chunk, tile): m[16], l[16], O[16][hd]
-template <int HD> __device__ __forceinline__ int64_t kv4_state_at(const Kv4Attn& a, int Hkv, int seq, int h, int tile, int chunk) {
-    return ((((int64_t)seq * Hkv + h) * a.tiles + tile) * a.chunks + chunk) * (16 * (HD + 2));
+__device__ __forceinline__ int64_t kv4_tile_at(const Kv4Attn& a, int Hkv, int seq, int h, int tile) {
+    return (((int64_t)seq * Hkv + h) * a.tiles + tile) * a.chunks * 16;
 }
 
 // first column of a sequence and key head: sequences in order take disjoint tiles, for floor((a + b) / 16) + 1 >= floor(a / 16) +
@@ -431,12 +432,12 @@ __device__ __forceinline__ void kv4_few_block(const Kv4View& c, const Kv4Rows& b
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e] = fmaf(so[x][k][d + e], f, o[e]);
         }
+        const int64_t at = kv4_tile_at(a, c.Hkv, seq, h, tile);
+        if (a.ml && d == 0) a.ml[at + k * a.chunks + chunk] = f32x2{M, L};
         if (chunks > 1) {
-            float* sp = a.states + kv4_state_at<HD>(a, c.Hkv, seq, h, tile, chunk);
-            if (d == 0) { sp[k] = M; sp[16 + k] = L; }
+            float* sp = a.states + (at + chunk * 16 + k) * HD + d;
 #pragma unroll
-            for (int e = 0; e < 8; e += 4)
-                *reinterpret_cast<f32x4*>(sp + 32 + k * HD + d + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
+            for (int e = 0; e < 8; e += 4) *reinterpret_cast<f32x4*>(sp + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
         } else {
             const int jj = a.row(kcol), hh = h * a.group + kcol - jj * a.group;
             const float inv = L == 0.f ? 0.f : 1.0f / L;          // nothing seen: 0 (a NaN stays one)
@@ -456,52 +457,61 @@ __global__ __launch_bounds__(64 * KV4_FEW_WAVES, HD == 64 ? 4 : 2) void kv4_attn
 
 // Joins the chunks of a column.  A thread has 4 dims; 1024 / HD groups of threads walk the chunks side by side, group x the chunks
 // x, x + groups, ..., and are then added in order.
+template <int HD> struct Kv4JoinLds {
+    f32x2 ml[1024 / HD];
+    f32x4 o[1024 / HD][HD / 4];
+};
 template <int HD, bool F16>
-__global__ __launch_bounds__(256) void kv4_attn_join_kernel(Kv4View c, Kv4Rows b, Kv4Attn a) {
-    constexpr int T = HD / 4, GROUPS = 256 / T, step = 16 * (HD + 2);
-    __shared__ float sm[GROUPS][2];
-    __shared__ __attribute__((aligned(16))) f32x4 so[GROUPS][T];
-    const int h = blockIdx.x % c.Hkv, col = blockIdx.x / c.Hkv;
-    const Kv4Seq s = kv4_seq_of(b, c, blockIdx.y);
+__device__ __forceinline__ void kv4_join_block(const Kv4View& c, const Kv4Rows& b, const Kv4Attn& a, Kv4JoinLds<HD>& lds, int h, int col, int seq) {
+    constexpr int T = HD / 4, GROUPS = 256 / T;
+    const Kv4Seq s = kv4_seq_of(b, c, seq);
     const int rows = s.n < b.max_rows ? s.n : b.max_rows, cols = rows * a.group;
     if (s.state || cols > KV4_FEW_COLUMNS || col >= cols) return;
     const int chunks = kv4_chunks(s.ctx);
     if (chunks <= 1) return;
     const int k = col & 15, group = threadIdx.x / T, t = threadIdx.x % T;
-    const float* sp = a.states + kv4_state_at<HD>(a, c.Hkv, blockIdx.y, h, col >> 4, 0);
+    const int64_t at = kv4_tile_at(a, c.Hkv, seq, h, col >> 4);
+    const f32x2* ml = a.ml + at + k * a.chunks;
+    const float* sp = a.states + (at + k) * HD + 4 * t;
     float M = KV4_NONE, L = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
     for (int x = group; x < chunks; x += GROUPS) {
-        const float* p = sp + (int64_t)x * step;
-        const float m = p[k], l = p[16 + k];
-        const f32x4 v = *reinterpret_cast<const f32x4*>(p + 32 + k * HD + 4 * t);
-        const float top = fmaxf(M, m), f0 = __builtin_amdgcn_exp2f(M - top), f1 = __builtin_amdgcn_exp2f(m - top);
-        L = fmaf(L, f0, l * f1);
+        const f32x2 part = ml[x];
+        const f32x4 v = *reinterpret_cast<const f32x4*>(sp + (int64_t)x * (16 * HD));
+        const float top = fmaxf(M, part[0]), f0 = __builtin_amdgcn_exp2f(M - top), f1 = __builtin_amdgcn_exp2f(part[0] - top);
+        L = fmaf(L, f0, part[1] * f1);
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = fmaf(o[e], f0, v[e] * f1);
         M = top;
     }
-    if (t == 0) { sm[group][0] = M; sm[group][1] = L; }
-    so[group][t] = o;
+    if (t == 0) lds.ml[group] = f32x2{M, L};
+    lds.o[group][t] = o;
     __syncthreads();
     if (threadIdx.x >= T) return;
-    M = sm[0][0];
+    M = lds.ml[0][0];
 #pragma unroll
-    for (int x = 1; x < GROUPS; ++x) M = fmaxf(M, sm[x][0]);
+    for (int x = 1; x < GROUPS; ++x) M = fmaxf(M, lds.ml[x][0]);
     L = 0.f;
     o = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
+#pragma unroll 4
     for (int x = 0; x < GROUPS; ++x) {
-        const float f = __builtin_amdgcn_exp2f(sm[x][0] - M);
-        L = fmaf(sm[x][1], f, L);
+        const float f = __builtin_amdgcn_exp2f(lds.ml[x][0] - M);
+        L = fmaf(lds.ml[x][1], f, L);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = fmaf(so[x][t][e], f, o[e]);
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(lds.o[x][t][e], f, o[e]);
     }
     const int j = a.row(col), head = h * a.group + col - j * a.group;
     const float inv = L == 0.f ? 0.f : 1.0f / L;
     const u32x2 r = {kv4_pack2<F16>(o[0] * inv, o[1] * inv), kv4_pack2<F16>(o[2] * inv, o[3] * inv)};
     *reinterpret_cast<u32x2*>(a.out_at(s.start + j, head * HD + 4 * t)) = r;
-    if (a.norm && t == 0) a.norm[kv4_column(a, h, blockIdx.y, s) + col] = f32x2{M, inv};
+    if (a.norm && t == 0) a.norm[kv4_column(a, h, seq, s) + col] = f32x2{M, inv};
+}
+template <int HD, bool F16>
+__global__ __launch_bounds__(256) void kv4_attn_join_kernel(Kv4View c, Kv4Rows b, Kv4Attn a) {
+    __shared__ __attribute__((aligned(16))) Kv4JoinLds<HD> lds;
+    const int col = blockIdx.x / c.Hkv;
+    kv4_join_block<HD, F16>(c, b, a, lds, blockIdx.x - col * c.Hkv, col, blockIdx.y);
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -751,38 +761,69 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_mixed_kernel(K
 // are formed again from K (half a page's bytes, mostly still on the chip).
 // A stream that occurs in several sequences of the call is done, in their order, by the waves of the first of them.
 // ------------------------------------------------------------------------------------------------------------------
-// Walks the sequences of `stream` from `seq` on, 64 looked at at a time: fn(sequence index).  False if an earlier one has it.
-template <typename Fn> __device__ __forceinline__ bool kv4_of_stream(const Kv4Rows& b, int seq, int stream, int lane, Fn fn) {
-    for (int i = lane; i - lane < seq; i += 64)
-        if (__any(i < seq && b.stream[i < seq ? i : 0] == stream)) return false;
-    for (int i0 = seq; i0 < b.n_seqs; i0 += 64) {
-        const int i = i0 + lane;
-        uint64_t todo = __ballot(i < b.n_seqs && b.stream[i < b.n_seqs ? i : seq] == stream);
-        for (; todo; todo &= todo - 1) fn(i0 + __builtin_ctzll(todo));
+// Walks the sequences of the stream of sequence `seq` if that is the first of them, 64 looked at at a time: fn(their numbers).
+// False if an earlier one is, or if there is no such stream.
+template <typename Fn> __device__ __forceinline__ bool kv4_of_stream(const Kv4Rows& b, const Kv4View& c, int seq, int lane, Fn fn) {
+    const Kv4Seq own = kv4_seq_of(b, c, seq);
+    if (own.stream < 0 || own.stream >= c.n_streams) return false;
+    for (int i0 = 0; i0 < b.n_seqs; i0 += 64) {
+        uint64_t todo = __ballot(i0 + lane < b.n_seqs && b.stream[i0 + lane < b.n_seqs ? i0 + lane : seq] == own.stream);
+        for (; todo; todo &= todo - 1) {
+            const int i = i0 + __builtin_ctzll(todo);
+            if (i < seq) return false;
+            Kv4Seq s = own;
+            if (i != seq) s = kv4_seq_of(b, c, i);
+            fn(i, s);
+        }
     }
     return true;
 }
 
 // Every sequence of the call has its scores kept.  A thread has four entries; with GROUPS = 4 the workgroup's waves take every
 // fourth column each of the same entries and are added in order (the order of the single one while there are at most 4 columns).
+// The columns' m and l are joined here from their chunks', so that this runs beside the join of the outputs, in one launch.
+template <int GROUPS> struct Kv4KeptLds {
+    f32x2 part[256], norm[KV4_FEW_COLUMNS];
+    f32x4 sum[GROUPS][64];
+};
 template <int GROUPS>
-__global__ __launch_bounds__(256) void kv4_weights_kept_kernel(Kv4View c, Kv4Rows b, Kv4Attn a, float* weights, int64_t weights_stride) {
-    __shared__ f32x4 part[GROUPS][64];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = blockIdx.y, seq = blockIdx.z, stream = b.stream[seq];
-    if (stream < 0 || stream >= c.n_streams) return;
-    const int first = (GROUPS == 1 ? blockIdx.x * 256 + threadIdx.x : blockIdx.x * 64 + lane) * 4;
+__device__ __forceinline__ void kv4_kept_block(const Kv4View& c, const Kv4Rows& b, const Kv4Attn& a, Kv4KeptLds<GROUPS>& lds, float* weights,
+                                               int64_t weights_stride, int h, int piece, int seq) {
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int from = piece * (GROUPS == 1 ? 1024 : 256), first = from + (GROUPS == 1 ? tid : lane) * 4;
     f32x4 mine = {0.f, 0.f, 0.f, 0.f};
-    const bool own = kv4_of_stream(b, seq, stream, lane, [&](int i) {
-        const Kv4Seq s = kv4_seq_of(b, c, i);
-        if (s.state || first >= s.ctx) return;
-        const int rows = s.n < b.max_rows ? s.n : b.max_rows, cols = rows * a.group;
+    const bool own = kv4_of_stream(b, c, seq, lane, [&](int i, const Kv4Seq& s) {
+        if (s.state || from >= s.ctx) return;                     // (for all threads)
+        const int rows = s.n < b.max_rows ? s.n : b.max_rows, cols = rows * a.group, chunks = kv4_chunks(s.ctx);
+        // m and 1 / l: 16, 8 or 4 threads a column, every so many chunks each
+        const int log = cols <= 16 ? 4 : cols <= 32 ? 3 : 2, each = tid >> log;
+        float M = KV4_NONE, L = 0.f;
+        if (each < cols) {
+            const f32x2* ml = a.ml + kv4_tile_at(a, c.Hkv, i, h, each >> 4) + (each & 15) * a.chunks;
+            for (int x = tid & ((1 << log) - 1); x < chunks; x += 1 << log) {
+                const f32x2 part = ml[x];
+                const float top = fmaxf(M, part[0]);
+                L = fmaf(L, __builtin_amdgcn_exp2f(M - top), part[1] * __builtin_amdgcn_exp2f(part[0] - top));
+                M = top;
+            }
+        }
+        lds.part[tid] = f32x2{M, L};
+        __syncthreads();
+        if (tid < cols) {
+            M = KV4_NONE;
+            L = 0.f;
+            for (int x = tid << log; x < (tid + 1) << log; ++x) M = fmaxf(M, lds.part[x][0]);
+            for (int x = tid << log; x < (tid + 1) << log; ++x) L = fmaf(lds.part[x][1], __builtin_amdgcn_exp2f(lds.part[x][0] - M), L);
+            lds.norm[tid] = f32x2{M, L == 0.f ? 0.f : 1.0f / L};
+        }
+        __syncthreads();
+        if (first >= s.ctx) return;
         const int64_t width = kv4_kept_width(s.ctx);
         const float* sp = a.scores + ((int64_t)i * c.Hkv + h) * a.room + first;
-        const f32x2* norms = a.norm + kv4_column(a, h, i, s);
 #pragma unroll 4
         for (int col = GROUPS == 1 ? 0 : w; col < cols; col += GROUPS) {
             const int seen = s.ctx - s.n + a.row(col) + 1 - first;
-            const f32x2 norm = norms[col];
+            const f32x2 norm = lds.norm[col];
             const f32x4 x = *reinterpret_cast<const f32x4*>(sp + col * width);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -793,16 +834,35 @@ __global__ __launch_bounds__(256) void kv4_weights_kept_kernel(Kv4View c, Kv4Row
     });
     if (!own) return;                                             // the same in all waves
     if constexpr (GROUPS > 1) {
-        part[w][lane] = mine;
+        lds.sum[w][lane] = mine;
         __syncthreads();
         if (w) return;
 #pragma unroll
-        for (int x = 1; x < GROUPS; ++x) mine += part[x][lane];
+        for (int x = 1; x < GROUPS; ++x) mine += lds.sum[x][lane];
     }
-    float* wp = weights + ((int64_t)stream * c.Hkv + h) * weights_stride + first;
+    float* wp = weights + ((int64_t)b.stream[seq] * c.Hkv + h) * weights_stride + first;
+    const bool any = mine[0] != 0.f || mine[1] != 0.f || mine[2] != 0.f || mine[3] != 0.f;   // else nothing is touched
+    if (weights_stride % 4 == 0 && reinterpret_cast<uintptr_t>(weights) % 16 == 0) {
+        if (any && first < weights_stride) {
+            f32x4 v = *reinterpret_cast<const f32x4*>(wp);
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (mine[e] != 0.f && first + e < weights_stride) wp[e] += mine[e];
+            for (int e = 0; e < 4; ++e) v[e] = mine[e] != 0.f ? v[e] + mine[e] : v[e];
+            *reinterpret_cast<f32x4*>(wp) = v;
+        }
+    } else if (any) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (mine[e] != 0.f && first + e < weights_stride) wp[e] += mine[e];
+    }
+}
+// blocks of a sequence: `joins` columns x key heads of the outputs' join, then its pieces of entries x key heads
+template <int HD, bool F16, int GROUPS>
+__global__ __launch_bounds__(256, 8) void kv4_finish_kernel(Kv4View c, Kv4Rows b, Kv4Attn a, float* weights, int64_t weights_stride, int joins) {
+    __shared__ __attribute__((aligned(16))) union { Kv4JoinLds<HD> join; Kv4KeptLds<GROUPS> kept; } lds;
+    const bool join = (int)blockIdx.x < joins;
+    const int x = join ? blockIdx.x : blockIdx.x - joins, y = x / c.Hkv, h = x - y * c.Hkv;
+    if (join) kv4_join_block<HD, F16>(c, b, a, lds.join, h, y, blockIdx.y);
+    else kv4_kept_block<GROUPS>(c, b, a, lds.kept, weights, weights_stride, h, y, blockIdx.y);
 }
 
 // Some have not: a workgroup per (page, key head, stream).  A wave keeps the page's keys as operands, takes every fourth column tile
@@ -812,13 +872,10 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_kernel(Kv4View c, Kv4Rows 
     __shared__ float part[4][KV4_PAGE];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
     const int h = blockIdx.y, seq = blockIdx.z, p = blockIdx.x, first = p * KV4_PAGE;
-    const int stream = b.stream[seq];
-    if (stream < 0 || stream >= c.n_streams) return;
     bf16x8 kf[4][HD / 32];
     bool have = false;
     float mine = 0.f;                                             // of token first + lane
-    const bool own = kv4_of_stream(b, seq, stream, lane, [&](int i) {
-        const Kv4Seq s = kv4_seq_of(b, c, i);
+    const bool own = kv4_of_stream(b, c, seq, lane, [&](int i, const Kv4Seq& s) {
         if (s.state || first >= s.ctx) return;
         const int rows = s.n < b.max_rows ? s.n : b.max_rows, cols = rows * a.group;
         if (kv4_kept(cols, s.ctx)) {
@@ -834,7 +891,7 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_kernel(Kv4View c, Kv4Rows 
         }
         if (!have) {
             Kv4Page<HD> pg;
-            kv4_fetch_k<HD, false>(pg, c, __builtin_amdgcn_readfirstlane(c.table[(int64_t)stream * c.max_pages + p]), h, lane);
+            kv4_fetch_k<HD, false>(pg, c, __builtin_amdgcn_readfirstlane(c.table[(int64_t)s.stream * c.max_pages + p]), h, lane);
             kv4_operands<HD>(pg, kf);
             have = true;
         }
@@ -906,7 +963,7 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_kernel(Kv4View c, Kv4Rows 
     const int64_t t = first + lane;
     if (w == 0 && t < weights_stride) {
         const float all = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
-        float* wp = weights + ((int64_t)stream * c.Hkv + h) * weights_stride + t;
+        float* wp = weights + ((int64_t)b.stream[seq] * c.Hkv + h) * weights_stride + t;
         if (all != 0.f) *wp += all;
     }
 }
@@ -914,22 +971,28 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_kernel(Kv4View c, Kv4Rows 
 // ------------------------------------------------------------------------------------------------------------------
 // Entry points
 // ------------------------------------------------------------------------------------------------------------------
-// the work buffer: chunk states | kept scores | m and 1 / l | queries
-struct Kv4Work { int64_t states, scores, norm, frags, room; int tiles, chunks, slots; };
+// the work buffer: chunks' O | their m and l | kept scores | m and 1 / l | queries
+struct Kv4Work { int64_t states, ml, scores, norm, frags, room; int tiles, chunks, slots; };
 static Kv4Work plan_work(const t3_kv4_cache* c, const t3_kv4_batch* b, int H, bool weights) {
     Kv4Work w{};
     const int64_t cols = (int64_t)b->max_rows * (H / c->Hkv), few = cols < KV4_FEW_COLUMNS ? cols : KV4_FEW_COLUMNS;
     const int64_t cap = (int64_t)c->max_pages * KV4_PAGE, most = b->max_ctx < cap ? b->max_ctx : cap, pairs = (int64_t)b->n_seqs * c->Hkv;
     w.tiles = (int)((few + 15) / 16);
     w.chunks = kv4_chunks((int)most);
-    w.states = w.chunks > 1 ? pairs * w.tiles * w.chunks * (16 * (c->hd + 2)) * 4 : 0;
+    const int64_t parts = pairs * w.tiles * w.chunks * 16;
+    w.states = w.chunks > 1 ? parts * c->hd * 4 : 0;
+    w.ml = w.chunks > 1 ? parts * 8 : 0;
     if (weights) {
         const int64_t every = few * kv4_kept_width(most);
         w.room = every < KV4_KEEP ? every : KV4_KEEP;
         w.scores = pairs * w.room * 4;
         w.slots = (int)((int64_t)b->rows * (H / c->Hkv) / 16) + b->n_seqs + 1;
-        w.norm = (int64_t)c->Hkv * w.slots * 16 * 8;
-        w.frags = cols > few || every > KV4_KEEP ? (int64_t)c->Hkv * w.slots * 16 * c->hd * 2 : 0;
+        if (cols > few || every > KV4_KEEP) {                     // some scores are formed again
+            w.norm = (int64_t)c->Hkv * w.slots * 16 * 8;
+            w.frags = (int64_t)c->Hkv * w.slots * 16 * c->hd * 2;
+        } else {
+            w.ml = parts * 8;
+        }
     }
     return w;
 }
@@ -941,7 +1004,7 @@ static int check_heads(const t3_kv4_cache* c, int H) {
 extern "C" int64_t t3_op_attn_kv4_work_bytes(const t3_kv4_cache* cache, const t3_kv4_batch* batch, int32_t H, int32_t with_weights) {
     if (kv4_check_cache(cache, 0, 1, nullptr) || kv4_check_batch(batch) || check_heads(cache, H)) return -1;
     const Kv4Work w = plan_work(cache, batch, H, with_weights != 0);
-    return w.states + w.scores + w.norm + w.frags;
+    return w.states + w.ml + w.scores + w.norm + w.frags;
 }
 
 template <int HD, bool F16>
@@ -959,17 +1022,20 @@ static int launch_attn(const Kv4View& c, const Kv4Rows& b, const Kv4Attn& a, flo
         T3_REQUIRE(blocks <= INT32_MAX, "attn_kv4: too many sequences of that many rows in one call");
         T3_LAUNCH((kv4_attn_mixed_kernel<HD, F16, NC>), dim3((unsigned)blocks), dim3(256), 0, st, c, b, a, (int)turns);
     }
-    if (a.chunks > 1)
-        T3_LAUNCH((kv4_attn_join_kernel<HD, F16>), dim3((cols < KV4_FEW_COLUMNS ? (int)cols : KV4_FEW_COLUMNS) * c.Hkv, b.n_seqs), dim3(256), 0, st, c, b, a);
-    if (weights) {
-        const int64_t cap = (int64_t)c.max_pages * KV4_PAGE, most = b.max_ctx < cap ? b.max_ctx : cap;
-        if (!a.frags && cols <= 4)
-            T3_LAUNCH(kv4_weights_kept_kernel<1>, dim3((unsigned)((most + 1023) / 1024), c.Hkv, b.n_seqs), dim3(256), 0, st, c, b, a, weights, weights_stride);
-        else if (!a.frags)
-            T3_LAUNCH(kv4_weights_kept_kernel<4>, dim3((unsigned)((most + 255) / 256), c.Hkv, b.n_seqs), dim3(256), 0, st, c, b, a, weights, weights_stride);
+    const int joins = a.chunks > 1 ? (cols < KV4_FEW_COLUMNS ? (int)cols : KV4_FEW_COLUMNS) * c.Hkv : 0;
+    const int64_t cap = (int64_t)c.max_pages * KV4_PAGE, most = b.max_ctx < cap ? b.max_ctx : cap;
+    if (weights && !a.frags) {
+        if (cols <= 4)
+            T3_LAUNCH((kv4_finish_kernel<HD, F16, 1>), dim3((unsigned)(joins + (most + 1023) / 1024 * c.Hkv), b.n_seqs), dim3(256), 0, st,
+                      c, b, a, weights, weights_stride, joins);
         else
+            T3_LAUNCH((kv4_finish_kernel<HD, F16, 4>), dim3((unsigned)(joins + (most + 255) / 256 * c.Hkv), b.n_seqs), dim3(256), 0, st,
+                      c, b, a, weights, weights_stride, joins);
+    } else {
+        if (joins) T3_LAUNCH((kv4_attn_join_kernel<HD, F16>), dim3(joins, b.n_seqs), dim3(256), 0, st, c, b, a);
+        if (weights)
             T3_LAUNCH((kv4_weights_kernel<HD, F16>), dim3((unsigned)((most + KV4_PAGE - 1) / KV4_PAGE), c.Hkv, b.n_seqs), dim3(256), 0, st,
-                  c, b, a, weights, weights_stride);
+                      c, b, a, weights, weights_stride);
     }
     T3_HIP_CHECK(hipGetLastError());
     return 0;
@@ -1004,9 +1070,13 @@ extern "C" int t3_op_attn_kv4(const t3_kv4_cache* cache, const t3_kv4_batch* bat
     uint8_t* work = static_cast<uint8_t*>(work_dev);
     a.tiles = w.tiles; a.chunks = w.chunks; a.room = w.room;
     a.states = reinterpret_cast<float*>(work);
-    a.scores = w.scores ? reinterpret_cast<float*>(work + w.states) : nullptr;
-    a.norm = weights_dev ? reinterpret_cast<f32x2*>(work + w.states + w.scores) : nullptr;
-    a.frags = w.frags ? work + w.states + w.scores + w.norm : nullptr;
+    work += w.states;
+    a.ml = w.ml ? reinterpret_cast<f32x2*>(work) : nullptr;
+    work += w.ml;
+    a.scores = w.scores ? reinterpret_cast<float*>(work) : nullptr;
+    work += w.scores;
+    a.norm = w.norm ? reinterpret_cast<f32x2*>(work) : nullptr;
+    a.frags = w.frags ? work + w.norm : nullptr;
     a.slots = w.slots;
     const Kv4View c = kv4_view(cache, layer);
     const Kv4Rows b = kv4_rows(batch);
