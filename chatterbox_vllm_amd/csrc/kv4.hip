@@ -589,7 +589,7 @@ extern "C" int64_t t3_op_kv4_page_bytes(int32_t Hkv, int32_t hd) {
 // workgroups along the pages of a sequence, one a key head or one for four; capped (the kernels stride over the rest)
 static int page_groups(const t3_kv4_cache* c, const t3_kv4_batch* b, bool pages) {
     const int64_t heads = pages ? c->Hkv : (c->Hkv + 3) / 4, slices = ((int64_t)b->max_rows + KV4_PAGE - 2) / KV4_PAGE + 1;
-    return (int)(heads * (slices < 16384 ? slices : 16384));
+    return (int)(heads * (slices < 4096 ? slices : 4096));
 }
 template <int HD, bool F16> static void kv4_append_launch(const t3_kv4_cache* cache, const t3_kv4_batch* batch, int layer, const uint16_t* k,
                                                           const uint16_t* v, int64_t k_stride, int64_t v_stride, hipStream_t st) {

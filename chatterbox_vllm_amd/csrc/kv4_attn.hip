@@ -996,13 +996,14 @@ static Kv4Work plan_work(const t3_kv4_cache* c, const t3_kv4_batch* b, int H, bo
     }
     return w;
 }
-static int check_heads(const t3_kv4_cache* c, int H) {
+static int check_sizes(const t3_kv4_cache* c, const t3_kv4_batch* b, int H) {
+    T3_REQUIRE(b->max_ctx <= (1 << 26) || c->max_pages <= (1 << 26) / KV4_PAGE, "attn_kv4: more than 2^26 entries in a stream");
     T3_REQUIRE(H >= c->Hkv && H % c->Hkv == 0 && H / c->Hkv <= 64, "attn_kv4: query heads must be 1..64 times the key heads");
     return 0;
 }
 
 extern "C" int64_t t3_op_attn_kv4_work_bytes(const t3_kv4_cache* cache, const t3_kv4_batch* batch, int32_t H, int32_t with_weights) {
-    if (kv4_check_cache(cache, 0, 1, nullptr) || kv4_check_batch(batch) || check_heads(cache, H)) return -1;
+    if (kv4_check_cache(cache, 0, 1, nullptr) || kv4_check_batch(batch) || check_sizes(cache, batch, H)) return -1;
     const Kv4Work w = plan_work(cache, batch, H, with_weights != 0);
     return w.states + w.ml + w.scores + w.norm + w.frags;
 }
@@ -1045,7 +1046,7 @@ extern "C" int t3_op_attn_kv4(const t3_kv4_cache* cache, const t3_kv4_batch* bat
                               void* out_dev, int64_t out_stride, int32_t H, int32_t dtype, float scale, float* weights_dev,
                               int64_t weights_stride, void* work_dev, int64_t work_bytes, int32_t layer, void* stream) {
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (kv4_check_cache(cache, layer, 1, st) || kv4_check_batch(batch) || check_heads(cache, H)) return 1;
+    if (kv4_check_cache(cache, layer, 1, st) || kv4_check_batch(batch) || check_sizes(cache, batch, H)) return 1;
     T3_REQUIRE(q_dev && out_dev, "attn_kv4: null argument");
     T3_REQUIRE(dtype == 0 || dtype == 1, "attn_kv4: dtype must be 0 (bf16) or 1 (fp16)");
     T3_REQUIRE(scale > 0.f && scale < 1e8f, "attn_kv4: scale must be positive");

@@ -362,7 +362,8 @@ typedef struct t3_kv4_cache {
 } t3_kv4_cache;
 /* The batch that append, attention and read share: sequence i owns rows [seq_start[i], seq_start[i+1]) of the row tensors
  * (prompt rows, drafted tokens, or one row for a decode step), which are the entries ctx[i] - n_i .. ctx[i] - 1 of its stream:
- * ctx counts the entries of the stream AFTER the rows are appended.  A stream may occur in one sequence of a call to append.
+ * ctx counts the entries of the stream AFTER the rows are appended.  A stream may occur in one sequence of a call to append, and
+ * a page that a call writes (append, the dst of evict) must be in one place of the table only.
  * stream < 0: the sequence is skipped, its rows are left as they were.  Rows before entry 0 (n_i > ctx[i]) are not stored and
  * attend to nothing (output 0).  Numbers that do not fit (stream >= n_streams, ctx beyond max_ctx or the block table, rows
  * beyond `rows` or more than max_rows of them, page ids outside the pool) never lead outside a buffer: nothing is stored for
@@ -386,7 +387,7 @@ int t3_op_kv4_read(const t3_kv4_cache* cache, const t3_kv4_batch* batch, void* k
                    int32_t layer, int32_t n_layers, void* stream);
 /* Attention of the batch's rows over the cache: row j of n of a sequence sees its first ctx - n + j + 1 entries (causal).
  * q_dev: row r at q_dev + r * q_stride elements, [H][hd] inside it, H = group * Hkv, group 1..64 query heads per key head; out
- * likewise.  A row that sees nothing gets 0.  scale > 0 multiplies the scores.
+ * likewise.  A row that sees nothing gets 0.  scale > 0 multiplies the scores.  At most 2^26 entries a stream.
  * weights_dev (optional): [n_streams][Hkv][weights_stride] fp32; every entry's softmax weights, summed over the call's rows and
  * over the query heads of its key head, are added to it (in a fixed order: equal calls give equal bits).  weights_stride >=
  * max_ctx.  A refused sequence adds nothing.

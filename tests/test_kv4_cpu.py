@@ -212,6 +212,14 @@ def test_evict_refusals(kw, words):
     _refused(lib, lib.t3_op_kv4_evict(C.byref(_cache()), None, None), "null")
 
 
+def test_attention_refuses_what_its_grid_cannot_hold():
+    lib = _capi.load()
+    cache, batch = _cache(max_pages=1 << 21), _batch(max_ctx=(1 << 26) + 1)
+    _refused(lib, lib.t3_op_attn_kv4(C.byref(cache), C.byref(batch), A, 1024, A, 1024, 16, 0, 0.125, None, 0, A, 1 << 60, 0, None), r"2\^26")
+    assert lib.t3_op_attn_kv4_work_bytes(C.byref(cache), C.byref(batch), 16, 0) == -1
+    assert lib.t3_op_attn_kv4_work_bytes(C.byref(cache), C.byref(_batch(max_ctx=1 << 26)), 16, 0) > 0
+
+
 def test_sizes():
     lib = _capi.load()
     assert lib.t3_op_kv4_page_bytes(16, 64) == 16 * 4352 and lib.t3_op_kv4_page_bytes(1, 128) == 8704

@@ -314,6 +314,43 @@ def test_weights_of_a_stream_that_occurs_twice():
         assert torch.equal(check_attend(m, cache, rows, ctx, 2, "bf16", True, streams=streams)[2], w)
 
 
+@pytest.mark.parametrize("hd,group", [(64, 1), (64, 5), (128, 8), (128, 21)])
+def test_weights_of_few_columns_over_many_chunks(hd, group):
+    """Scores kept, contexts of one to three chunks, a stream in two sequences; rows of weights that are not a multiple of four long."""
+    m = _kv4.Model(hd, 2, 1, 4 * 40, 4, 40, seed=23)
+    rows, ctx, streams = [1, 3, 2, 1, 1], [2500, 1025, 1500, 2490, 3], [2, 0, 2, 3, 1]
+    for i, t in ((0, 1025), (1, 3), (2, 2500), (3, 2490)):
+        m.fill(i, t)
+    cache = device_cache(m)
+    q, out, w = check_attend(m, cache, rows, ctx, group, "bf16", True, streams=streams)
+    assert torch.equal(check_attend(m, cache, rows, ctx, group, "bf16", True, streams=streams)[2], w)
+    batch = cache.batch(i32(starts(rows)), i32(streams), i32(ctx), rows=sum(rows), max_rows=3, max_ctx=2500)
+    wide, odd = (torch.zeros(4, 2, width, device=DEV) for width in (2560, 2501))
+    for one in (wide, odd):
+        assert torch.equal(cache.attend(q.to(DEV), batch, weights=one), out)
+    assert torch.equal(wide[..., :2501], odd)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_rows_beyond_what_one_launch_has_workgroups_for(hd):
+    """270000 rows of one sequence at once give the bytes that they give a thousand at a time, and come back."""
+    n, pages = 270000, 4219
+    caches = [KV4Cache(1, hd, num_pages=pages, block_table=torch.randperm(pages, generator=torch.Generator().manual_seed(24)).to(torch.int32).to(DEV).view(1, -1)) for _ in range(2)]
+    g = torch.Generator(device=DEV).manual_seed(25)
+    k, v = (torch.randn(n, 1, hd, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    whole = [c.batch(i32([0, n]), i32([0]), i32([n]), rows=n) for c in caches]
+    caches[0].append(k, v, whole[0])
+    for i in range(0, n, 999):
+        part = min(999, n - i)
+        caches[1].append(k[i:i + part], v[i:i + part], caches[1].batch(i32([0, part]), i32([0]), i32([i + part]), rows=part))
+    assert torch.equal(caches[0].pool, caches[1].pool)
+    got = caches[0].read(whole[0])
+    for i in (0, 200000, n - 1000):
+        part = caches[1].read(caches[1].batch(i32([0, 1000]), i32([0]), i32([i + 1000]), rows=1000))
+        assert all(torch.equal(a[i:i + 1000], b) for a, b in zip(got, part))
+        assert ((got[0][i:i + 1000].float() - k[i:i + 1000].float()).abs() <= k[i:i + 1000].float().abs().amax(-1, keepdim=True) / 3.5).all()   # half a step
+
+
 def test_offsets_past_32_bits():
     """A pool of more than 4 GiB, pages at its end."""
     pages = (1 << 32) // page_bytes(8, 128) + 40
