@@ -7,7 +7,9 @@
 //   2^e = the smallest power of two with a / 2^e < 7,   code = e2m1 value nearest to x / 2^e (ties to the even code).
 // A thread takes 8 dims of K and the same of V (two 16-byte loads).  The bits of |x| of either type order like the values, so the
 // maxima run on 16-bit halves, K's in the low one and V's in the high one after the first step; the conversion rounds, scales and packs
-// two values at a time from the type that they come in.
+// two values at a time from the type that they come in.  Bound by what it reads: 12 x 1000 rows x 8 heads of 128, 49 MB in and 13 MB
+// out, 11 us (5.6 TB/s; with values widened to fp32, one wave a page and two-byte stores of V 20).  A row for each of 64 streams x 16
+// heads of 64: 3.5 us, all of it launch and latency.
 // ------------------------------------------------------------------------------------------------------------------
 typedef __attribute__((ext_vector_type(2))) uint16_t u16x2;
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
@@ -129,7 +131,8 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4View c, Kv4Rows b, c
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Read: the inverse, a thread 8 dims of K and of V.
+// Read: the inverse, a thread 8 dims of K and of V.  Bound by what it writes: 8 streams x 30 layers x 16 heads x 640 entries of 64, 167 MB
+// in and 629 MB out, 133 us (6.0 TB/s; straight from memory with divisions per thread 268).
 // ------------------------------------------------------------------------------------------------------------------
 template <bool F16> __device__ __forceinline__ u32x4 kv4_values8(unsigned codes, unsigned byte, bool nan) {
     if constexpr (F16) {
@@ -211,6 +214,9 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4View c, Kv4Rows b, int
 // the lower index, so that the set is what any correct sort would give.  Per (entry, key head, layer) on its own:
 //   T = the largest key with at least `need` candidate keys >= T, found from the highest bit in which they differ down;
 //   what is above T stays, and the first need - |above T| of those equal to it.
+// Bound by the bytes moved: the kept entries lie scattered, so every line of the source is read (8 streams x 30 layers x 16 heads of
+// 64, 1500..2011 entries to 640: 457 MB, with 208 MB written 690 MB in 146 us, 4.7 TB/s; choice and move as two launches 355).  One layer
+// of 4 streams x 16 heads is latency, a chain of about eight loads and barriers: 9 us (17.4).
 // ------------------------------------------------------------------------------------------------------------------
 struct Kv4Evict {
     const int32_t* src; const int32_t* dst; const int32_t* ctx;
@@ -327,17 +333,18 @@ __device__ __forceinline__ void kv4_lds_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// Entries of at most THREADS * PER tokens, choice and move in one launch.  The weights go through shared memory to threads that have
+// Entries of at most THREADS * PER tokens, with MOVE choice and move in one launch.  The weights go through shared memory to threads that have
 // PER neighbouring ones.  The bits that all candidates share are skipped; a histogram of the next 8 gives the bin of T, and so on
-// within it, until a bin stays whole: two rounds for weights that differ.  Every wave reads the histogram for itself.
-template <int HD, int THREADS, int PER>
+// within it, until a bin stays whole: two rounds for weights that differ, 1300 clocks each (bit by bit 15 steps of 520).  Every wave
+// reads the histogram for itself.
+template <int HD, int THREADS, int PER, bool MOVE>
 __global__ __launch_bounds__(THREADS) void kv4_evict_kernel(Kv4View c, Kv4Evict e, int64_t layer_stride) {
     constexpr int WAVES = THREADS / 64, MOST = THREADS * PER;
     __shared__ __attribute__((aligned(16))) float weight[MOST];
     __shared__ uint16_t list[MOST];
     __shared__ int32_t pages[2][MOST / KV4_PAGE];                // source, destination
     __shared__ __attribute__((aligned(16))) int hist[4 * 256];   // a round each
-    __shared__ const uint8_t* where[WAVES][64];
+    __shared__ const uint8_t* where[MOVE ? WAVES : 1][64];
     __shared__ unsigned differ[WAVES];
     __shared__ int ends[WAVES], refused;
     const int h = blockIdx.x, i = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
@@ -444,19 +451,21 @@ __global__ __launch_bounds__(THREADS) void kv4_evict_kernel(Kv4View c, Kv4Evict 
         room -= tie;
     }
     kv4_lds_barrier();
-    uint8_t* pool = c.pool + (int64_t)layer * layer_stride;
-    for (int pg = w; pg < nd; pg += WAVES) {
-        const int n = left - pg * KV4_PAGE;
-        kv4_move_page<HD>(pool, c.Hkv, h, list + pg * KV4_PAGE, n < KV4_PAGE ? n : KV4_PAGE, pages[1][pg], where[w],
-                          [&](int old) { return pages[0][old / KV4_PAGE]; });
+    if constexpr (MOVE) {
+        uint8_t* pool = c.pool + (int64_t)layer * layer_stride;
+        for (int pg = w; pg < nd; pg += WAVES) {
+            const int n = left - pg * KV4_PAGE;
+            kv4_move_page<HD>(pool, c.Hkv, h, list + pg * KV4_PAGE, n < KV4_PAGE ? n : KV4_PAGE, pages[1][pg], where[w],
+                              [&](int old) { return pages[0][old / KV4_PAGE]; });
+        }
     }
     for (int j = tid; j < e.keep; j += THREADS) kept[j] = j < left ? list[j] : -1;
     for (int64_t j = tid; j < e.weights_stride; j += THREADS) wd[j] = j < left ? weight[list[j]] : 0.f;
     if (first && tid == 0) e.new_ctx[i] = left;
 }
 
-// Longer entries: the weights are read again for each of four rounds of an 8-bit radix histogram and once for the places; the pages
-// are moved by a launch of their own, which has workgroups for all of them.
+// Longer entries than a workgroup holds: the weights are read again for each of four rounds of an 8-bit radix histogram and once for
+// the places.
 #define KV4_CHOOSE_THREADS 1024
 
 // sum over the workgroup's threads before this one; total in *all
@@ -645,13 +654,19 @@ extern "C" int t3_op_kv4_read(const t3_kv4_cache* cache, const t3_kv4_batch* bat
     return 0;
 }
 
-#ifndef KV4_HELD_MOST
-#define KV4_HELD_MOST 8192
-#endif
-template <int HD> static void kv4_evict_held(const Kv4View& c, const Kv4Evict& e, int layers, int64_t layer_stride, hipStream_t st) {
+template <int HD> static void kv4_evict_launch(const Kv4View& c, const Kv4Evict& e, int layers, int64_t layer_stride, hipStream_t st) {
     const dim3 grid(c.Hkv, e.n, layers);
-    if (e.max_ctx <= 2048) T3_LAUNCH((kv4_evict_kernel<HD, 256, 8>), grid, dim3(256), 0, st, c, e, layer_stride);
-    else T3_LAUNCH((kv4_evict_kernel<HD, 1024, 8>), grid, dim3(1024), 0, st, c, e, layer_stride);
+    // Pages moved by the workgroup that chose them, up to 2048 entries: 4 streams of 2000 x 16 heads of 64 10.5 us, 8 streams x 30 layers
+    // 158; moved by a launch of their own 12.3 and 209.  Above, few workgroups would move many pages: one stream of 8000 to 6000 x 8 heads
+    // of 128 17 us, moved by those that chose 71.  Above 8192 the weights are not held: 4 streams of 8000 18.5 us held, 36.9 not.
+    if (e.max_ctx <= 2048) {
+        T3_LAUNCH((kv4_evict_kernel<HD, 256, 8, true>), grid, dim3(256), 0, st, c, e, layer_stride);
+        return;
+    }
+    if (e.max_ctx <= 8192) T3_LAUNCH((kv4_evict_kernel<HD, 1024, 8, false>), grid, dim3(1024), 0, st, c, e, layer_stride);
+    else T3_LAUNCH(kv4_choose_kernel, grid, dim3(KV4_CHOOSE_THREADS), 0, st, c, e);
+    const int most = e.keep < e.max_ctx ? e.keep : e.max_ctx;
+    T3_LAUNCH(kv4_move_kernel<HD>, dim3((most + 4 * KV4_PAGE - 1) / (4 * KV4_PAGE), c.Hkv * e.n, layers), dim3(256), 0, st, c, e, layer_stride);
 }
 
 extern "C" int t3_op_kv4_evict(const t3_kv4_cache* cache, const t3_kv4_evict_desc* d, void* stream) {
@@ -666,16 +681,8 @@ extern "C" int t3_op_kv4_evict(const t3_kv4_cache* cache, const t3_kv4_evict_des
     const Kv4View c = kv4_view(cache, d->layer);
     const Kv4Evict e{d->src_dev, d->dst_dev, d->ctx_dev, d->weights_dev, d->weights_stride, d->new_ctx_dev, d->kept_dev,
                      d->n, d->max_ctx, d->keep, d->sink, d->recent};
-    if (d->max_ctx <= KV4_HELD_MOST) {
-        if (cache->hd == 64) kv4_evict_held<64>(c, e, d->n_layers, cache->layer_stride, st);
-        else kv4_evict_held<128>(c, e, d->n_layers, cache->layer_stride, st);
-    } else {
-        T3_LAUNCH(kv4_choose_kernel, dim3(cache->Hkv, d->n, d->n_layers), dim3(KV4_CHOOSE_THREADS), 0, st, c, e);
-        const int most = d->keep < d->max_ctx ? d->keep : d->max_ctx;
-        const dim3 grid((most + 4 * KV4_PAGE - 1) / (4 * KV4_PAGE), cache->Hkv * d->n, d->n_layers);
-        if (cache->hd == 64) T3_LAUNCH(kv4_move_kernel<64>, grid, dim3(256), 0, st, c, e, cache->layer_stride);
-        else T3_LAUNCH(kv4_move_kernel<128>, grid, dim3(256), 0, st, c, e, cache->layer_stride);
-    }
+    if (cache->hd == 64) kv4_evict_launch<64>(c, e, d->n_layers, cache->layer_stride, st);
+    else kv4_evict_launch<128>(c, e, d->n_layers, cache->layer_stride, st);
     T3_HIP_CHECK(hipGetLastError());
     return 0;
 }

@@ -3,7 +3,7 @@
 // A column is a (row, query head) pair; the group = H / Hkv query heads of a key head and the rows of a sequence share its keys,
 // so column c of a sequence and key head is row c / group, head c % group, and 16 columns make one tile of
 //   S^T[token][column] = K Q^T        K codes -> bf16 in registers (exact), Q held in registers for the whole pass
-//   O^T[dim][column]   = V^T P^T      P as bf16 hi + lo parts, so the probabilities keep 16 significant bits
+//   O^T[dim][column]   = V^T P^T      P as bf16 hi + lo parts, so the probabilities keep 16 significant bits (bf16 prompts: hi)
 // on v_mfma_f32_16x16x32_bf16, a page of 64 tokens at a time.  A lane ends the first product with 16 consecutive tokens of one
 // column, which is what the second takes from it: no exchange but the maximum over the four lane groups.
 // fp16 queries enter as bf16 hi + lo (exact to 2^-16 of the value, fp16 has 11 bits), so one set of products serves both types.
@@ -13,8 +13,14 @@
 // sums are rarely rescaled.  Keeping m as the rounded product makes the factors between pages and chunks, exp2(m - m'), consistent at any size of s.
 //
 // Sequences of at most KV4_FEW_COLUMNS columns (decode steps, drafted tokens) are cut into chunks of their cache, a workgroup of
-// four waves each; a second launch joins the chunks in order.  The chunk length follows from the sequence's own length, so a
-// row's bits do not depend on the batch.  Longer ones (prompts) run whole: a wave keeps four column tiles and walks the cache.
+// four waves each; a second launch joins the chunks in order.  Longer ones (prompts) run whole: a wave keeps one or two column tiles and
+// walks the cache.  Which form and how many chunks follow from the sequence alone, so a row's bits do not depend on the batch.
+//
+// Few columns are bound by the cache's bytes where there are many (16 x 32 heads on 8 key heads of 128, 9000..32749 entries: 386 MB in
+// 77 us, 5.0 TB/s) and by latency where there are few (64 x 16 heads of 64, 120..1000 entries: 39 MB in 13 us; one stream 5 us).
+// Many are bound by the instructions: matrix and vector instructions of a SIMD do not run beside each other (measured: a 16x16x32
+// product 17.6 clocks, an fma 2.5, an exp2 10, mixed ones the sum), so both count, and the products stand in blocks, each change
+// from one kind to the other costing about 5 clocks.  2 x 4095 rows x 32 heads on 8 of 128: 347 GFLOP in 388 us, 0.9 PFLOP/s.
 #include "kv4_common.h"
 
 #include <type_traits>
@@ -23,8 +29,9 @@
 #define KV4_SLACK 8.f             // the reference moves when a maximum passes it by 2^8
 #define KV4_NONE -1e30f           // running maximum before the first visible token
 
-// A chunk is 16 pages: the four waves of its workgroup take four each.  (8 waves: 64 x 12 heads of 64 over 1.4k entries 13.2 -> 14.9 us,
-// 16 heads of 128 over up to 32k 77 -> 107; 32 pages: one sequence of 4k 13.5 -> 18.5, the long one 76.)
+// A chunk is 16 pages: the four waves of its workgroup take four each.  (8 waves: 64 x 16 heads of 64 over up to 1000 entries 13.2 -> 14.9 us,
+// 16 x 32 heads of 128 over up to 32k 77 -> 107; 32 pages: one sequence of 4k 13.5 -> 18.5, the long ones 76; 8 pages: 10 and 79, one of
+// 1k 6.6 -> 10, drafts of 40 columns 27.2 -> 28.1.)
 #define KV4_FEW_WAVES 4
 #define KV4_CHUNK_PAGES 16
 KV4_FN int kv4_chunks(int ctx) { return (int)(((int64_t)ctx + KV4_CHUNK_PAGES * KV4_PAGE - 1) / (KV4_CHUNK_PAGES * KV4_PAGE)); }
@@ -456,7 +463,7 @@ __global__ __launch_bounds__(64 * KV4_FEW_WAVES, HD == 64 ? 4 : 2) void kv4_attn
 }
 
 // Joins the chunks of a column.  A thread has 4 dims; 1024 / HD groups of threads walk the chunks side by side, group x the chunks
-// x, x + groups, ..., and are then added in order.
+// x, x + groups, ..., and are then added in order.  Latency: 4 to 5 us at 64 x 16 heads x 2 chunks and at 16 x 32 heads x 32 chunks.
 template <int HD> struct Kv4JoinLds {
     f32x2 ml[1024 / HD];
     f32x4 o[1024 / HD][HD / 4];
@@ -756,9 +763,11 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_mixed_kernel(K
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Weights: W[stream][key head][t] += sum over the sequence's columns of exp2(s c - m) / l.  One wave per (page, key head, stream)
-// walks the columns in order, so there are no atomics.  Scores of sequences of few columns were kept by the pass above; the others
-// are formed again from K (half a page's bytes, mostly still on the chip).
+// Weights: W[stream][key head][t] += sum over the sequence's columns of exp2(s c - m) / l.  A workgroup owns its entries and walks the
+// columns in a fixed order, so there are no atomics.  Scores of sequences of few columns were kept by the pass above (64 decode rows x
+// 16 heads of 64 over up to 2000 entries 55 us -> 37, 32 x 64 heads on 8 of 128 over up to 8000 122 -> 74; 40 columns 37 -> 28); the
+// others are formed again from K, from queries that the pass above leaves in operand order (2 x 4095 rows x 32 heads of 128: 300 us
+// beside the pass's 388; from the rows as given 380, by one wave a page 1170).
 // A stream that occurs in several sequences of the call is done, in their order, by the waves of the first of them.
 // ------------------------------------------------------------------------------------------------------------------
 // Walks the sequences of the stream of sequence `seq` if that is the first of them, 64 looked at at a time: fn(their numbers).
@@ -781,7 +790,8 @@ template <typename Fn> __device__ __forceinline__ bool kv4_of_stream(const Kv4Ro
 
 // Every sequence of the call has its scores kept.  A thread has four entries; with GROUPS = 4 the workgroup's waves take every
 // fourth column each of the same entries and are added in order (the order of the single one while there are at most 4 columns).
-// The columns' m and l are joined here from their chunks', so that this runs beside the join of the outputs, in one launch.
+// The columns' m and l are joined here from their chunks', so that this runs beside the join of the outputs, in one launch: 9 to 10 us
+// at 64 x 16 heads x 300..2000 entries, latency (a chain of six loads and barriers at 32 waves a CU).
 template <int GROUPS> struct Kv4KeptLds {
     f32x2 part[256], norm[KV4_FEW_COLUMNS];
     f32x4 sum[GROUPS][64];
