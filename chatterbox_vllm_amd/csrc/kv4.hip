@@ -678,6 +678,9 @@ extern "C" int t3_op_kv4_evict(const t3_kv4_cache* cache, const t3_kv4_evict_des
     T3_REQUIRE(d->max_ctx >= 1 && d->max_ctx <= d->weights_stride, "kv4_evict: max_ctx must be 1..weights_stride");
     T3_REQUIRE(d->sink >= 0 && d->recent >= 0 && d->keep >= 1 && (int64_t)d->sink + d->recent <= d->keep, "kv4_evict: sink + recent <= keep, keep >= 1");
     T3_REQUIRE(d->keep <= d->weights_stride, "kv4_evict: keep must be at most weights_stride");
+    // (entries are read by workgroups that start while others have finished)
+    const auto apart = [&](const int32_t* p) { return p >= d->new_ctx_dev + d->n || d->new_ctx_dev >= p + d->n; };
+    T3_REQUIRE(apart(d->src_dev) && apart(d->dst_dev) && apart(d->ctx_dev), "kv4_evict: new_ctx must not overlap src, dst or ctx");
     const Kv4View c = kv4_view(cache, d->layer);
     const Kv4Evict e{d->src_dev, d->dst_dev, d->ctx_dev, d->weights_dev, d->weights_stride, d->new_ctx_dev, d->kept_dev,
                      d->n, d->max_ctx, d->keep, d->sink, d->recent};

@@ -387,7 +387,7 @@ int t3_op_kv4_read(const t3_kv4_cache* cache, const t3_kv4_batch* batch, void* k
                    int32_t layer, int32_t n_layers, void* stream);
 /* Attention of the batch's rows over the cache: row j of n of a sequence sees its first ctx - n + j + 1 entries (causal).
  * q_dev: row r at q_dev + r * q_stride elements, [H][hd] inside it, H = group * Hkv, group 1..64 query heads per key head; out
- * likewise.  A row that sees nothing gets 0.  scale > 0 multiplies the scores.  At most 2^26 entries a stream.
+ * likewise; out may be q (the same rows), but not overlap it otherwise.  A row that sees nothing gets 0.  scale > 0 multiplies the scores.  At most 2^26 entries a stream.
  * weights_dev (optional): [n_streams][Hkv][weights_stride] fp32; every entry's softmax weights, summed over the call's rows and
  * over the query heads of its key head, are added to it (in a fixed order: equal calls give equal bits).  weights_stride >=
  * max_ctx.  A refused sequence adds nothing.
@@ -404,7 +404,8 @@ int t3_op_attn_kv4(const t3_kv4_cache* cache, const t3_kv4_batch* batch, const v
  * lowest).  min(ctx, keep) entries remain, in their old order; their weights move along and the rest of dst's weights row is
  * cleared.  src is left as it was: its pages are the caller's to free (or to keep, where another stream shares them).
  * weights_dev [n_layers][n_streams][Hkv][weights_stride] fp32, new_ctx_dev [n], kept_dev [n_layers][n][Hkv][keep] (old entry of
- * each new one, ascending, -1 behind the last).  sink + recent <= keep <= weights_stride, max_ctx <= weights_stride.
+ * each new one, ascending, -1 behind the last).  sink + recent <= keep <= weights_stride, max_ctx <= weights_stride.  new_ctx is a
+ * buffer of its own.
  * Refused with new_ctx = -1 (nothing moved, kept -1): streams or page ids out of range, ctx < 0 or > max_ctx, a page of dst that
  * is also a page of src, a dst that an earlier entry has too or that any entry has as src. */
 typedef struct t3_kv4_evict_desc {

@@ -134,10 +134,13 @@ def _batch(**kw):
 
 
 def _evict(**kw):
-    d = dict(src_dev=A, dst_dev=A, ctx_dev=A, weights_dev=A, weights_stride=256, new_ctx_dev=A, kept_dev=A, n=2, max_ctx=256, keep=32,
+    d = dict(src_dev=A, dst_dev=A, ctx_dev=A, weights_dev=A, weights_stride=256, new_ctx_dev=A + 4096, kept_dev=A, n=2, max_ctx=256, keep=32,
              sink=4, recent=8, layer=0, n_layers=2)
     d.update(kw)
     return _capi.T3Kv4EvictDesc(**d)
+
+
+B = A + 4096                                                     # another
 
 
 def _refused(lib, rc, words):
@@ -204,7 +207,8 @@ def test_attention_refusals(kw, words):
 @pytest.mark.parametrize("kw,words", [
     (dict(src_dev=None), "null"), (dict(dst_dev=None), "null"), (dict(ctx_dev=None), "null"), (dict(weights_dev=None), "null"),
     (dict(new_ctx_dev=None), "null"), (dict(kept_dev=None), "null"), (dict(n=0), "entries"), (dict(n=5000), "entries"), (dict(max_ctx=257), "max_ctx"),
-    (dict(max_ctx=0), "max_ctx"), (dict(keep=0), "keep"), (dict(sink=25), "sink"), (dict(sink=-1), "sink"), (dict(recent=-1), "sink"),
+    (dict(max_ctx=0), "max_ctx"), (dict(new_ctx_dev=A), "overlap"), (dict(new_ctx_dev=A + 4), "overlap"), (dict(ctx_dev=B + 4), "overlap"), (dict(dst_dev=B - 4), "overlap"),
+    (dict(keep=0), "keep"), (dict(sink=25), "sink"), (dict(sink=-1), "sink"), (dict(recent=-1), "sink"),
     (dict(sink=2147483647, recent=2147483647), "sink"), (dict(keep=257), "keep"), (dict(layer=1), "layer"), (dict(n_layers=3), "layer"), (dict(n_layers=0), "layer")])
 def test_evict_refusals(kw, words):
     lib = _capi.load()

@@ -351,6 +351,20 @@ def test_rows_beyond_what_one_launch_has_workgroups_for(hd):
         assert ((got[0][i:i + 1000].float() - k[i:i + 1000].float()).abs() <= k[i:i + 1000].float().abs().amax(-1, keepdim=True) / 3.5).all()   # half a step
 
 
+@pytest.mark.parametrize("hd,rows,ctx", [(64, [1, 5, 3], [40, 2000, 3]), (128, [200, 1, 70], [200, 3000, 500])])
+def test_out_may_be_q(hd, rows, ctx):
+    m = _kv4.Model(hd, 2, 1, 3 * 47, 3, 47, seed=26)
+    for i, t in enumerate(ctx):
+        m.fill(i, t)
+    cache = device_cache(m)
+    q = torch.randn(sum(rows), 6, hd, generator=torch.Generator().manual_seed(27)).to(torch.bfloat16).to(DEV)
+    batch = cache.batch(i32(starts(rows)), i32([0, 1, 2]), i32(ctx), rows=sum(rows), max_rows=max(rows), max_ctx=max(ctx))
+    w, w2 = cache.new_weights()[0], cache.new_weights()[0]
+    want = cache.attend(q, batch, weights=w)
+    assert cache.attend(q, batch, out=q, weights=w2) is q
+    assert torch.equal(q, want) and torch.equal(w, w2)
+
+
 def test_offsets_past_32_bits():
     """A pool of more than 4 GiB, pages at its end."""
     pages = (1 << 32) // page_bytes(8, 128) + 40
