@@ -27,7 +27,7 @@
 
 #define KV4_FEW_COLUMNS 64        // rows x group up to which a sequence is cut along its cache
 #define KV4_SLACK 8.f             // the reference moves when a maximum passes it by 2^8
-#define KV4_NONE -1e30f           // running maximum before the first visible token
+#define KV4_NONE -3e38f           // running maximum before the first visible token (finite: differences of it stay numbers)
 
 // A chunk is 16 pages: the four waves of its workgroup take four each.  (8 waves: 64 x 16 heads of 64 over up to 1000 entries 13.2 -> 14.9 us,
 // 16 x 32 heads of 128 over up to 32k 77 -> 107; 32 pages: one sequence of 4k 13.5 -> 18.5, the long ones 76; 8 pages: 10 and 79, one of

@@ -218,6 +218,24 @@ def test_sharp_and_flat_scores():
         assert ((out[:-3].double() - ref).abs() <= _kv4.out_bound(ref, size, bound, t, torch.bfloat16, rows)).all()
 
 
+@pytest.mark.parametrize("hd,rows,ctx", [(64, 1, 2000), (128, 3, 70), (64, 130, 130)])
+def test_scores_far_below_zero(hd, rows, ctx):
+    """Scores of -1.6e32 and below: the maximum is still found, and equal scores still share the weight."""
+    m = _kv4.Model(hd, 1, 1, 40, 1, 32, seed=28)
+    k = torch.full((ctx, 1, hd), -2.0 ** 44)
+    k[5:9] = -2.0 ** 43                                           # the heaviest four
+    v = torch.randn(ctx, 1, hd, generator=torch.Generator().manual_seed(29))
+    m.put(m.pool, 0, torch.arange(ctx), k, v)
+    _, v = m.get(m.pool, 0, torch.arange(ctx))
+    cache = device_cache(m)
+    q = torch.full((rows, 1, hd), 2.0 ** 60, dtype=torch.bfloat16, device=DEV)
+    out = cache.attend(q, cache.batch(i32([0, rows]), i32([0]), i32([ctx]), rows=rows)).cpu().double()
+    for j in range(rows):
+        sees = ctx - rows + j + 1
+        want = v[5:9].mean(0) if sees >= 9 else v[5:sees].mean(0) if sees > 5 else v[:sees].mean(0)
+        assert ((out[j] - want).abs() <= v.abs().max() * 2.0 ** -8 * 1.01).all(), j
+
+
 def test_what_lies_behind_the_last_entry_does_not_matter():
     """Every byte behind the last entry set, scales to NaN among them."""
     outs = []
