@@ -20,7 +20,7 @@
 // 77 us, 5.0 TB/s) and by latency where there are few (64 x 16 heads of 64, 120..1000 entries: 39 MB in 13 us; one stream 5 us).
 // Many are bound by the instructions: matrix and vector instructions of a SIMD do not run beside each other (measured: a 16x16x32
 // product 17.6 clocks, an fma 2.5, an exp2 10, mixed ones the sum), so both count, and the products stand in blocks, each change
-// from one kind to the other costing about 5 clocks.  2 x 4095 rows x 32 heads on 8 of 128: 347 GFLOP in 388 us, 0.9 PFLOP/s.
+// from one kind to the other costing about 5 clocks.  2 x 4095 rows x 32 heads on 8 of 128: 346 GFLOP in 348 us, 1.0 PFLOP/s.
 #include "kv4_common.h"
 
 #include <type_traits>
@@ -55,6 +55,8 @@ struct Kv4Attn {
     f32x2* norm;                  // m and 1 / l of each column, where scores are formed again
     uint8_t* frags;               // the queries of each tile as the product takes them: [hd / 32][64 lanes][16 bytes]
     int slots;                    // tiles of a key head that these have room for
+    uint8_t* images;              // [sequence][key head][pages]: pages as bf16 fragments, K's then V's; or null
+    int pages;
     float* scores;                // [sequence][key head][room]: raw scores [column][kv4_kept_width], or null
     int64_t room;
     // row of a column: col / group without a division (exact below 2^26, and there are at most 2^22 columns)
@@ -528,7 +530,7 @@ __global__ __launch_bounds__(256) void kv4_attn_join_kernel(Kv4View c, Kv4Rows b
 // wave will read them, while the products of the page before run from the other half of the buffer: one barrier a page.
 // For bf16 rows P is rounded to bf16: each probability is off by at most 2^-8 of itself, independently, which adds an error of the
 // size of the output's own rounding (at most 1.42 times it in all, measured over flat to sharp scores) and halves the second
-// product (4095 rows x 32 heads: 386 us against 476 with hi + lo parts).  For fp16 rows P is hi + lo.
+// product (2 x 4095 rows x 32 heads of 128: 386 us against 476 with hi + lo parts, pages converted by each workgroup).  For fp16 rows P is hi + lo.
 // ------------------------------------------------------------------------------------------------------------------
 template <int HD> struct Kv4Stage {
     u32x4 k, v;                                                   // at hd 64 a wave's part of K is 8 bytes
@@ -605,6 +607,35 @@ template <int FRAGMENTS, int PRODUCTS> __device__ __forceinline__ void kv4_inter
     }
 }
 
+// Where many workgroups look at each page it is converted once for all of them: a launch before leaves the pages' fragments in memory as
+// they stand in LDS, where loads without a register on the way bring them (2 x 4095 rows x 32 heads of 128 384 us -> 348, of them 12 the
+// conversion; through registers 354).
+template <int HD> __device__ __forceinline__ uint8_t* kv4_image(const Kv4Attn& a, int Hkv, int seq, int h, int p) {
+    return a.images + (((int64_t)seq * Hkv + h) * a.pages + p) * (256 * HD);
+}
+// wave w's quarter: half of K's or of V's fragments, 1 KiB a load
+template <int HD> __device__ __forceinline__ void kv4_image_to_lds(const uint8_t* from, uint8_t* k, uint8_t* v, int w, int lane) {
+    uint8_t* to = (w < 2 ? k : v) + (w & 1) * (HD * 64);
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i)
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + (w * (HD / 16) + i) * 1024 + lane * 16),
+                                         (__attribute__((address_space(3))) void*)(to + i * 1024), 16, 0, 0);
+}
+template <int HD>
+__global__ __launch_bounds__(256) void kv4_image_kernel(Kv4View c, Kv4Rows b, Kv4Attn a) {
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), p = blockIdx.x / c.Hkv, h = blockIdx.x - p * c.Hkv;
+    const Kv4Seq s = kv4_seq_of(b, c, blockIdx.y);
+    const int rows = s.n < b.max_rows ? s.n : b.max_rows;
+    if (s.state || rows * a.group <= KV4_FEW_COLUMNS || p * KV4_PAGE >= s.ctx) return;
+    const int id = __builtin_amdgcn_readfirstlane(c.table[(int64_t)s.stream * c.max_pages + p]);
+    uint8_t* to = kv4_image<HD>(a, c.Hkv, blockIdx.y, h, p);
+    Kv4Stage<HD> stage;
+    stage.load_k(c, id, h, w, lane);
+    stage.load_v(c, id, h, w, lane);
+    stage.store_k(to, w, lane);
+    stage.store_v(to + 128 * HD, s.ctx - p * KV4_PAGE, w, lane);
+}
+
 // S^T of a page from its fragments in LDS
 template <int HD, bool F16, int NC>
 __device__ __forceinline__ void kv4_lds_scores(const uint8_t* kbuf, const Kv4Query<HD, F16> (&q)[NC], f32x4 (&s)[NC][4], int lane) {
@@ -644,7 +675,7 @@ __device__ __forceinline__ void kv4_lds_values(const uint8_t* vbuf, const bf16x8
 
 template <int HD> struct Kv4ManyLds { __attribute__((aligned(16))) uint8_t k[2][128 * HD], v[2][128 * HD]; };
 
-template <int HD, bool F16, int NC>
+template <int HD, bool F16, int NC, bool IMAGES>
 __device__ __forceinline__ void kv4_many_block(const Kv4View& c, const Kv4Rows& b, const Kv4Attn& a, Kv4ManyLds<HD>& lds, int h, int turn, int seq) {
     uint8_t (&kbuf)[2][128 * HD] = lds.k;
     uint8_t (&vbuf)[2][128 * HD] = lds.v;
@@ -679,21 +710,32 @@ __device__ __forceinline__ void kv4_many_block(const Kv4View& c, const Kv4Rows& 
     const int pages = all > 0 ? (all + KV4_PAGE - 1) / KV4_PAGE : 0;
     const int mine = most > 0 ? (most + KV4_PAGE - 1) / KV4_PAGE : 0;        // pages that the wave looks at
     const auto page_id = [&](int p) { return __builtin_amdgcn_readfirstlane(bt[p < pages ? p : pages - 1]); };
+    // a page on its way to its half of the buffer: load() sets out, store() is done when it has arrived
     Kv4Stage<HD> stage;
-    if (pages > 0) {
-        stage.load_k(c, page_id(0), h, w, lane);
-        stage.load_v(c, page_id(0), h, w, lane);
-        stage.store_k(kbuf[0], w, lane);
-        stage.store_v(vbuf[0], s.ctx, w, lane);
-    }
-    int id = pages > 0 ? page_id(1) : 0;
+    int id = pages > 0 && !IMAGES ? page_id(0) : 0;
+    const auto load = [&](int p) {
+        if constexpr (IMAGES) {
+            if (p < pages) kv4_image_to_lds<HD>(kv4_image<HD>(a, c.Hkv, seq, h, p), kbuf[p & 1], vbuf[p & 1], w, lane);
+        } else {
+            stage.load_k(c, id, h, w, lane);
+            stage.load_v(c, id, h, w, lane);
+            id = page_id(p + 1);
+        }
+    };
+    const auto store = [&](int p) {
+        if constexpr (IMAGES) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        } else {
+            stage.store_k(kbuf[p & 1], w, lane);
+            stage.store_v(vbuf[p & 1], s.ctx - p * KV4_PAGE, w, lane);
+        }
+    };
+    if (pages > 0) { load(0); store(0); }
     __syncthreads();
     int p = 0;
     for (; p < mine; ++p) {
         const int first = p * KV4_PAGE;
-        stage.load_k(c, id, h, w, lane);
-        stage.load_v(c, id, h, w, lane);
-        id = page_id(p + 2);
+        load(p + 1);
         f32x4 sc[NC][4];
         bf16x8 ph[NC][2], pl[NC][2];
         kv4_lds_scores<HD, F16, NC>(kbuf[p & 1], q, sc, lane);
@@ -709,17 +751,13 @@ __device__ __forceinline__ void kv4_many_block(const Kv4View& c, const Kv4Rows& 
         kv4_lds_values<HD, F16, NC>(vbuf[p & 1], ph, pl, st, lane);
         kv4_interleave<HD / 8, NC * (F16 ? 2 : 1)>();
         __builtin_amdgcn_sched_barrier(0);
-        stage.store_k(kbuf[(p + 1) & 1], w, lane);
-        stage.store_v(vbuf[(p + 1) & 1], s.ctx - first - KV4_PAGE, w, lane);
+        store(p + 1);
         __syncthreads();
     }
     // pages that only later waves of the workgroup see
     for (; p < pages; ++p) {
-        stage.load_k(c, id, h, w, lane);
-        stage.load_v(c, id, h, w, lane);
-        id = page_id(p + 2);
-        stage.store_k(kbuf[(p + 1) & 1], w, lane);
-        stage.store_v(vbuf[(p + 1) & 1], s.ctx - (p + 1) * KV4_PAGE, w, lane);
+        load(p + 1);
+        store(p + 1);
         __syncthreads();
     }
 #pragma unroll
@@ -743,7 +781,7 @@ __device__ __forceinline__ void kv4_many_block(const Kv4View& c, const Kv4Rows& 
 }
 
 // Both in one launch, for a batch that may hold sequences of either kind: the long blocks start first.
-template <int HD, bool F16, int NC>
+template <int HD, bool F16, int NC, bool IMAGES>
 __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_mixed_kernel(Kv4View c, Kv4Rows b, Kv4Attn a, int turns) {
     __shared__ union { Kv4ManyLds<HD> many; Kv4FewLds<HD> few; } lds;
     const unsigned many = (unsigned)c.Hkv * turns * b.n_seqs;
@@ -751,7 +789,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_mixed_kernel(K
     if (x < many) {
         const int h = x % c.Hkv;
         x /= c.Hkv;
-        kv4_many_block<HD, F16, NC>(c, b, a, lds.many, h, x % turns, x / turns);
+        kv4_many_block<HD, F16, NC, IMAGES>(c, b, a, lds.many, h, x % turns, x / turns);
     } else {
         x -= many;
         const int h = x % c.Hkv;
@@ -981,8 +1019,12 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_kernel(Kv4View c, Kv4Rows 
 // ------------------------------------------------------------------------------------------------------------------
 // Entry points
 // ------------------------------------------------------------------------------------------------------------------
-// the work buffer: chunks' O | their m and l | kept scores | m and 1 / l | queries
-struct Kv4Work { int64_t states, ml, scores, norm, frags, room; int tiles, chunks, slots; };
+// the work buffer: chunks' O | their m and l | kept scores | m and 1 / l | queries | converted pages
+struct Kv4Work { int64_t states, ml, scores, norm, frags, images, room; int tiles, chunks, slots, pages; };
+// Pages are converted by a launch of their own from this many columns on (6 x 513 rows x 16 heads of 64 18.0 us, so 18.4; 4 x 1000 34.3 and
+// 28.9; 64 x 100 41 and 60), unless they need more than this many bytes
+#define KV4_IMAGE_COLUMNS 768
+#define KV4_IMAGE_BYTES (1ll << 29)
 static Kv4Work plan_work(const t3_kv4_cache* c, const t3_kv4_batch* b, int H, bool weights) {
     Kv4Work w{};
     const int64_t cols = (int64_t)b->max_rows * (H / c->Hkv), few = cols < KV4_FEW_COLUMNS ? cols : KV4_FEW_COLUMNS;
@@ -1004,6 +1046,9 @@ static Kv4Work plan_work(const t3_kv4_cache* c, const t3_kv4_batch* b, int H, bo
             w.ml = parts * 8;
         }
     }
+    w.pages = (int)((most + KV4_PAGE - 1) / KV4_PAGE);
+    w.images = pairs * w.pages * 256 * c->hd;
+    if (cols < KV4_IMAGE_COLUMNS || cols <= few || w.images > KV4_IMAGE_BYTES) w.images = 0;
     return w;
 }
 static int check_sizes(const t3_kv4_cache* c, const t3_kv4_batch* b, int H) {
@@ -1015,7 +1060,7 @@ static int check_sizes(const t3_kv4_cache* c, const t3_kv4_batch* b, int H) {
 extern "C" int64_t t3_op_attn_kv4_work_bytes(const t3_kv4_cache* cache, const t3_kv4_batch* batch, int32_t H, int32_t with_weights) {
     if (kv4_check_cache(cache, 0, 1, nullptr) || kv4_check_batch(batch) || check_sizes(cache, batch, H)) return -1;
     const Kv4Work w = plan_work(cache, batch, H, with_weights != 0);
-    return w.states + w.ml + w.scores + w.norm + w.frags;
+    return w.states + w.ml + w.scores + w.norm + w.frags + w.images;
 }
 
 template <int HD, bool F16>
@@ -1031,7 +1076,12 @@ static int launch_attn(const Kv4View& c, const Kv4Rows& b, const Kv4Attn& a, flo
     } else {
         const int64_t turns = (cols + 64 * NC - 1) / (64 * NC), blocks = c.Hkv * (int64_t)b.n_seqs * (turns + (int64_t)a.tiles * a.chunks);
         T3_REQUIRE(blocks <= INT32_MAX, "attn_kv4: too many sequences of that many rows in one call");
-        T3_LAUNCH((kv4_attn_mixed_kernel<HD, F16, NC>), dim3((unsigned)blocks), dim3(256), 0, st, c, b, a, (int)turns);
+        if (a.images) {
+            T3_LAUNCH(kv4_image_kernel<HD>, dim3(a.pages * c.Hkv, b.n_seqs), dim3(256), 0, st, c, b, a);
+            T3_LAUNCH((kv4_attn_mixed_kernel<HD, F16, NC, true>), dim3((unsigned)blocks), dim3(256), 0, st, c, b, a, (int)turns);
+        } else {
+            T3_LAUNCH((kv4_attn_mixed_kernel<HD, F16, NC, false>), dim3((unsigned)blocks), dim3(256), 0, st, c, b, a, (int)turns);
+        }
     }
     const int joins = a.chunks > 1 ? (cols < KV4_FEW_COLUMNS ? (int)cols : KV4_FEW_COLUMNS) * c.Hkv : 0;
     const int64_t cap = (int64_t)c.max_pages * KV4_PAGE, most = b.max_ctx < cap ? b.max_ctx : cap;
@@ -1088,6 +1138,9 @@ extern "C" int t3_op_attn_kv4(const t3_kv4_cache* cache, const t3_kv4_batch* bat
     work += w.scores;
     a.norm = w.norm ? reinterpret_cast<f32x2*>(work) : nullptr;
     a.frags = w.frags ? work + w.norm : nullptr;
+    work += w.norm + w.frags;
+    a.images = w.images ? work : nullptr;
+    a.pages = w.pages;
     a.slots = w.slots;
     const Kv4View c = kv4_view(cache, layer);
     const Kv4Rows b = kv4_rows(batch);

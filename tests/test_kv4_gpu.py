@@ -181,6 +181,32 @@ def test_prompts(hd, kv, group, rows, ctx, dtype, with_weights):
     check_attend(m, device_cache(m), rows, ctx, group, dtype, with_weights)
 
 
+@pytest.mark.parametrize("hd,group,rows,ctx", [(64, 3, [300, 5, 130, 21], [300, 1400, 191, 21]), (128, 8, [130, 90, 1, 100], [333, 90, 2000, 164])])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_prompts_with_pages_converted_beforehand(hd, group, rows, ctx, dtype):
+    """Batches of long prompts convert their pages in a launch of their own; a prompt alone, or bounds for which that would take too
+    much memory, do not.  All give the same bits."""
+    m = _kv4.Model(hd, 2, 1, 4 * 32, 4, 32, seed=31)
+    for i, t in enumerate(ctx):
+        m.fill(i, t)
+    cache = device_cache(m)
+    q, out, w = check_attend(m, cache, rows, ctx, group, dtype, True)
+    s = starts(rows)
+    for i in range(4):
+        alone = cache.attend(q[s[i]:s[i + 1]].to(DEV), cache.batch(i32([0, rows[i]]), i32([i]), i32([ctx[i]]), rows=rows[i]))
+        assert torch.equal(alone, out[s[i]:s[i + 1]]), i
+    wide = torch.full((4, 1 << 15), -1, dtype=torch.int32, device=DEV)
+    wide[:, :32] = cache.block_table
+    loose = KV4Cache(2, hd, pool=cache.pool, block_table=wide)
+    assert torch.equal(loose.attend(q.to(DEV), loose.batch(i32(s), i32([0, 1, 2, 3]), i32(ctx), rows=sum(rows))), out)
+    # a page that there is not, inside one prompt and behind another's entries
+    cache.block_table[0, 2] = -1
+    cache.block_table[1, ctx[1] // 64 + 1:] = 4 * 32
+    bad = cache.attend(q.to(DEV), cache.batch(i32(s), i32([0, 1, 2, 3]), i32(ctx), rows=sum(rows), max_rows=max(rows), max_ctx=max(ctx)))
+    first = max(0, 128 - (ctx[0] - rows[0]))                       # the first row that sees the page
+    assert torch.isnan(bad[first:rows[0]]).all() and torch.equal(bad[:first], out[:first]) and torch.equal(bad[rows[0]:], out[rows[0]:])
+
+
 @pytest.mark.parametrize("rows", [[1, 1, 1, 1], [4, 1, 2, 3], [90, 1, 200, 7]])
 def test_rows_do_not_depend_on_the_batch(rows):
     ctx = [700, 65, 1500, 33]
