@@ -217,6 +217,11 @@ __device__ __forceinline__ float kv4_group_sum(float x) {
     const auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
+// over the 16 lanes of a group: neighbours, pairs, quads, eights (each step's operands are equal in the lanes that hold them)
+template <int CTRL> __device__ __forceinline__ float kv4_lane_add(float x) {
+    return x + __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float kv4_row_sum(float x) { return kv4_lane_add<0x140>(kv4_lane_add<0x141>(kv4_lane_add<0x4e>(kv4_lane_add<0xb1>(x)))); }
 // two values as bf16 hi and lo parts, one word each
 __device__ __forceinline__ void kv4_split(float p0, float p1, unsigned& hi, unsigned& lo) {
     typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
@@ -804,8 +809,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_mixed_kernel(K
 // Weights: W[stream][key head][t] += sum over the sequence's columns of exp2(s c - m) / l.  A workgroup owns its entries and walks the
 // columns in a fixed order, so there are no atomics.  Scores of sequences of few columns were kept by the pass above (64 decode rows x
 // 16 heads of 64 over up to 2000 entries 55 us -> 37, 32 x 64 heads on 8 of 128 over up to 8000 122 -> 74; 40 columns 37 -> 28); the
-// others are formed again from K, from queries that the pass above leaves in operand order (2 x 4095 rows x 32 heads of 128: 300 us
-// beside the pass's 388; from the rows as given 380, by one wave a page 1170).
+// others are formed again from K, from queries that the pass above leaves in operand order (2 x 4095 rows x 32 heads of 128: 280 us
+// beside the pass's 349; from the rows as given 380, by one wave a page 1170).
 // A stream that occurs in several sequences of the call is done, in their order, by the waves of the first of them.
 // ------------------------------------------------------------------------------------------------------------------
 // Walks the sequences of the stream of sequence `seq` if that is the first of them, 64 looked at at a time: fn(their numbers).
@@ -998,11 +1003,8 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_kernel(Kv4View c, Kv4Rows 
         // over the 16 columns; lane r of a group takes token 16 g + r
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            sum[e] += __shfl_xor(sum[e], 1);
-            sum[e] += __shfl_xor(sum[e], 2);
-            sum[e] += __shfl_xor(sum[e], 4);
-            sum[e] += __shfl_xor(sum[e], 8);
-            mine += (lane & 15) == e ? sum[e] : 0.f;
+            const float all = kv4_row_sum(sum[e]);
+            mine += (lane & 15) == e ? all : 0.f;
         }
     });
     if (!own) return;                                             // the same in all waves
