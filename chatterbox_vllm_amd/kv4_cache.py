@@ -20,7 +20,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
-from torch._C import _cuda_getCurrentRawStream as _raw_stream    # the handle alone: a Stream object costs 2 us a call
+from torch._C import _cuda_getCurrentRawStream as _raw_stream, _cuda_getDevice as _current_device    # (a Stream object costs 2 us a call)
 
 from . import _capi
 
@@ -186,7 +186,7 @@ class KV4Cache:
 
     # -- checks ------------------------------------------------------------------------------------------------------
     def _run(self, fn, *args) -> None:
-        if torch.cuda.current_device() != self._index:
+        if _current_device() != self._index:
             with torch.cuda.device(self._index):
                 return self._run(fn, *args)
         status = fn(*args, _raw_stream(self._index))
