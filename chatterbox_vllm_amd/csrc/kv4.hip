@@ -139,8 +139,10 @@ template <bool F16> __device__ __forceinline__ u32x4 kv4_values8(unsigned codes,
         // a value appended from fp16 can stand for up to 6 * 2^14: cut at the type's largest instead of becoming infinite
         const f16x2 most = {(_Float16)65504.f, (_Float16)65504.f};
         const float sc = kv4_scale(byte);
-        f16x2 p[4] = {__builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, sc, 0)), __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, sc, 1)),
-                      __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, sc, 2)), __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, sc, 3))};
+        const f16x2 p[4] = {__builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, sc, 0)),
+                            __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, sc, 1)),
+                            __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, sc, 2)),
+                            __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, sc, 3))};
         u32x4 o;
 #pragma unroll
         for (int i = 0; i < 4; ++i)

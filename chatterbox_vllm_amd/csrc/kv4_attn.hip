@@ -37,9 +37,7 @@
 KV4_FN int kv4_chunks(int ctx) { return (int)(((int64_t)ctx + KV4_CHUNK_PAGES * KV4_PAGE - 1) / (KV4_CHUNK_PAGES * KV4_PAGE)); }
 
 // Where weights are wanted, the scores of a (sequence, key head) of few columns are kept if they are at most KV4_KEEP values (4 MiB).
-#ifndef KV4_KEEP
 #define KV4_KEEP (1 << 20)
-#endif
 KV4_FN int64_t kv4_kept_width(int64_t ctx) { return (ctx + KV4_PAGE - 1) / KV4_PAGE * KV4_PAGE; }
 KV4_FN bool kv4_kept(int cols, int ctx) { return cols <= KV4_FEW_COLUMNS && cols * kv4_kept_width(ctx) <= KV4_KEEP; }
 

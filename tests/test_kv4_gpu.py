@@ -395,6 +395,27 @@ def test_rows_beyond_what_one_launch_has_workgroups_for(hd):
         assert ((got[0][i:i + 1000].float() - k[i:i + 1000].float()).abs() <= k[i:i + 1000].float().abs().amax(-1, keepdim=True) / 3.5).all()   # half a step
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows", [[1, 2], [100, 1], [900, 70]])
+def test_empty_streams(hd, rows):
+    """Streams without entries: nothing is stored, rows get 0, no weight is added, and the sequence beside them is as it is alone."""
+    m = _kv4.Model(hd, 1, 1, 60, 3, 20, seed=33)
+    m.fill(2, 1000)
+    cache = device_cache(m)
+    R = sum(rows) + 80
+    x = torch.randn(R, 1, hd, generator=torch.Generator().manual_seed(34)).to(torch.bfloat16).to(DEV)
+    batch = cache.batch(i32(starts(rows + [80])), i32([0, 1, 2]), i32([0, 0, 1000]), rows=R, max_rows=max(max(rows), 80))
+    pool = cache.pool.clone()
+    w, w2 = cache.new_weights()[0], cache.new_weights()[0]
+    out = cache.attend(x, batch, weights=w)
+    alone = cache.attend(x[-80:], cache.batch(i32([0, 80]), i32([2]), i32([1000]), rows=80), weights=w2)
+    assert (out[:-80] == 0).all() and torch.equal(out[-80:], alone) and (w[:2] == 0).all()
+    assert torch.equal(w[2] != 0, w2[2] != 0)
+    cache.append(x[:-80], x[:-80], cache.batch(i32(starts(rows)), i32([0, 1]), i32([0, 0]), rows=R - 80))
+    k, v = cache.read(cache.batch(i32(starts(rows)), i32([0, 1]), i32([0, 0]), rows=R - 80))
+    assert torch.equal(cache.pool, pool) and (k == 0).all() and (v == 0).all()
+
+
 @pytest.mark.parametrize("hd,rows,ctx", [(64, [1, 5, 3], [40, 2000, 3]), (128, [200, 1, 70], [200, 3000, 500])])
 def test_out_may_be_q(hd, rows, ctx):
     m = _kv4.Model(hd, 2, 1, 3 * 47, 3, 47, seed=26)
