@@ -660,12 +660,14 @@ template <int HD> static void kv4_evict_launch(const Kv4View& c, const Kv4Evict&
     const dim3 grid(c.Hkv, e.n, layers);
     // Pages moved by the workgroup that chose them, up to 2048 entries: 4 streams of 2000 x 16 heads of 64 10.5 us, 8 streams x 30 layers
     // 158; moved by a launch of their own 12.3 and 209.  Above, few workgroups would move many pages: one stream of 8000 to 6000 x 8 heads
-    // of 128 17 us, moved by those that chose 71.  Above 8192 the weights are not held: 4 streams of 8000 18.5 us held, 36.9 not.
+    // of 128 17 us, moved by those that chose 71.  Above 16384 the weights are not held: 4 streams of 8000 18.5 us held, 36.9 not; of
+    // 16000 32 and 67.
     if (e.max_ctx <= 2048) {
         T3_LAUNCH((kv4_evict_kernel<HD, 256, 8, true>), grid, dim3(256), 0, st, c, e, layer_stride);
         return;
     }
     if (e.max_ctx <= 8192) T3_LAUNCH((kv4_evict_kernel<HD, 1024, 8, false>), grid, dim3(1024), 0, st, c, e, layer_stride);
+    else if (e.max_ctx <= 16384) T3_LAUNCH((kv4_evict_kernel<HD, 1024, 16, false>), grid, dim3(1024), 0, st, c, e, layer_stride);
     else T3_LAUNCH(kv4_choose_kernel, grid, dim3(KV4_CHOOSE_THREADS), 0, st, c, e);
     const int most = e.keep < e.max_ctx ? e.keep : e.max_ctx;
     T3_LAUNCH(kv4_move_kernel<HD>, dim3((most + 4 * KV4_PAGE - 1) / (4 * KV4_PAGE), c.Hkv * e.n, layers), dim3(256), 0, st, c, e, layer_stride);

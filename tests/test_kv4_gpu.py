@@ -513,7 +513,8 @@ def test_evict_long_and_nan_entries():
     assert torch.isnan(cache.read(cache.batch(i32([0, 5]), i32([1]), i32([5]), rows=5))[0][3, 1]).all()
 
 
-@pytest.mark.parametrize("pages,ctx", [(32, [2048, 2047, 1025, 64, 513, 1, 0]), (33, [2049, 2048, 300]), (128, [8192, 8191, 4097, 640]), (129, [8193, 130])])
+@pytest.mark.parametrize("pages,ctx", [(32, [2048, 2047, 1025, 64, 513, 1, 0]), (33, [2049, 2048, 300]), (128, [8192, 8191, 4097, 640]), (129, [8193, 130]),
+                                       (256, [16384, 9001]), (257, [16385, 700])])
 @pytest.mark.parametrize("keep,sink,recent", [(500, 34, 100), (1, 0, 0), (1500, 0, 0), (1024, 1000, 24)])
 def test_evict_at_every_length(pages, ctx, keep, sink, recent):
     """The choice for entries up to and past each number that the threads of a workgroup hold: weights that differ everywhere, in one
