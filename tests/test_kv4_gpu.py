@@ -375,6 +375,15 @@ def test_weights_of_few_columns_over_many_chunks(hd, group):
     assert torch.equal(wide[..., :2501], odd)
 
 
+@pytest.mark.parametrize("hd,group,rows,ctx,streams", [(64, 64, [1, 1, 1], [17000, 900, 16500], [0, 1, 0]), (128, 32, [2, 1, 40], [16400, 16400, 700], [1, 1, 0])])
+def test_weights_of_more_scores_than_are_kept(hd, group, rows, ctx, streams):
+    """Few columns over contexts whose scores are formed again, beside ones whose scores are kept, of one stream too."""
+    m = _kv4.Model(hd, 1, 1, 2 * 266, 2, 266, seed=35)
+    for i in range(2):
+        m.fill(i, max(t for t, x in zip(ctx, streams) if x == i))
+    check_attend(m, device_cache(m), rows, ctx, group, "bf16", True, streams=streams)
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 def test_rows_beyond_what_one_launch_has_workgroups_for(hd):
     """270000 rows of one sequence at once give the bytes that they give a thousand at a time, and come back."""
