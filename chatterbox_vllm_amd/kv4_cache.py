@@ -130,7 +130,7 @@ class KV4Cache:
         w_ptr, w_stride = None, 0
         if weights is not None:
             self._weights(weights, 3)
-            w_ptr, w_stride = weights.data_ptr(), weights.stride(1)
+            w_ptr, w_stride = weights.data_ptr(), weights.shape[2]       # (a contiguous tensor's stride of a single head may be any)
         size = batch._work.get(heads if weights is None else -heads)
         if size is None:
             size = self._lib.t3_op_attn_kv4_work_bytes(self._ref, batch._ref, heads, int(weights is not None))

@@ -10,6 +10,7 @@ import torch
 
 import _kv4
 from chatterbox_vllm_amd import _capi
+from chatterbox_vllm_amd.kv4_cache import KV4Cache
 
 ROOT = os.path.abspath(os.path.join(os.path.dirname(__file__), ".."))
 CSRC = os.path.join(ROOT, "chatterbox_vllm_amd", "csrc")
@@ -233,3 +234,37 @@ def test_sizes():
     assert lib.t3_op_attn_kv4_work_bytes(c, b, 16, 1) >= 6 * 16 * 8
     c = C.byref(_cache(max_pages=1 << 20))
     assert lib.t3_op_attn_kv4_work_bytes(c, C.byref(_batch(max_ctx=40000)), 16, 0) > 0
+
+
+class HostCache(KV4Cache):
+    """A cache whose tensors lie on the host and whose calls are written down instead of made."""
+
+    def __init__(self, kv, hd, streams, max_pages, pages=8):
+        self._lib, self.device, self._index, self._scale, self.calls = _capi.load(), torch.device("cpu"), -1, hd ** -0.5, []
+        self.num_kv_heads, self.head_dim, self.num_layers, self.num_pages, self.num_streams, self.max_pages = kv, hd, 1, pages, streams, max_pages
+        self._c = _cache(n_layers=1, n_pages=pages, n_streams=streams, max_pages=max_pages, Hkv=kv, hd=hd)
+        self._ref = C.byref(self._c)
+
+    def _run(self, fn, *args):
+        self.calls.append(args)
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("weights", [lambda: torch.zeros(5, 1, 128), lambda: torch.zeros(1, 5, 128).transpose(0, 1),
+                                     lambda: torch.zeros(5, 128)[:, None], lambda: torch.zeros(5, 128).as_strided((5, 1, 128), (128, 7, 1))])
+def test_a_row_of_weights_is_as_long_as_its_entries(weights):
+    """Contiguous tensors of one key head, whose stride along it is any number: stream s lies at s * 128."""
+    cache, w = HostCache(1, 64, 5, 2), weights()
+    assert w.is_contiguous() and w.shape == (5, 1, 128)
+    cache.attend(torch.zeros(1, 2, 64, dtype=torch.bfloat16), cache.batch(i32([0, 1]), i32([4]), i32([100]), rows=1), weights=w)
+    assert cache.calls[0][9] == w.data_ptr() and cache.calls[0][10] == 128
+
+
+def test_a_narrow_row_of_weights_is_no_longer_than_it_is():
+    cache, w = HostCache(1, 64, 1, 4), torch.zeros(1, 1, 200)[..., :100]
+    assert w.is_contiguous() and w.stride(1) == 200
+    cache.attend(torch.zeros(1, 2, 64, dtype=torch.bfloat16), cache.batch(i32([0, 1]), i32([0]), i32([100]), rows=1, max_ctx=100), weights=w)
+    assert cache.calls[0][10] == 100                             # the library refuses max_ctx past it

@@ -346,6 +346,30 @@ def test_numbers_that_do_not_fit_give_nan_and_store_nothing():
     assert (out == 7).all()
 
 
+@pytest.mark.parametrize("layout", ["transposed", "view", "narrow"])
+def test_weights_of_one_key_head_in_any_contiguous_layout(layout):
+    """The stride along a single key head is any number: rows go where the tensor has them, what lies around it stays."""
+    m = _kv4.Model(64, 1, 1, 15, 3, 5, seed=36)
+    for i, t in enumerate((300, 70, 150)):
+        m.fill(i, t)
+    cache = device_cache(m)
+    q = torch.randn(3, 2, 64, generator=torch.Generator().manual_seed(37)).to(torch.bfloat16).to(DEV)
+    memory = torch.zeros(4 * 3 * 320, device=DEV)
+    w = {"transposed": lambda: memory[:960].view(1, 3, 320).transpose(0, 1), "view": lambda: memory[:960].view(3, 320)[:, None],
+         "narrow": lambda: memory[:640].view(1, 1, 640)[..., :320]}[layout]()
+    if layout == "narrow":                                       # one stream; a bound past the row is refused
+        one = KV4Cache(1, 64, pool=cache.pool, block_table=cache.block_table[:1].contiguous())
+        with pytest.raises(_capi.T3Error, match="weights_stride"):
+            one.attend(q[:1], one.batch(i32([0, 1]), i32([0]), i32([300]), rows=1, max_ctx=320), weights=memory[:640].view(1, 1, 640)[..., :300])
+        batch = one.batch(i32([0, 1]), i32([0]), i32([300]), rows=1)
+        cache, q = one, q[:1]
+    else:
+        batch = cache.batch(i32([0, 1, 2, 3]), i32([0, 1, 2]), i32([300, 70, 150]), rows=3, max_rows=1)
+    want = cache.new_weights()[0]
+    assert w.is_contiguous() and torch.equal(cache.attend(q, batch, weights=w), cache.attend(q, batch, weights=want))
+    assert torch.equal(w, want) and (w[:, 0, 0] > 0).all() and (memory[w.numel():] == 0).all()
+
+
 def test_weights_of_a_stream_that_occurs_twice():
     """Two sequences of one stream (two drafts, say) are added in their order; equal calls give equal bits."""
     m = _kv4.Model(64, 2, 1, 20, 4, 5, seed=13)
