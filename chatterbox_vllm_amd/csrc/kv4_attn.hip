@@ -8,9 +8,11 @@
 // column, which is what the second takes from it: no exchange but the maximum over the four lane groups.
 // fp16 queries enter as bf16 hi + lo (exact to 2^-16 of the value, fp16 has 11 bits), so one set of products serves both types.
 //
-//   p = exp2(s c - m),  c = scale log2(e),  m the running maximum of s c as rounded, l the running sum:  one pass, fp32.
-// m follows the maximum in jumps: it stays while the maximum is at most 2^8 above it (p <= 2^8 costs fp32 and bf16 nothing), so the
-// sums are rarely rescaled.  Keeping m as the rounded product makes the factors between pages and chunks, exp2(m - m'), consistent at any size of s.
+//   p = exp2((s - m) c),  c = scale log2(e),  m the running maximum of the scores themselves, l the running sum:  one pass, fp32.
+// m follows the maximum in jumps: it stays while p is at most 2^8 (which costs fp32 and bf16 nothing), so the sums are rarely rescaled.
+// The difference is taken before the product: it is exact near the maximum, whose p is then at least 1 at any size of s, and the factors
+// between pages and chunks, exp2((m - m') c), agree with it.  (One fma(s, c, -m c) would leave the maximum the rounding of m c, which from
+// m c = 2^31 on is more than all of fp32's exponents.)
 //
 // Sequences of at most KV4_FEW_COLUMNS columns (decode steps, drafted tokens) are cut into chunks of their cache, a workgroup of
 // four waves each; a second launch joins the chunks in order.  Longer ones (prompts) run whole: a wave keeps one or two column tiles and
@@ -27,7 +29,9 @@
 
 #define KV4_FEW_COLUMNS 64        // rows x group up to which a sequence is cut along its cache
 #define KV4_SLACK 8.f             // the reference moves when a maximum passes it by 2^8
-#define KV4_NONE -3e38f           // running maximum before the first visible token (finite: differences of it stay numbers)
+#define KV4_NONE -3.402823466e38f // running maximum before the first visible token (the lowest finite: no score lies below, no difference of two is NaN)
+// 2^((s - m) c)
+__device__ __forceinline__ float kv4_exp(float s, float m, float c) { return __builtin_amdgcn_exp2f((s - m) * c); }
 
 // A chunk is 16 pages: the four waves of its workgroup take four each.  (8 waves: 64 x 16 heads of 64 over up to 1000 entries 13.2 -> 14.9 us,
 // 16 x 32 heads of 128 over up to 32k 77 -> 107; 32 pages: one sequence of 4k 13.5 -> 18.5, the long ones 76; 8 pages: 10 and 79, one of
@@ -236,10 +240,10 @@ template <int HD, int NC> __device__ __forceinline__ void kv4_reference(const f3
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) top = fmaxf(top, s[n][i][j]);
-        top = kv4_group_max(top) * c;
-        const float m = top > st.m[n] + KV4_SLACK ? top : st.m[n];
+        top = kv4_group_max(top);
+        const float m = (top - st.m[n]) * c > KV4_SLACK ? top : st.m[n];
         if (__any(m != st.m[n])) {                                // a column that keeps its reference multiplies by one
-            const float alpha = __builtin_amdgcn_exp2f(st.m[n] - m);
+            const float alpha = kv4_exp(st.m[n], m, c);
             st.m[n] = m;
             st.l[n] *= alpha;
 #pragma unroll
@@ -261,8 +265,8 @@ __device__ __forceinline__ void kv4_probabilities(const f32x4 (&s)[NC][4], Kv4St
 #pragma unroll
             for (int y = 0; y < 8; y += 2) {
                 const int e = 8 * x + y;                          // tokens 16 g + e, + e + 1
-                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[n][e & 3][e >> 2], c, -st.m[n]));
-                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[n][(e & 3) + 1][e >> 2], c, -st.m[n]));
+                const float p0 = kv4_exp(s[n][e & 3][e >> 2], st.m[n], c);
+                const float p1 = kv4_exp(s[n][(e & 3) + 1][e >> 2], st.m[n], c);
                 sum += p0 + p1;
                 unsigned h, l;
                 kv4_split(p0, p1, h, l);
@@ -439,7 +443,7 @@ __device__ __forceinline__ void kv4_few_block(const Kv4View& c, const Kv4Rows& b
         for (int e = 0; e < 8; ++e) o[e] = 0.f;
 #pragma unroll
         for (int x = 0; x < KV4_FEW_WAVES; ++x) {
-            const float f = __builtin_amdgcn_exp2f(sm[x][0][k] - M);
+            const float f = kv4_exp(sm[x][0][k], M, a.c);
             L = fmaf(sm[x][1][k], f, L);
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e] = fmaf(so[x][k][d + e], f, o[e]);
@@ -491,7 +495,7 @@ __device__ __forceinline__ void kv4_join_block(const Kv4View& c, const Kv4Rows& 
     for (int x = group; x < chunks; x += GROUPS) {
         const f32x2 part = ml[x];
         const f32x4 v = *reinterpret_cast<const f32x4*>(sp + (int64_t)x * (16 * HD));
-        const float top = fmaxf(M, part[0]), f0 = __builtin_amdgcn_exp2f(M - top), f1 = __builtin_amdgcn_exp2f(part[0] - top);
+        const float top = fmaxf(M, part[0]), f0 = kv4_exp(M, top, a.c), f1 = kv4_exp(part[0], top, a.c);
         L = fmaf(L, f0, part[1] * f1);
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = fmaf(o[e], f0, v[e] * f1);
@@ -508,7 +512,7 @@ __device__ __forceinline__ void kv4_join_block(const Kv4View& c, const Kv4Rows& 
     o = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int x = 0; x < GROUPS; ++x) {
-        const float f = __builtin_amdgcn_exp2f(lds.ml[x][0] - M);
+        const float f = kv4_exp(lds.ml[x][0], M, a.c);
         L = fmaf(lds.ml[x][1], f, L);
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = fmaf(lds.o[x][t][e], f, o[e]);
@@ -804,7 +808,7 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_mixed_kernel(K
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Weights: W[stream][key head][t] += sum over the sequence's columns of exp2(s c - m) / l.  A workgroup owns its entries and walks the
+// Weights: W[stream][key head][t] += sum over the sequence's columns of exp2((s - m) c) / l.  A workgroup owns its entries and walks the
 // columns in a fixed order, so there are no atomics.  Scores of sequences of few columns were kept by the pass above (64 decode rows x
 // 16 heads of 64 over up to 2000 entries 55 us -> 37, 32 x 64 heads on 8 of 128 over up to 8000 122 -> 74; 40 columns 37 -> 28); the
 // others are formed again from K, from queries that the pass above leaves in operand order (2 x 4095 rows x 32 heads of 128: 280 us
@@ -854,7 +858,7 @@ __device__ __forceinline__ void kv4_kept_block(const Kv4View& c, const Kv4Rows& 
             for (int x = tid & ((1 << log) - 1); x < chunks; x += 1 << log) {
                 const f32x2 part = ml[x];
                 const float top = fmaxf(M, part[0]);
-                L = fmaf(L, __builtin_amdgcn_exp2f(M - top), part[1] * __builtin_amdgcn_exp2f(part[0] - top));
+                L = fmaf(L, kv4_exp(M, top, a.c), part[1] * kv4_exp(part[0], top, a.c));
                 M = top;
             }
         }
@@ -864,7 +868,7 @@ __device__ __forceinline__ void kv4_kept_block(const Kv4View& c, const Kv4Rows& 
             M = KV4_NONE;
             L = 0.f;
             for (int x = tid << log; x < (tid + 1) << log; ++x) M = fmaxf(M, lds.part[x][0]);
-            for (int x = tid << log; x < (tid + 1) << log; ++x) L = fmaf(lds.part[x][1], __builtin_amdgcn_exp2f(lds.part[x][0] - M), L);
+            for (int x = tid << log; x < (tid + 1) << log; ++x) L = fmaf(lds.part[x][1], kv4_exp(lds.part[x][0], M, a.c), L);
             lds.norm[tid] = f32x2{M, L == 0.f ? 0.f : 1.0f / L};
         }
         __syncthreads();
@@ -878,7 +882,7 @@ __device__ __forceinline__ void kv4_kept_block(const Kv4View& c, const Kv4Rows& 
             const f32x4 x = *reinterpret_cast<const f32x4*>(sp + col * width);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float v = __builtin_amdgcn_exp2f(fmaf(x[e], a.c, -norm[0]));
+                const float v = kv4_exp(x[e], norm[0], a.c);
                 mine[e] += e < seen ? v * norm[1] : 0.f;
             }
         }
@@ -935,7 +939,7 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_kernel(Kv4View c, Kv4Rows 
             for (int col = w; col < cols; col += 4) {
                 const int j = a.row(col);
                 const f32x2 norm = a.norm[kv4_column(a, h, i, s) + col];
-                const float v = __builtin_amdgcn_exp2f(fmaf(sp[col * width], a.c, -norm[0]));
+                const float v = kv4_exp(sp[col * width], norm[0], a.c);
                 mine += first + lane < s.ctx - s.n + j + 1 ? v * norm[1] : 0.f;
             }
             return;
@@ -981,11 +985,11 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_kernel(Kv4View c, Kv4Rows 
             if (__all(seen >= 16)) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    sum[e] = fmaf(__builtin_amdgcn_exp2f(fmaf(sc[e & 3][e >> 2], a.c, -t.norm[0])), t.norm[1], sum[e]);
+                    sum[e] = fmaf(kv4_exp(sc[e & 3][e >> 2], t.norm[0], a.c), t.norm[1], sum[e]);
             } else {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const float v = __builtin_amdgcn_exp2f(fmaf(sc[e & 3][e >> 2], a.c, -t.norm[0]));
+                    const float v = kv4_exp(sc[e & 3][e >> 2], t.norm[0], a.c);
                     sum[e] = e < seen ? fmaf(v, t.norm[1], sum[e]) : sum[e];
                 }
             }

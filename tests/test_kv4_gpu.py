@@ -262,6 +262,70 @@ def test_scores_far_below_zero(hd, rows, ctx):
         assert ((out[j] - want).abs() <= v.abs().max() * 2.0 ** -8 * 1.01).all(), j
 
 
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("dtype,low,high", [("fp16", 3.3e4, 6.5e4), ("bf16", 2.0 ** 46, 2.0 ** 47)])
+@pytest.mark.parametrize("hd,group,rows,ctx", [(64, 2, [1, 3], [700, 2500]), (128, 1, [1, 1], [130, 1500]), (64, 1, [100, 70], [100, 300]), (128, 8, [120, 1], [200, 70]),
+                                               (64, 64, [1, 1], [16500, 300])])
+def test_large_scores(hd, group, rows, ctx, dtype, low, high, sign):
+    """Scores of one sign that are far from powers of two, from 1e10 on: the largest takes everything, equal ones share it.
+
+    q has at most 11 significant bits and k two, each within a factor of two: products and their sums over hd <= 128 dims take at most
+    2 + 11 + 1 + 2 + 7 < 24 bits, so the scores of 32 bits are exact, and two that differ do so by more than 10^4 after the scale.  What
+    is left are the last roundings: 1 / n and the sums of n equal terms (2^-22 covers them) and the output's own."""
+    n, H = len(rows), group
+    m = _kv4.Model(hd, 1, 1, n * 260 + 1, n, 260, seed=38)
+    g = torch.Generator().manual_seed(39)
+    for i, t in enumerate(ctx):
+        k = (low + (high - low) * torch.rand(t, 1, hd, generator=g)).to(DT[dtype]).float() * sign
+        k[t // 2:t // 2 + 2] = k[t // 2]                          # neighbours that are equal
+        m.put(m.pool, i, torch.arange(t), k, torch.randn(t, 1, hd, generator=g).to(torch.bfloat16))
+    q = (low + (high - low) * torch.rand(sum(rows), H, hd, generator=g)).to(DT[dtype])
+    cache, s = device_cache(m), starts(rows)
+    batch = cache.batch(i32(s), i32(list(range(n))), i32(ctx), rows=sum(rows), max_rows=max(rows), max_ctx=max(ctx))
+    w = cache.new_weights()[0]
+    plain, out = cache.attend(q.to(DEV), batch), cache.attend(q.to(DEV), batch, weights=w).cpu().double()
+    assert torch.equal(plain.cpu().double(), out)
+    half = torch.finfo(DT[dtype]).eps / 2
+    for i in range(n):
+        k, v = m.get(m.pool, i, torch.arange(ctx[i]))
+        ref, p, size, _ = _kv4.attend(q[s[i]:s[i + 1]].double(), k, v, ctx[i], hd ** -0.5)
+        tol = half * ref.abs() + size * 2.0 ** -22 + torch.finfo(DT[dtype]).smallest_normal
+        bad = ~((out[s[i]:s[i + 1]] - ref).abs() <= tol)
+        assert not bad.any(), f"sequence {i}: {int(bad.any(-1).sum())} of {bad[..., 0].numel()} columns"
+        assert ((w[i, :, :ctx[i]].cpu().double() - p).abs() <= p * 2.0 ** -22).all() and (w[i, :, ctx[i]:] == 0).all()
+
+
+@pytest.mark.parametrize("hd,group,rows,ctx", [(64, 1, 1, 2500), (128, 4, 2, 700), (64, 1, 130, 400), (128, 8, 120, 1100)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("offset", [0, 5 * 2.0 ** 10, 5 * 2.0 ** 15])
+def test_a_common_offset_of_the_scores_cancels(hd, group, rows, ctx, dtype, offset):
+    """Scores offset + x with x of a few units, x / 8 and offset whole numbers below 2^24: the same softmax as of x.
+
+    The scores of 32 bits are exact.  A difference of two of them is exact, its product with the scale off by 2^-23 of it at most, of
+    at most 64 units: each probability is off by 2^-16 and by what its rounding for the second product leaves (_kv4.out_bound)."""
+    m = _kv4.Model(hd, 1, 1, 41, 1, 40, seed=40)
+    g = torch.Generator().manual_seed(41)
+    k = torch.zeros(ctx, 1, hd)
+    k[:, 0, 0] = 2.0 ** 10 if offset else 0.0
+    k[:, 0, 32:40] = torch.randint(-2, 3, (ctx, 8), generator=g).float()
+    m.put(m.pool, 0, torch.arange(ctx), k, torch.randn(ctx, 1, hd, generator=g).to(torch.bfloat16))
+    q = torch.zeros(rows, group, hd)
+    q[..., 0] = offset / 2.0 ** 10
+    q[..., 32:40] = torch.randint(-3, 4, (rows, group, 8), generator=g).float()
+    q = q.to(DT[dtype])
+    cache = device_cache(m)
+    w = cache.new_weights()[0]
+    out = cache.attend(q.to(DEV), cache.batch(i32([0, rows]), i32([0]), i32([ctx]), rows=rows), weights=w).cpu().double()
+    kk, v = m.get(m.pool, 0, torch.arange(ctx))
+    assert torch.equal(kk, k.double())
+    ref, p, size, _ = _kv4.attend(q.double(), kk, v, ctx, hd ** -0.5)
+    half = torch.finfo(DT[dtype]).eps / 2
+    rounding = 2.0 ** -8 if dtype == "bf16" and rows * group > 64 else 2.0 ** -16
+    inner = size * (2.0 ** -15 + rounding + (ctx / 16 + 64) * 2.0 ** -24)
+    assert ((out - ref).abs() <= half * (ref.abs() + inner) + inner + torch.finfo(DT[dtype]).smallest_normal).all()
+    assert ((w[0, :, :ctx].cpu().double() - p).abs() <= p * (2.0 ** -15 + (ctx + rows * group) / 16 * 2.0 ** -24)).all()
+
+
 def test_what_lies_behind_the_last_entry_does_not_matter():
     """Every byte behind the last entry set, scales to NaN among them."""
     outs = []
