@@ -40,35 +40,49 @@ __device__ __forceinline__ float kv4_exp(float s, float m, float c) { return __b
 #define KV4_CHUNK_PAGES 16
 KV4_FN int kv4_chunks(int ctx) { return (int)(((int64_t)ctx + KV4_CHUNK_PAGES * KV4_PAGE - 1) / (KV4_CHUNK_PAGES * KV4_PAGE)); }
 
-// Where weights are wanted, the scores of a (sequence, key head) of few columns are kept if they are at most KV4_KEEP values (4 MiB).
+// Where weights are wanted, the scores of a (sequence, key head) of few columns are kept if they are at most `room` values: KV4_KEEP (4 MiB),
+// less where a call's would take more than KV4_KEEP_BYTES in all.
 #define KV4_KEEP (1 << 20)
+#define KV4_KEEP_BYTES (1ll << 29)
 KV4_FN int64_t kv4_kept_width(int64_t ctx) { return (ctx + KV4_PAGE - 1) / KV4_PAGE * KV4_PAGE; }
-KV4_FN bool kv4_kept(int cols, int ctx) { return cols <= KV4_FEW_COLUMNS && cols * kv4_kept_width(ctx) <= KV4_KEEP; }
+KV4_FN bool kv4_kept(int cols, int ctx, int64_t room) { return cols <= KV4_FEW_COLUMNS && cols * kv4_kept_width(ctx) <= room; }
 
+// Where a buffer by (sequence, key head) has its parts: by the number of the sequence, each part as large as there may be one, or by its
+// rows, each part as large as they ask for.  The host takes what is less: few rows under loose bounds, or few sequences, some of them
+// prompts.  Below 2^32 either way (65535 sequences of 64 columns, 1024 key heads; scores are fewer).
+struct Kv4Place {
+    unsigned seq, head, row, row_head;
+    __device__ __forceinline__ unsigned at(int i, int h, const Kv4Seq& s) const { return i * seq + h * head + s.start * row + h * s.n * row_head; }
+};
 struct Kv4Attn {
     const uint16_t* q; uint16_t* out;
     unsigned q_stride, out_stride, inv;        // row strides in elements; ceil(2^32 / group), 0 for a group of one
-    int group, tiles, chunks;     // query heads per key head; column tiles and chunks the state buffer holds per (sequence, key head)
+    int group, tiles, chunks;     // query heads per key head; column tiles and chunks that a sequence of few columns has at most
     float c;                      // scale * log2(e)
-    // of sequences of few columns, by (sequence, key head, tile): O before its division by l [chunk][16][hd], m and l [16][chunk]
+    // of sequences of few columns, from kv4_states_at() on: O before its division by l [chunk][hd], m and l [chunk]
     float* states;
     f32x2* ml;
+    Kv4Place few;
     // for the weights, or null.  Columns of a (sequence, key head) start at kv4_column(), tiles of 16 of them being whole:
     f32x2* norm;                  // m and 1 / l of each column, where scores are formed again
     uint8_t* frags;               // the queries of each tile as the product takes them: [hd / 32][64 lanes][16 bytes]
     int slots;                    // tiles of a key head that these have room for
     uint8_t* images;              // [sequence][key head][pages]: pages as bf16 fragments, K's then V's; or null
     int pages;
-    float* scores;                // [sequence][key head][room]: raw scores [column][kv4_kept_width], or null
-    int64_t room;
+    float* scores;                // raw scores where kv4_kept(), from kv4_scores_at() on: [column][kv4_kept_width]; or null
+    Kv4Place kept;
+    int64_t kept_unit, room;
     // row of a column: col / group without a division (exact below 2^26, and there are at most 2^22 columns)
     __device__ __forceinline__ int row(int col) const { return inv ? (int)__umulhi((unsigned)col, inv) : col; }
     __device__ __forceinline__ const uint16_t* q_at(int row, int head_at) const { return q + (uint64_t)(unsigned)row * q_stride + head_at; }
     __device__ __forceinline__ uint16_t* out_at(int row, int head_at) const { return out + (uint64_t)(unsigned)row * out_stride + head_at; }
 };
-__device__ __forceinline__ int64_t kv4_tile_at(const Kv4Attn& a, int Hkv, int seq, int h, int tile) {
-    return (((int64_t)seq * Hkv + h) * a.tiles + tile) * a.chunks * 16;
+// chunk states of a column of a sequence of few columns, one behind the other
+__device__ __forceinline__ int64_t kv4_states_at(const Kv4Attn& a, int h, int seq, const Kv4Seq& s, int col) {
+    return (int64_t)(a.few.at(seq, h, s) + col) * a.chunks;
 }
+// scores of a sequence and key head
+__device__ __forceinline__ float* kv4_scores_at(const Kv4Attn& a, int h, int seq, const Kv4Seq& s) { return a.scores + a.kept.at(seq, h, s) * a.kept_unit; }
 
 // first column of a sequence and key head: sequences in order take disjoint tiles, for floor((a + b) / 16) + 1 >= floor(a / 16) +
 // ceil(b / 16), and never one outside the buffer
@@ -375,7 +389,7 @@ __device__ __forceinline__ void kv4_few_block(const Kv4View& c, const Kv4Rows& b
     const int least = s.ctx - s.n + a.row(tile * 16) + 1;    // what the tile's first row sees
     Kv4Query<HD, F16> q[1];
     q[0].load(col < cols ? a.q_at(s.start + j, head * HD) : nullptr, lane,
-              a.frags && !kv4_kept(cols, s.ctx) && chunk == 0 && w == 0 ? a.frags + (kv4_column(a, h, seq, s) + tile * 16) * (2 * HD) : nullptr);
+              a.frags && !kv4_kept(cols, s.ctx, a.room) && chunk == 0 && w == 0 ? a.frags + (kv4_column(a, h, seq, s) + tile * 16) * (2 * HD) : nullptr);
     Kv4State<HD, 1> st;
     st.clear();
 
@@ -386,8 +400,8 @@ __device__ __forceinline__ void kv4_few_block(const Kv4View& c, const Kv4Rows& b
     const int32_t* bt = c.table + (int64_t)s.stream * c.max_pages + p0;
     const int ids = lane < np ? bt[lane] : -1;
     // where the lane's 16 tokens' scores go, if they are wanted
-    float* keep = a.scores && col < cols && kv4_kept(cols, s.ctx)
-                      ? a.scores + ((int64_t)seq * c.Hkv + h) * a.room + col * kv4_kept_width(s.ctx) + 16 * (lane >> 4) : nullptr;
+    float* keep = a.scores && col < cols && kv4_kept(cols, s.ctx, a.room)
+                      ? kv4_scores_at(a, h, seq, s) + col * kv4_kept_width(s.ctx) + 16 * (lane >> 4) : nullptr;
     Kv4Page<HD> pg;
     if (w < np) {
         const int id = __builtin_amdgcn_readlane(ids, w);
@@ -448,10 +462,10 @@ __device__ __forceinline__ void kv4_few_block(const Kv4View& c, const Kv4Rows& b
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e] = fmaf(so[x][k][d + e], f, o[e]);
         }
-        const int64_t at = kv4_tile_at(a, c.Hkv, seq, h, tile);
-        if (a.ml && d == 0) a.ml[at + k * a.chunks + chunk] = f32x2{M, L};
+        const int64_t at = kv4_states_at(a, h, seq, s, kcol) + chunk;
+        if (a.ml && d == 0) a.ml[at] = f32x2{M, L};
         if (chunks > 1) {
-            float* sp = a.states + (at + chunk * 16 + k) * HD + d;
+            float* sp = a.states + at * HD + d;
 #pragma unroll
             for (int e = 0; e < 8; e += 4) *reinterpret_cast<f32x4*>(sp + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
         } else {
@@ -485,16 +499,16 @@ __device__ __forceinline__ void kv4_join_block(const Kv4View& c, const Kv4Rows& 
     if (s.state || cols > KV4_FEW_COLUMNS || col >= cols) return;
     const int chunks = kv4_chunks(s.ctx);
     if (chunks <= 1) return;
-    const int k = col & 15, group = threadIdx.x / T, t = threadIdx.x % T;
-    const int64_t at = kv4_tile_at(a, c.Hkv, seq, h, col >> 4);
-    const f32x2* ml = a.ml + at + k * a.chunks;
-    const float* sp = a.states + (at + k) * HD + 4 * t;
+    const int group = threadIdx.x / T, t = threadIdx.x % T;
+    const int64_t at = kv4_states_at(a, h, seq, s, col);
+    const f32x2* ml = a.ml + at;
+    const float* sp = a.states + at * HD + 4 * t;
     float M = KV4_NONE, L = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 2
     for (int x = group; x < chunks; x += GROUPS) {
         const f32x2 part = ml[x];
-        const f32x4 v = *reinterpret_cast<const f32x4*>(sp + (int64_t)x * (16 * HD));
+        const f32x4 v = *reinterpret_cast<const f32x4*>(sp + (int64_t)x * HD);
         const float top = fmaxf(M, part[0]), f0 = kv4_exp(M, top, a.c), f1 = kv4_exp(part[0], top, a.c);
         L = fmaf(L, f0, part[1] * f1);
 #pragma unroll
@@ -854,7 +868,7 @@ __device__ __forceinline__ void kv4_kept_block(const Kv4View& c, const Kv4Rows& 
         const int log = cols <= 16 ? 4 : cols <= 32 ? 3 : 2, each = tid >> log;
         float M = KV4_NONE, L = 0.f;
         if (each < cols) {
-            const f32x2* ml = a.ml + kv4_tile_at(a, c.Hkv, i, h, each >> 4) + (each & 15) * a.chunks;
+            const f32x2* ml = a.ml + kv4_states_at(a, h, i, s, each);
             for (int x = tid & ((1 << log) - 1); x < chunks; x += 1 << log) {
                 const f32x2 part = ml[x];
                 const float top = fmaxf(M, part[0]);
@@ -874,7 +888,7 @@ __device__ __forceinline__ void kv4_kept_block(const Kv4View& c, const Kv4Rows& 
         __syncthreads();
         if (first >= s.ctx) return;
         const int64_t width = kv4_kept_width(s.ctx);
-        const float* sp = a.scores + ((int64_t)i * c.Hkv + h) * a.room + first;
+        const float* sp = kv4_scores_at(a, h, i, s) + first;
 #pragma unroll 4
         for (int col = GROUPS == 1 ? 0 : w; col < cols; col += GROUPS) {
             const int seen = s.ctx - s.n + a.row(col) + 1 - first;
@@ -933,9 +947,9 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_kernel(Kv4View c, Kv4Rows 
     const bool own = kv4_of_stream(b, c, seq, lane, [&](int i, const Kv4Seq& s) {
         if (s.state || first >= s.ctx) return;
         const int rows = s.n < b.max_rows ? s.n : b.max_rows, cols = rows * a.group;
-        if (kv4_kept(cols, s.ctx)) {
+        if (kv4_kept(cols, s.ctx, a.room)) {
             const int64_t width = kv4_kept_width(s.ctx);
-            const float* sp = a.scores + ((int64_t)i * c.Hkv + h) * a.room + first + lane;
+            const float* sp = kv4_scores_at(a, h, i, s) + first + lane;
             for (int col = w; col < cols; col += 4) {
                 const int j = a.row(col);
                 const f32x2 norm = a.norm[kv4_column(a, h, i, s) + col];
@@ -1024,30 +1038,50 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_kernel(Kv4View c, Kv4Rows 
 // Entry points
 // ------------------------------------------------------------------------------------------------------------------
 // the work buffer: chunks' O | their m and l | kept scores | m and 1 / l | queries | converted pages
-struct Kv4Work { int64_t states, ml, scores, norm, frags, images, room; int tiles, chunks, slots, pages; };
+struct Kv4Work {
+    int64_t states, ml, scores, norm, frags, images, room, kept_unit;
+    Kv4Place few, kept;
+    int tiles, chunks, slots, pages;
+    int64_t bytes() const { return states + ml + scores + norm + frags + images; }
+};
 // Pages are converted by a launch of their own from this many columns on (6 x 513 rows x 16 heads of 64 18.0 us, so 18.4; 4 x 1000 34.3 and
 // 28.9; 64 x 100 41 and 60), unless they need more than this many bytes
 #define KV4_IMAGE_COLUMNS 768
 #define KV4_IMAGE_BYTES (1ll << 29)
 static Kv4Work plan_work(const t3_kv4_cache* c, const t3_kv4_batch* b, int H, bool weights) {
     Kv4Work w{};
-    const int64_t cols = (int64_t)b->max_rows * (H / c->Hkv), few = cols < KV4_FEW_COLUMNS ? cols : KV4_FEW_COLUMNS;
+    const int64_t group = H / c->Hkv, cols = b->max_rows * group, few = cols < KV4_FEW_COLUMNS ? cols : KV4_FEW_COLUMNS;
     const int64_t cap = (int64_t)c->max_pages * KV4_PAGE, most = b->max_ctx < cap ? b->max_ctx : cap, pairs = (int64_t)b->n_seqs * c->Hkv;
+    const auto whole = [](int64_t bytes) { return (bytes + 255) / 256 * 256; };
     w.tiles = (int)((few + 15) / 16);
     w.chunks = kv4_chunks((int)most);
-    const int64_t parts = pairs * w.tiles * w.chunks * 16;
-    w.states = w.chunks > 1 ? parts * c->hd * 4 : 0;
-    w.ml = w.chunks > 1 ? parts * 8 : 0;
+    // columns of sequences of few: not more than the rows have, nor than `few` a sequence
+    const int64_t by_row = b->rows * group, by_seq = b->n_seqs * few, columns = by_row < by_seq ? by_row : by_seq;
+    const auto by_rows = [&] { return Kv4Place{0, 0, (unsigned)(c->Hkv * group), (unsigned)group}; };
+    w.few = by_row < by_seq ? by_rows() : Kv4Place{(unsigned)(c->Hkv * few), (unsigned)few, 0, 0};
+    const int64_t parts = c->Hkv * columns * w.chunks;
+    w.states = w.chunks > 1 ? whole(parts * c->hd * 4) : 0;
+    w.ml = w.chunks > 1 ? whole(parts * 8) : 0;
     if (weights) {
-        const int64_t every = few * kv4_kept_width(most);
+        const int64_t width = kv4_kept_width(most), every = few * width;
         w.room = every < KV4_KEEP ? every : KV4_KEEP;
-        w.scores = pairs * w.room * 4;
-        w.slots = (int)((int64_t)b->rows * (H / c->Hkv) / 16) + b->n_seqs + 1;
-        if (cols > few || every > KV4_KEEP) {                     // some scores are formed again
+        // by rows; by sequences; by sequences with less room for each, so that fewer have their scores kept
+        if (by_row * width < b->n_seqs * w.room && c->Hkv * by_row * width * 4 <= KV4_KEEP_BYTES) {
+            w.kept = by_rows();
+            w.kept_unit = width;
+            w.scores = c->Hkv * by_row * width * 4;
+        } else {
+            if (pairs * w.room * 4 > KV4_KEEP_BYTES) w.room = KV4_KEEP_BYTES / 4 / pairs / KV4_PAGE * KV4_PAGE;
+            w.kept = Kv4Place{(unsigned)c->Hkv, 1, 0, 0};
+            w.kept_unit = w.room;
+            w.scores = pairs * w.room * 4;
+        }
+        w.slots = (int)(by_row / 16) + b->n_seqs + 1;
+        if (cols > few || every > w.room) {                       // some scores are formed again
             w.norm = (int64_t)c->Hkv * w.slots * 16 * 8;
             w.frags = (int64_t)c->Hkv * w.slots * 16 * c->hd * 2;
         } else {
-            w.ml = parts * 8;
+            w.ml = whole(parts * 8);
         }
     }
     w.pages = (int)((most + KV4_PAGE - 1) / KV4_PAGE);
@@ -1058,13 +1092,15 @@ static Kv4Work plan_work(const t3_kv4_cache* c, const t3_kv4_batch* b, int H, bo
 static int check_sizes(const t3_kv4_cache* c, const t3_kv4_batch* b, int H) {
     T3_REQUIRE(b->max_ctx <= (1 << 26) || c->max_pages <= (1 << 26) / KV4_PAGE, "attn_kv4: more than 2^26 entries in a stream");
     T3_REQUIRE(H >= c->Hkv && H % c->Hkv == 0 && H / c->Hkv <= 64, "attn_kv4: query heads must be 1..64 times the key heads");
+    T3_REQUIRE((int64_t)b->max_rows * (H / c->Hkv) <= (1 << 22), "attn_kv4: more than 2^22 rows x query heads of a key head");
+    T3_REQUIRE((int64_t)b->rows * (H / c->Hkv) <= (1 << 30), "attn_kv4: more than 2^30 rows x query heads of a key head in one call");
     return 0;
 }
 
 extern "C" int64_t t3_op_attn_kv4_work_bytes(const t3_kv4_cache* cache, const t3_kv4_batch* batch, int32_t H, int32_t with_weights) {
     if (kv4_check_cache(cache, 0, 1, nullptr) || kv4_check_batch(batch) || check_sizes(cache, batch, H)) return -1;
     const Kv4Work w = plan_work(cache, batch, H, with_weights != 0);
-    return w.states + w.ml + w.scores + w.norm + w.frags + w.images;
+    return w.bytes();
 }
 
 template <int HD, bool F16>
@@ -1114,8 +1150,6 @@ extern "C" int t3_op_attn_kv4(const t3_kv4_cache* cache, const t3_kv4_batch* bat
     T3_REQUIRE(q_dev && out_dev, "attn_kv4: null argument");
     T3_REQUIRE(dtype == 0 || dtype == 1, "attn_kv4: dtype must be 0 (bf16) or 1 (fp16)");
     T3_REQUIRE(scale > 0.f && scale < 1e8f, "attn_kv4: scale must be positive");
-    T3_REQUIRE((int64_t)batch->max_rows * (H / cache->Hkv) <= (1 << 22), "attn_kv4: more than 2^22 rows x query heads of a key head");
-    T3_REQUIRE((int64_t)batch->rows * (H / cache->Hkv) <= (1 << 30), "attn_kv4: more than 2^30 rows x query heads of a key head in one call");
     const int64_t width = (int64_t)H * cache->hd;
     T3_REQUIRE(q_stride >= width && out_stride >= width && q_stride % 8 == 0 && out_stride % 8 == 0 &&
                reinterpret_cast<uintptr_t>(q_dev) % 16 == 0 && reinterpret_cast<uintptr_t>(out_dev) % 16 == 0,
@@ -1133,7 +1167,7 @@ extern "C" int t3_op_attn_kv4(const t3_kv4_cache* cache, const t3_kv4_batch* bat
     a.c = scale * 1.44269504088896340736f;
     const Kv4Work w = plan_work(cache, batch, H, weights_dev != nullptr);
     uint8_t* work = static_cast<uint8_t*>(work_dev);
-    a.tiles = w.tiles; a.chunks = w.chunks; a.room = w.room;
+    a.tiles = w.tiles; a.chunks = w.chunks; a.room = w.room; a.few = w.few; a.kept = w.kept; a.kept_unit = w.kept_unit;
     a.states = reinterpret_cast<float*>(work);
     work += w.states;
     a.ml = w.ml ? reinterpret_cast<f32x2*>(work) : nullptr;

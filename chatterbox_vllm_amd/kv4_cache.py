@@ -6,7 +6,7 @@ counterpart in the reference: 4.25 bits a value, 3.76 times less to store and to
 
     cache = KV4Cache(num_kv_heads=16, head_dim=64, num_pages=4096, num_streams=64, max_pages=16)
     cache.block_table[s, i] = page                               # page allocation is the caller's
-    batch = cache.batch(seq_start, streams, ctx, rows=R)         # one object for the calls of a step
+    batch = cache.batch(seq_start, streams, ctx, rows=R, max_rows=1, max_ctx=n)      # one object for the calls of a step
     cache.append(k, v, batch)
     out = cache.attend(q, batch, weights=weights[0])             # weights: cache.new_weights(), where eviction is wanted
     new_ctx, kept = cache.evict(src, dst, ctx, keep=256, sink=34, recent=64, weights=weights)
@@ -40,7 +40,8 @@ class KV4Batch:
     """The rows of a call: sequence i owns rows ``seq_start[i] .. seq_start[i + 1] - 1`` of the row tensors, which are entries
     ``ctx[i] - n_i .. ctx[i] - 1`` of stream ``streams[i]`` (< 0: skipped).  The three tensors (int32, on the cache's device) are
     read when the kernels run, so a captured graph follows what is written into them; ``rows``, ``max_rows`` and ``max_ctx`` are
-    the host's bounds for them."""
+    the host's bounds for them, by default the loosest ones (all rows in one sequence, the whole block table).  Grids and the work
+    buffer of ``attend`` follow the bounds: what is known to be less is worth giving."""
 
     def __init__(self, cache: "KV4Cache", seq_start: torch.Tensor, streams: torch.Tensor, ctx: torch.Tensor, rows: int,
                  max_rows: Optional[int] = None, max_ctx: Optional[int] = None):

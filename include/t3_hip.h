@@ -392,7 +392,10 @@ int t3_op_kv4_read(const t3_kv4_cache* cache, const t3_kv4_batch* batch, void* k
  * over the query heads of its key head, are added to it (in a fixed order: equal calls give equal bits).  weights_stride >=
  * max_ctx.  A refused sequence adds nothing.
  * work_dev: t3_op_attn_kv4_work_bytes() bytes, 16-byte aligned, for this call alone while it runs: calls that may overlap
- * (streams, replayed graphs) need one each.  It need not be cleared.
+ * (streams, replayed graphs) need one each.  It need not be cleared.  Its size follows the batch's bounds: chunk states of hd + 2
+ * values for every 1024 entries of each column (a row and query head) of sequences that have at most 64 of them, at most rows *
+ * group columns a key head; for prompts up to 512 MiB of converted pages; with weights the queries once more and up to 512 MiB of
+ * scores (weights of entries whose scores found no room are formed again, which takes longer).
  * A row's bits depend on its sequence alone, not on what else is in the call. */
 int64_t t3_op_attn_kv4_work_bytes(const t3_kv4_cache* cache, const t3_kv4_batch* batch, int32_t H, int32_t with_weights);
 int t3_op_attn_kv4(const t3_kv4_cache* cache, const t3_kv4_batch* batch, const void* q_dev, int64_t q_stride, void* out_dev,

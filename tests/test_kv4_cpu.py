@@ -268,3 +268,41 @@ def test_a_narrow_row_of_weights_is_no_longer_than_it_is():
     assert w.is_contiguous() and w.stride(1) == 200
     cache.attend(torch.zeros(1, 2, 64, dtype=torch.bfloat16), cache.batch(i32([0, 1]), i32([0]), i32([100]), rows=1, max_ctx=100), weights=w)
     assert cache.calls[0][10] == 100                             # the library refuses max_ctx past it
+
+
+def _work_bytes(kv, hd, n_seqs, rows, max_rows, max_ctx, heads, weights):
+    lib = _capi.load()
+    cache = _cache(n_layers=1, n_pages=1 << 20, n_streams=4096, max_pages=1 << 20, Hkv=kv, hd=hd)
+    return lib.t3_op_attn_kv4_work_bytes(C.byref(cache), C.byref(_batch(n_seqs=n_seqs, rows=rows, max_rows=max_rows, max_ctx=max_ctx)), heads, weights)
+
+
+MIB = 1 << 20
+
+
+@pytest.mark.parametrize("kv,hd,n_seqs,rows,max_rows,max_ctx,heads", [
+    (16, 64, 64, 64, 64, 1 << 15, 16),                            # a decode step, bounds as they are when none is given
+    (16, 64, 64, 64, 1, 1 << 15, 16),
+    (8, 128, 64, 320, 5, 16000, 64),                              # drafts on shared key heads
+    (8, 128, 16, 32000, 2000, 33000, 8),                          # prompts alone
+    (16, 128, 16, 32000, 2000, 33000, 16),
+    (8, 128, 16, 4110, 4095, 5001, 32),                           # a prompt among decode rows
+    (1024, 128, 65535, 1 << 22, 1 << 16, 1 << 26, 1024),          # the largest bounds
+    (1, 64, 1, 1, 1, 1 << 26, 1), (1, 64, 1, 1, 1, 1, 64)])
+@pytest.mark.parametrize("weights", [0, 1])
+def test_the_work_buffer_is_bounded(kv, hd, n_seqs, rows, max_rows, max_ctx, heads, weights):
+    """Chunk states of the columns that there are, at most 512 MiB of converted pages, of scores at most 512 MiB and what the columns
+    have; beside them per row what the queries have."""
+    group, chunks = heads // kv, -(-max_ctx // 1024)
+    columns = kv * min(rows * group, n_seqs * min(64, max_rows * group))
+    states = columns * chunks * (hd * 4 + 8)
+    kept = min(512 * MIB, columns * min(4 * MIB, (max_ctx + 63) * 4)) + kv * (rows * group + 16 * (n_seqs + 1)) * (hd * 2 + 8)
+    images = 512 * MIB if max_rows * group >= 768 else 0
+    size = _work_bytes(kv, hd, n_seqs, rows, max_rows, max_ctx, heads, weights)
+    assert 0 <= size <= states + (kept if weights else 0) + images + 1024
+
+
+def test_work_buffers_of_loose_bounds():
+    tight, loose = (_work_bytes(16, 64, 64, 64, m, 1 << 15, 16, 1) for m in (1, 64))
+    assert tight <= loose <= 2 * tight and loose <= 160 * MIB
+    assert _work_bytes(16, 64, 64, 64, 64, 1 << 15, 16, 0) <= 16 * MIB
+    assert _work_bytes(64, 64, 4, 1 << 25, 1 << 22, 100, 64 * 64, 1) == -1      # more columns than a call may have

@@ -473,6 +473,37 @@ def test_weights_of_more_scores_than_are_kept(hd, group, rows, ctx, streams):
 
 
 @pytest.mark.parametrize("hd", [64, 128])
+def test_weights_where_scores_find_less_room(hd):
+    """Bounds under which the scores' share of the work buffer is cut: 1000 sequences, most of them skipped, over a table of 2^21 entries.
+    What is kept of the scores and what is formed again follow the room; outputs are the same bits, weights the same sums."""
+    m = _kv4.Model(hd, 4, 1, 3 * 40, 3, 40, seed=42)
+    rows, ctx, group = [4, 3, 1], [2500, 1000, 2400], 4
+    for i, t in enumerate(ctx):
+        m.fill(i, t)
+    cache = device_cache(m)
+    q, out, w = check_attend(m, cache, rows, ctx, group, "bf16", True)
+    wide = torch.full((3, 1 << 15), -1, dtype=torch.int32, device=DEV)
+    wide[:, :40] = cache.block_table
+    loose = KV4Cache(4, hd, pool=cache.pool, block_table=wide)
+    s, n = starts(rows) + [8] * 997, 1000
+    batch = loose.batch(i32(s), i32([0, 1, 2] + [-1] * 997), i32(ctx + [0] * 997), rows=8, max_rows=4)
+    size = cache._lib.t3_op_attn_kv4_work_bytes(loose._ref, batch._ref, 16, 1)
+    assert size < 2 << 30
+    many = loose.new_weights()[0]
+    assert torch.equal(loose.attend(q.to(DEV), batch, weights=many), out)
+    tight = cache.new_weights()[0]
+    cache.attend(q.to(DEV), cache.batch(i32(starts(rows)), i32([0, 1, 2]), i32(ctx), rows=8, max_rows=4, max_ctx=2500), weights=tight)
+    got = many[..., :2560].cpu()
+    assert (many[..., 2560:] == 0).all()
+    for i, t in enumerate(ctx):
+        k, v = m.get(m.pool, i, torch.arange(t))
+        a = sum(rows[:i])
+        _, p, _, bound = _kv4.attend(q[a:a + rows[i]].double(), k, v, t, hd ** -0.5)
+        for x in (got, tight.cpu()):
+            assert ((x[i, :, :t].double() - p).abs() <= _kv4.weights_bound(p, p, bound, t, rows[i] * group)).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
 def test_rows_beyond_what_one_launch_has_workgroups_for(hd):
     """270000 rows of one sequence at once give the bytes that they give a thousand at a time, and come back."""
     n, pages = 270000, 4219
