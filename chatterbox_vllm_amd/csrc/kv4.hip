@@ -136,7 +136,8 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4View c, Kv4Rows b, c
 // ------------------------------------------------------------------------------------------------------------------
 template <bool F16> __device__ __forceinline__ u32x4 kv4_values8(unsigned codes, unsigned byte, bool nan) {
     if constexpr (F16) {
-        // a value appended from fp16 can stand for up to 6 * 2^14: cut at the type's largest instead of becoming infinite
+        // from 57344 on a value appended from fp16 is held as 4 * 2^14, and bf16 has larger ones: cut at the type's largest instead of
+        // becoming infinite
         const f16x2 most = {(_Float16)65504.f, (_Float16)65504.f};
         const float sc = kv4_scale(byte);
         const f16x2 p[4] = {__builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, sc, 0)),

@@ -326,10 +326,15 @@ __device__ __forceinline__ void kv4_values(const Kv4Page<HD>& pg, const bf16x8 (
         }
 }
 
+// Two outputs.  In fp16 cut at the type's largest, as read cuts them: an entry appended from fp16 can be held as up to 65536.  (The bits of
+// an infinity less one are those of the largest; a NaN stays one.)
 template <bool F16> __device__ __forceinline__ unsigned kv4_pack2(float lo, float hi) {
     if constexpr (F16) {
+        typedef __attribute__((ext_vector_type(2))) uint16_t u16x2;
         const f16x2 p = {(_Float16)lo, (_Float16)hi};
-        return __builtin_bit_cast(unsigned, p);
+        u16x2 u = __builtin_bit_cast(u16x2, p);
+        u -= (u & (uint16_t)0x7fff) == (uint16_t)0x7c00 ? u16x2{1, 1} : u16x2{0, 0};
+        return __builtin_bit_cast(unsigned, u);
     } else {
         return pack_bf2(lo, hi);
     }

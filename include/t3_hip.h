@@ -388,6 +388,8 @@ int t3_op_kv4_read(const t3_kv4_cache* cache, const t3_kv4_batch* batch, void* k
 /* Attention of the batch's rows over the cache: row j of n of a sequence sees its first ctx - n + j + 1 entries (causal).
  * q_dev: row r at q_dev + r * q_stride elements, [H][hd] inside it, H = group * Hkv, group 1..64 query heads per key head; out
  * likewise; out may be q (the same rows), but not overlap it otherwise.  A row that sees nothing gets 0.  scale > 0 multiplies the scores.  At most 2^26 entries a stream.
+ * An fp16 output is cut at the type's largest value, as read's are.  The sums are in fp32 before they are divided: they hold any values
+ * below 2^119 / ctx.
  * weights_dev (optional): [n_streams][Hkv][weights_stride] fp32; every entry's softmax weights, summed over the call's rows and
  * over the query heads of its key head, are added to it (in a fixed order: equal calls give equal bits).  weights_stride >=
  * max_ctx.  A refused sequence adds nothing.

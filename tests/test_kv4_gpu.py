@@ -326,6 +326,27 @@ def test_a_common_offset_of_the_scores_cancels(hd, group, rows, ctx, dtype, offs
     assert ((w[0, :, :ctx].cpu().double() - p).abs() <= p * (2.0 ** -15 + (ctx + rows * group) / 16 * 2.0 ** -24)).all()
 
 
+@pytest.mark.parametrize("hd,group,rows,ctx", [(64, 1, 1, 1), (128, 2, 3, 1100), (64, 3, 100, 130), (128, 8, 120, 200)])
+def test_the_largest_fp16_values_stay_finite(hd, group, rows, ctx):
+    """65504 is held as 65536, which fp16 does not have: fp16 outputs are cut as read cuts them, bf16 ones are exact, NaN entries stay NaN."""
+    m = _kv4.Model(hd, 2, 1, 20, 1, 18, seed=43)
+    v = torch.full((ctx, 2, hd), 65504.0)
+    v[..., 1::2] *= -1
+    m.put(m.pool, 0, torch.arange(ctx), torch.zeros(ctx, 2, hd), v)
+    cache = device_cache(m)
+    batch = cache.batch(i32([0, rows]), i32([0]), i32([ctx]), rows=rows)
+    sign = torch.tensor([1.0, -1.0]).repeat(hd // 2).to(DEV)
+    q = torch.randn(rows, 2 * group, hd, generator=torch.Generator().manual_seed(44)).to(DEV)
+    assert (cache.attend(q.half(), batch) == (65504 * sign).half()).all()
+    assert (cache.attend(q.bfloat16(), batch) == (65536 * sign).bfloat16()).all()
+    k = torch.zeros(1, 2, hd)
+    k[0, 0, 0] = math.nan
+    m.put(m.pool, 0, torch.tensor([ctx - rows]), k, v[:1])          # of head 0: seen by every row
+    bad = device_cache(m)
+    out = bad.attend(q.half(), bad.batch(i32([0, rows]), i32([0]), i32([ctx]), rows=rows))
+    assert torch.isnan(out[:, :group]).all() and (out[:, group:] == (65504 * sign).half()).all()
+
+
 def test_what_lies_behind_the_last_entry_does_not_matter():
     """Every byte behind the last entry set, scales to NaN among them."""
     outs = []
