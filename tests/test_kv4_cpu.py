@@ -306,3 +306,12 @@ def test_work_buffers_of_loose_bounds():
     assert tight <= loose <= 2 * tight and loose <= 160 * MIB
     assert _work_bytes(16, 64, 64, 64, 64, 1 << 15, 16, 0) <= 16 * MIB
     assert _work_bytes(64, 64, 4, 1 << 25, 1 << 22, 100, 64 * 64, 1) == -1      # more columns than a call may have
+
+
+@pytest.mark.parametrize("given", [[], ["EXTRA=-DONE", "BUILD=build_x"], ["EXTRA=-DONE", "PRELOAD="]])
+def test_no_build_of_the_cache_has_packed_fp32_instructions(given):
+    """Their switch is on every compile line of the cache's kernels, whatever else the build is given."""
+    lines = subprocess.run(["make", "-n", "-B", "-C", CSRC, *given], capture_output=True, text=True, check=True).stdout.splitlines()
+    lines = [x for x in lines if re.search(r" -c kv4(_attn)?\.hip ", x)]
+    assert len(lines) == 2 and all("-Xclang -target-feature -Xclang -packed-fp32-ops" in x for x in lines)
+    assert all(("-DONE" in x) == (len(given) > 0) for x in lines)
