@@ -486,7 +486,35 @@ __device__ __forceinline__ int kv4_prefix(int v, int* wave_sums, int* all) {
     return before + x - v;
 }
 
+// What kv4_pages_bad finds, in time that grows with the pages and not with their square: the destination's are marked in shared memory,
+// KV4_MARKS page ids at a time, and the source's looked up.  (One head of 64, 2^20 entries to half of them: the whole eviction 2.7 ms, by
+// pairs of pages 21; 2^22 entries 13.7 and 326.)
+#define KV4_MARKS (1 << 19)
+__device__ __forceinline__ bool kv4_many_pages_bad(const int32_t* sp, const int32_t* dp, int ns, int nd, int n_pages, unsigned* marks) {
+    const int tid = threadIdx.x;
+    bool bad = false;
+    for (int o = tid; o < ns; o += KV4_CHOOSE_THREADS) bad = bad || !kv4_page_ok(sp[o], n_pages);
+    for (int d = tid; d < nd; d += KV4_CHOOSE_THREADS) bad = bad || !kv4_page_ok(dp[d], n_pages);
+    for (int64_t from = 0; from < n_pages; from += KV4_MARKS) {
+        const int here = n_pages - from < KV4_MARKS ? (int)(n_pages - from) : KV4_MARKS;
+        for (int x = tid; x < (here + 31) / 32; x += KV4_CHOOSE_THREADS) marks[x] = 0;
+        __syncthreads();
+        for (int d = tid; d < nd; d += KV4_CHOOSE_THREADS) {
+            const int64_t at = dp[d] - from;
+            if (at >= 0 && at < here) atomicOr(&marks[at >> 5], 1u << (at & 31));
+        }
+        __syncthreads();
+        for (int o = tid; o < ns; o += KV4_CHOOSE_THREADS) {
+            const int64_t at = sp[o] - from;
+            if (at >= 0 && at < here) bad = bad || (marks[at >> 5] >> (at & 31) & 1u);
+        }
+        __syncthreads();
+    }
+    return bad;
+}
+
 __global__ __launch_bounds__(KV4_CHOOSE_THREADS) void kv4_choose_kernel(Kv4View c, Kv4Evict e) {
+    __shared__ unsigned marks[KV4_MARKS / 32];
     __shared__ int hist[256];
     __shared__ int wave_sums[KV4_CHOOSE_THREADS / 64];
     __shared__ int pick[2];
@@ -496,9 +524,10 @@ __global__ __launch_bounds__(KV4_CHOOSE_THREADS) void kv4_choose_kernel(Kv4View 
     const Kv4Entry x = kv4_entry(c, e, i);
     if (!x.ok) { kv4_refuse<KV4_CHOOSE_THREADS>(e, kept, i, first); return; }
     const int ctx = x.ctx, left = ctx < e.keep ? ctx : e.keep;
-    if (__syncthreads_or(kv4_entry_taken<KV4_CHOOSE_THREADS>(e, x, i) ||
-                         kv4_pages_bad<KV4_CHOOSE_THREADS>(c.table + (int64_t)x.src * c.max_pages, c.table + (int64_t)x.dst * c.max_pages,
-                                                           (ctx + KV4_PAGE - 1) / KV4_PAGE, (left + KV4_PAGE - 1) / KV4_PAGE, c.n_pages))) { kv4_refuse<KV4_CHOOSE_THREADS>(e, kept, i, first); return; }
+    const bool taken = kv4_entry_taken<KV4_CHOOSE_THREADS>(e, x, i);
+    const bool bad = kv4_many_pages_bad(c.table + (int64_t)x.src * c.max_pages, c.table + (int64_t)x.dst * c.max_pages,
+                                        (int)(((int64_t)ctx + KV4_PAGE - 1) / KV4_PAGE), (int)(((int64_t)left + KV4_PAGE - 1) / KV4_PAGE), c.n_pages, marks);
+    if (__syncthreads_or(taken || bad)) { kv4_refuse<KV4_CHOOSE_THREADS>(e, kept, i, first); return; }
     const float* w = e.weights + (((int64_t)layer * c.n_streams + x.src) * c.Hkv + h) * e.weights_stride;
     float* wd = e.weights + (((int64_t)layer * c.n_streams + x.dst) * c.Hkv + h) * e.weights_stride;
 

@@ -724,6 +724,60 @@ def test_evict_refuses_entry_by_entry():
     assert new.tolist() == [70, 70] and kept.max() < 190
 
 
+def test_evict_refuses_long_entries_with_bad_pages():
+    """The page check of entries past 16384, in a pool of more page ids than it marks at a time."""
+    n_pages, width = (1 << 19) + 700, 300
+    ids = torch.randperm(n_pages, generator=torch.Generator().manual_seed(45))
+    ids = torch.cat([ids[ids >= 1 << 19], ids[ids < 1 << 19]])[:12 * width].to(torch.int32)
+    table = ids[torch.randperm(12 * width, generator=torch.Generator().manual_seed(46))].view(12, width)
+    ctx, keep, sink, recent = [19200, 17000, 19200, 18000, 16385, 19199], 9000, 10, 500
+    nd = -(-keep // 64)
+    table[6, nd:] = table[0, :width - nd]                         # behind what is written: does not count
+    top = (table[1, :17000 // 64] >= 1 << 19).nonzero()[-1, 0]
+    table[7, nd - 1] = table[1, top]                              # 1 -> 7: one page of both, with an id behind the first 2^19
+    low = (table[2] < 1 << 19).nonzero()[-1, 0]
+    table[8, 0] = table[2, low]                                   # 2 -> 8: the same before
+    table[9, nd - 1] = n_pages                                    # 3 -> 9: a page that there is not
+    table[4, 256] = -5                                            # 4 -> 10: the source's last page
+    assert (table[0] >= 1 << 19).any() and (table[0] < 1 << 19).any()
+    cache = KV4Cache(1, 64, num_pages=n_pages, block_table=table.to(DEV))
+    for i in (0, 5):
+        cache.pool[0, table[i].long().to(DEV)] = torch.randint(0, 200, (width, 4352), dtype=torch.uint8, generator=torch.Generator().manual_seed(i)).to(DEV)
+    w = cache.new_weights()
+    w[0, :6, 0] = torch.rand(6, width * 64, generator=torch.Generator().manual_seed(47)).to(DEV)
+    w0, whole = w.cpu(), cache.pool[0, table[5].long().to(DEV)].clone()
+    new, kept = cache.evict(i32(list(range(6))), i32([6, 7, 8, 9, 10, 11]), i32(ctx), keep, sink, recent, w)
+    assert new.tolist() == [keep, -1, -1, -1, -1, keep]
+    assert (kept[0, 1:5] == -1).all() and torch.equal(w.cpu()[0, 7:11], w0[0, 7:11])
+    for i in (0, 5):
+        stay = _kv4.choose(w0[0, i, 0].tolist(), ctx[i], keep, sink, recent)
+        assert kept[0, i, 0].tolist() == stay
+        old = cache.read(cache.batch(i32([0, ctx[i]]), i32([i]), i32([ctx[i]]), rows=ctx[i]))
+        got = cache.read(cache.batch(i32([0, keep]), i32([6 + i]), i32([keep]), rows=keep))
+        assert all(torch.equal(b, a[stay]) for a, b in zip(old, got))
+    assert torch.equal(cache.pool[0, table[5].long().to(DEV)], whole)
+
+
+def test_evict_four_million_entries():
+    ctx, keep, sink, recent = (1 << 22) - 5, 3000001, 100, 4000
+    pages = 1 << 16
+    cache = KV4Cache(1, 64, num_pages=2 * pages, block_table=torch.arange(2 * pages, dtype=torch.int32, device=DEV).flip(0).view(2, pages))
+    g = torch.Generator(device=DEV).manual_seed(48)
+    cache.pool[0, :, :4096] = torch.randint(0, 256, (4096,), dtype=torch.uint8, generator=g, device=DEV)
+    cache.pool[0, :, 4096:] = 127
+    cache.pool[0, pages:, 3] = torch.randint(0, 256, (pages,), dtype=torch.uint8, generator=g, device=DEV)
+    w = cache.new_weights()
+    w[0, 0, 0] = torch.rand(pages * 64, generator=g, device=DEV)
+    order = w[0, 0, 0, sink:ctx - recent].argsort(descending=True, stable=True)[:keep - sink - recent].sort().values + sink
+    stay = torch.cat([torch.arange(sink, device=DEV), order, torch.arange(ctx - recent, ctx, device=DEV)])
+    old = w[0, 0, 0].clone()
+    new, kept = cache.evict(i32([0]), i32([1]), i32([ctx]), keep, sink, recent, w)
+    assert new.tolist() == [keep] and torch.equal(kept.view(-1).long(), stay)
+    assert torch.equal(w[0, 1, 0, :keep], old[stay]) and (w[0, 1, 0, keep:] == 0).all()
+    before, after = cache.read(cache.batch(i32([0, ctx]), i32([0]), i32([ctx]), rows=ctx))[0], cache.read(cache.batch(i32([0, keep]), i32([1]), i32([keep]), rows=keep))[0]
+    assert torch.equal(after, before[stay])
+
+
 # ---- the operators together ---------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("hd,kv,group", [(64, 4, 1), (128, 2, 4)])
 def test_a_stream_from_prompt_to_eviction_and_on(hd, kv, group):
