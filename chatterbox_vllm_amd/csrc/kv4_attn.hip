@@ -808,10 +808,10 @@ __device__ __forceinline__ void kv4_many_block(const Kv4View& c, const Kv4Rows& 
 
 // Both in one launch, for a batch that may hold sequences of either kind: the long blocks start first.
 template <int HD, bool F16, int NC, bool IMAGES>
-__global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_mixed_kernel(Kv4View c, Kv4Rows b, Kv4Attn a, int turns) {
+__global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_mixed_kernel(Kv4View c, Kv4Rows b, Kv4Attn a, int turns, unsigned first) {
     __shared__ union { Kv4ManyLds<HD> many; Kv4FewLds<HD> few; } lds;
     const unsigned many = (unsigned)c.Hkv * turns * b.n_seqs;
-    unsigned x = blockIdx.x;
+    unsigned x = first + blockIdx.x;
     if (x < many) {
         const int h = x % c.Hkv;
         x /= c.Hkv;
@@ -1108,24 +1108,28 @@ extern "C" int64_t t3_op_attn_kv4_work_bytes(const t3_kv4_cache* cache, const t3
     return w.bytes();
 }
 
+// The launch for few columns has its chunks along the grid's third axis, which ends at 65535; one for both kinds, and none of the other,
+// takes more.  That has at most KV4_LAUNCH_BLOCKS workgroups (a grid's threads end at 2^32); what is more goes into further ones.
+#define KV4_LAUNCH_CHUNKS 65535
+#define KV4_LAUNCH_BLOCKS (1ll << 23)
 template <int HD, bool F16>
 static int launch_attn(const Kv4View& c, const Kv4Rows& b, const Kv4Attn& a, float* weights, int64_t weights_stride, hipStream_t st) {
     // column tiles of a wave: at hd 128 two share each fragment's way through LDS (372 us; one, with eight waves a workgroup, 395); at
     // hd 64 one leaves room for four waves a SIMD instead of two (4 x 2000 rows 70.6 us; two 78, four 98)
     constexpr int NC = HD == 64 ? 1 : 2;
     const int64_t cols = (int64_t)b.max_rows * a.group;
-    if (cols <= KV4_FEW_COLUMNS) {
+    if (cols <= KV4_FEW_COLUMNS && a.chunks <= KV4_LAUNCH_CHUNKS) {
         const dim3 grid(a.tiles * c.Hkv, b.n_seqs, a.chunks);
         if (a.tiles == 1) T3_LAUNCH((kv4_attn_few_kernel<HD, F16, true>), grid, dim3(64 * KV4_FEW_WAVES), 0, st, c, b, a);
         else T3_LAUNCH((kv4_attn_few_kernel<HD, F16, false>), grid, dim3(64 * KV4_FEW_WAVES), 0, st, c, b, a);
     } else {
-        const int64_t turns = (cols + 64 * NC - 1) / (64 * NC), blocks = c.Hkv * (int64_t)b.n_seqs * (turns + (int64_t)a.tiles * a.chunks);
+        const int64_t turns = cols > KV4_FEW_COLUMNS ? (cols + 64 * NC - 1) / (64 * NC) : 0, blocks = c.Hkv * (int64_t)b.n_seqs * (turns + (int64_t)a.tiles * a.chunks);
         T3_REQUIRE(blocks <= INT32_MAX, "attn_kv4: too many sequences of that many rows in one call");
-        if (a.images) {
-            T3_LAUNCH(kv4_image_kernel<HD>, dim3(a.pages * c.Hkv, b.n_seqs), dim3(256), 0, st, c, b, a);
-            T3_LAUNCH((kv4_attn_mixed_kernel<HD, F16, NC, true>), dim3((unsigned)blocks), dim3(256), 0, st, c, b, a, (int)turns);
-        } else {
-            T3_LAUNCH((kv4_attn_mixed_kernel<HD, F16, NC, false>), dim3((unsigned)blocks), dim3(256), 0, st, c, b, a, (int)turns);
+        if (a.images) T3_LAUNCH(kv4_image_kernel<HD>, dim3(a.pages * c.Hkv, b.n_seqs), dim3(256), 0, st, c, b, a);
+        for (int64_t first = 0; first < blocks; first += KV4_LAUNCH_BLOCKS) {
+            const dim3 grid((unsigned)(blocks - first < KV4_LAUNCH_BLOCKS ? blocks - first : KV4_LAUNCH_BLOCKS));
+            if (a.images) T3_LAUNCH((kv4_attn_mixed_kernel<HD, F16, NC, true>), grid, dim3(256), 0, st, c, b, a, (int)turns, (unsigned)first);
+            else T3_LAUNCH((kv4_attn_mixed_kernel<HD, F16, NC, false>), grid, dim3(256), 0, st, c, b, a, (int)turns, (unsigned)first);
         }
     }
     const int joins = a.chunks > 1 ? (cols < KV4_FEW_COLUMNS ? (int)cols : KV4_FEW_COLUMNS) * c.Hkv : 0;

@@ -347,6 +347,24 @@ def test_the_largest_fp16_values_stay_finite(hd, group, rows, ctx):
     assert torch.isnan(out[:, :group]).all() and (out[:, group:] == (65504 * sign).half()).all()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows", [[1, 2], [90, 1]])
+def test_the_loosest_bounds(hd, rows):
+    """A table of 2^26 entries a stream, and no other bound: more chunks than a grid has room for, more workgroups than a launch."""
+    m = _kv4.Model(hd, 2, 1, 2 * 24, 2, 24, seed=49)
+    ctx = [1500, 300]
+    for i, t in enumerate(ctx):
+        m.fill(i, t)
+    cache = device_cache(m)
+    q, out, w = check_attend(m, cache, rows, ctx, 2, "bf16", False)
+    wide = torch.full((2, 1 << 20), -1, dtype=torch.int32, device=DEV)
+    wide[:, :24] = cache.block_table
+    loose = KV4Cache(2, hd, pool=cache.pool, block_table=wide)
+    n = 2 if sum(rows) < 9 else 20                                # 20 x 2 heads x 4 tiles x 65536 chunks: past 2^23
+    batch = loose.batch(i32(starts(rows) + [sum(rows)] * (n - 2)), i32([0, 1] + [-1] * (n - 2)), i32(ctx + [0] * (n - 2)), rows=sum(rows))
+    assert torch.equal(loose.attend(q.to(DEV), batch), out)
+
+
 def test_what_lies_behind_the_last_entry_does_not_matter():
     """Every byte behind the last entry set, scales to NaN among them."""
     outs = []
