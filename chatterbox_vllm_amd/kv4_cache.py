@@ -123,7 +123,7 @@ class KV4Cache:
         dtype, q_stride = self._rows("q", q, batch, heads)
         if out is None:
             out = torch.empty_like(q)                            # dense, or q's own row stride where q is
-            out_stride = out.stride(0)
+            out_stride = out.stride(0) if batch.rows > 1 else heads * self.head_dim
         else:
             out_dtype, out_stride = self._rows("out", out, batch, heads)
             if out_dtype != dtype:
@@ -218,9 +218,9 @@ class KV4Cache:
             raise ValueError(f"{name} must be bfloat16 or float16 [{batch.rows}, {heads}, {self.head_dim}] on {self.device}, "
                              f"got {t.dtype} {tuple(t.shape)} on {t.device}")
         row, head, dim = t.stride()
-        if dim != 1 or head != self.head_dim:
+        if dim != 1 or (head != self.head_dim and heads != 1):   # (along one row or head a tensor's stride may be any number)
             raise ValueError(f"the heads of a row of {name} must lie one behind the other, strides are {t.stride()}")
-        return dtype, row
+        return dtype, row if batch.rows > 1 else heads * self.head_dim
 
     def _weights(self, w: torch.Tensor, dims: int) -> None:
         if w.dtype != torch.float32 or w.get_device() != self._index or w.dim() != dims or not w.is_contiguous() \

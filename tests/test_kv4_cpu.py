@@ -315,3 +315,18 @@ def test_no_build_of_the_cache_has_packed_fp32_instructions(given):
     lines = [x for x in lines if re.search(r" -c kv4(_attn)?\.hip ", x)]
     assert len(lines) == 2 and all("-Xclang -target-feature -Xclang -packed-fp32-ops" in x for x in lines)
     assert all(("-DONE" in x) == (len(given) > 0) for x in lines)
+
+
+@pytest.mark.parametrize("rows,kv,layout", [
+    (5, 1, lambda x: x.as_strided((5, 1, 64), (64, 320, 1))), (1, 2, lambda x: x.as_strided((1, 2, 64), (3, 64, 1))),
+    (1, 1, lambda x: x.as_strided((1, 1, 64), (5, 9, 1))), (5, 2, lambda x: x)])
+def test_rows_of_any_contiguous_layout_are_taken(rows, kv, layout):
+    """The stride along a single row or a single head is any number and plays no part."""
+    cache = HostCache(kv, 64, 2, 2)
+    x = layout(torch.zeros(rows, kv, 64, dtype=torch.bfloat16))
+    batch = cache.batch(i32([0, rows]), i32([0]), i32([rows]), rows=rows)
+    cache.append(x, x, batch)
+    cache.attend(x, batch)
+    cache.attend(x, batch, out=x)
+    assert x.is_contiguous()
+    assert all(call[i] == kv * 64 for call, at in zip(cache.calls, ((4, 5), (3, 5), (3, 5))) for i in at)

@@ -402,6 +402,21 @@ def test_skipped_rows_and_strides():
     assert sorted(changed) == sorted({int(m.table[0, 0]), int(m.table[2, 4])})
 
 
+def test_one_key_head_and_one_row_in_any_contiguous_layout():
+    m = _kv4.Model(64, 1, 1, 10, 2, 5, seed=50)
+    for i in range(2):
+        m.fill(i, 300)
+    cache, plain = device_cache(m), device_cache(m)
+    x = torch.randn(7, 1, 64, generator=torch.Generator().manual_seed(51)).to(torch.bfloat16).to(DEV)
+    apart = x.as_strided((7, 1, 64), (64, 448, 1))
+    for y, rows in ((apart, 7), (x[:1].as_strided((1, 1, 64), (5, 9, 1)), 1)):
+        assert y.is_contiguous()
+        batch, pbatch = (c.batch(i32([0, rows]), i32([1]), i32([290]), rows=rows) for c in (cache, plain))
+        cache.append(y, y, batch)
+        plain.append(x[:rows], x[:rows], pbatch)
+        assert torch.equal(cache.pool, plain.pool) and torch.equal(cache.attend(y, batch), plain.attend(x[:rows], pbatch))
+
+
 def test_numbers_that_do_not_fit_give_nan_and_store_nothing():
     """The kernels' own checks: nothing outside the buffers is followed, the rows in question are NaN, the others are right."""
     m = _kv4.Model(64, 2, 1, 30, 6, 5, seed=12)
