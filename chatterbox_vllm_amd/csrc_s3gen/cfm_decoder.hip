@@ -480,7 +480,7 @@ __global__ __launch_bounds__(KSPLIT == 8 ? 512 : 256, S3_LIN_OCC(KSPLIT, DEEP, S
 #pragma unroll
     for (int i = 0; i < 16; ++i) { acc0[i] = 0.f; acc1[i] = 0.f; }
     float ln_s1 = 0.f, ln_s2 = 0.f;                            // LN_IN: this lane's share of its frame's sum and sum of squares
-    f32x2 ln_p1 = {0.f, 0.f}, ln_p2 = {0.f, 0.f};              // the split form keeps them in pairs (packed adds and fmas)
+    f32x2 ln_p1 = {0.f, 0.f}, ln_p2 = {0.f, 0.f};              // the split form keeps them in pairs
     // one step of the split form on a lane's eight x values and the two blocks' planes
     auto split_step = [&](const float* bx, bool ok, const u32x4* s0p, const u32x4* s1p) {
         u32x4 P[3];
