@@ -940,9 +940,11 @@ __global__ __launch_bounds__(256, 8) void kv4_finish_kernel(Kv4View c, Kv4Rows b
 }
 
 // Some have not: a workgroup per (page, key head, stream).  A wave keeps the page's keys as operands, takes every fourth column tile
-// (the next one's queries are under way meanwhile) and sums over its tiles and their columns; the waves are added in order.
+// (the next one's queries are under way meanwhile) and sums over its tiles and their columns; the waves are added in order.  At hd 128 two
+// workgroups a CU share its L1 better than the three that the registers leave room for: 2 x 4095 rows x 32 heads with weights 663 us
+// and 713; at hd 64 four are better than two, 4 x 2000 rows x 16 heads 111 and 118.
 template <int HD, bool F16>
-__global__ __launch_bounds__(256, 2) void kv4_weights_kernel(Kv4View c, Kv4Rows b, Kv4Attn a, float* weights, int64_t weights_stride) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, HD == 64 ? 4 : 2))) void kv4_weights_kernel(Kv4View c, Kv4Rows b, Kv4Attn a, float* weights, int64_t weights_stride) {
     __shared__ float part[4][KV4_PAGE];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
     const int h = blockIdx.y, seq = blockIdx.z, p = blockIdx.x, first = p * KV4_PAGE;
