@@ -218,7 +218,7 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4View c, Kv4Rows b, int
 //   T = the largest key with at least `need` candidate keys >= T, found from the highest bit in which they differ down;
 //   what is above T stays, and the first need - |above T| of those equal to it.
 // Bound by the bytes moved: the kept entries lie scattered, so every line of the source is read (8 streams x 30 layers x 16 heads of
-// 64, 1500..2011 entries to 640: 457 MB, with 208 MB written 690 MB in 146 us, 4.7 TB/s; choice and move as two launches 355).  One layer
+// 64, 1500..2011 entries to 640: 457 MB, with 208 MB written 690 MB in 172 us, 4.0 TB/s; choice and move as two launches 355).  One layer
 // of 4 streams x 16 heads is latency, a chain of about eight loads and barriers: 9 us (17.4).
 // ------------------------------------------------------------------------------------------------------------------
 struct Kv4Evict {

@@ -19,10 +19,11 @@
 // walks the cache.  Which form and how many chunks follow from the sequence alone, so a row's bits do not depend on the batch.
 //
 // Few columns are bound by the cache's bytes where there are many (16 x 32 heads on 8 key heads of 128, 9000..32749 entries: 386 MB in
-// 77 us, 5.0 TB/s) and by latency where there are few (64 x 16 heads of 64, 120..1000 entries: 39 MB in 13 us; one stream 5 us).
-// Many are bound by the instructions: matrix and vector instructions of a SIMD do not run beside each other (measured: a 16x16x32
-// product 17.6 clocks, an fma 2.5, an exp2 10, mixed ones the sum), so both count, and the products stand in blocks, each change
-// from one kind to the other costing about 5 clocks.  2 x 4095 rows x 32 heads on 8 of 128: 346 GFLOP in 348 us, 1.0 PFLOP/s.
+// 77 us, 5.0 TB/s) and by latency where there are few (64 x 16 heads of 64, 120..1000 entries: 39 MB in 13.5 us; one stream 5 us).
+// Many are bound by the instructions: matrix and vector instructions of a SIMD hardly run beside each other (measured: a 16x16x32
+// product 17.4 clocks, an fma 2.5, an exp2 9.7, mixed ones six sevenths of the sum or more), so both count, and the products stand in
+// blocks, each change from one kind to the other costing about 5 clocks.  2 x 4095 rows x 32 heads on 8 of 128: 346 GFLOP in 351 us, 0.99
+// PFLOP/s (fp16 rows, whose queries and P are two bf16 parts each: 542 us).
 #include "kv4_common.h"
 
 #include <type_traits>
@@ -622,8 +623,8 @@ template <int HD> struct Kv4Stage {
 };
 
 // The order wanted of a product's block: four fragments read ahead, and one more behind the products of each, so that no product
-// waits for LDS.  Nothing else is put between them: on this chip vector instructions do not run beside matrix ones, of the same or
-// of another wave (17.6 clocks a product, 27.5 with four fmas behind each), and every change from one to the other costs ~5 clocks.
+// waits for LDS.  Nothing else is put between them: on this chip vector instructions hardly run beside matrix ones, of the same or
+// of another wave (17.4 clocks a product, 27.5 with four fmas behind each), and every change from one to the other costs ~5 clocks.
 template <int FRAGMENTS, int PRODUCTS> __device__ __forceinline__ void kv4_interleave() {
     __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);           // LDS reads
 #pragma unroll
@@ -634,8 +635,8 @@ template <int FRAGMENTS, int PRODUCTS> __device__ __forceinline__ void kv4_inter
 }
 
 // Where many workgroups look at each page it is converted once for all of them: a launch before leaves the pages' fragments in memory as
-// they stand in LDS, where loads without a register on the way bring them (2 x 4095 rows x 32 heads of 128 384 us -> 348, of them 12 the
-// conversion; through registers 354).
+// they stand in LDS, where loads without a register on the way bring them (2 x 4095 rows x 32 heads of 128: 36 us less of 384, the 10 us of
+// the conversion counted; through registers 30).
 template <int HD> __device__ __forceinline__ uint8_t* kv4_image(const Kv4Attn& a, int Hkv, int seq, int h, int p) {
     return a.images + (((int64_t)seq * Hkv + h) * a.pages + p) * (256 * HD);
 }
@@ -830,8 +831,8 @@ __global__ __launch_bounds__(256, HD == 64 ? 4 : 2) void kv4_attn_mixed_kernel(K
 // Weights: W[stream][key head][t] += sum over the sequence's columns of exp2((s - m) c) / l.  A workgroup owns its entries and walks the
 // columns in a fixed order, so there are no atomics.  Scores of sequences of few columns were kept by the pass above (64 decode rows x
 // 16 heads of 64 over up to 2000 entries 55 us -> 37, 32 x 64 heads on 8 of 128 over up to 8000 122 -> 74; 40 columns 37 -> 28); the
-// others are formed again from K, from queries that the pass above leaves in operand order (2 x 4095 rows x 32 heads of 128: 280 us
-// beside the pass's 349; from the rows as given 380, by one wave a page 1170).
+// others are formed again from K, from queries that the pass above leaves in operand order (2 x 4095 rows x 32 heads of 128: 312 us
+// beside the pass's 351; from the rows as given 100 us more, by one wave a page 890).
 // A stream that occurs in several sequences of the call is done, in their order, by the waves of the first of them.
 // ------------------------------------------------------------------------------------------------------------------
 // Walks the sequences of the stream of sequence `seq` if that is the first of them, 64 looked at at a time: fn(their numbers).
